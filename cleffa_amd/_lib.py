@@ -16,6 +16,7 @@ VIS_SCRATCH_BYTES = 64 << 20
 BLOCK_Q = 128
 KV_ALIGN = 8
 BLOCK_INTS = 8
+KV8_PAGE, KV8_MAX_SEQ, KV8_MAX_ROWS = 64, 4096, 262143
 
 # Every symbol include/clef_hip_attn.h declares.
 EXPORTS = (
@@ -32,6 +33,7 @@ EXPORTS = (
     "clef_hip_gguf_open", "clef_hip_gguf_close", "clef_hip_gguf_tensor_count", "clef_hip_gguf_tensor_at",
     "clef_hip_gguf_find_tensor", "clef_hip_gguf_get_u32", "clef_hip_gguf_get_f32", "clef_hip_gguf_attn_config",
     "clef_hip_gguf_attn_layer", "clef_hip_gguf_vis_layer",
+    "clef_hip_kv8_sizes", "clef_hip_kv8_plan", "clef_hip_kv8_append", "clef_hip_kv8_attention", "clef_hip_kv8_read",
 )
 
 GGML_F32, GGML_F16, GGML_BF16 = 0, 1, 30
@@ -88,6 +90,36 @@ class OmniAttnArgs(ctypes.Structure):
         ("nh", c_int), ("nkv", c_int), ("T", c_int), ("kvT", c_int), ("scale", c_float),
         ("q_plane", c_void_p), ("k_plane", c_void_p), ("v_plane", c_void_p), ("blocks", c_void_p),
         ("n_blk", c_int), ("out", c_void_p),
+    ]
+
+
+class Kv8PlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", c_int), ("max_pages", c_int), ("n_pages", c_int),
+        ("T", c_int), ("nh", c_int), ("nkv", c_int), ("max_new", c_int),
+        ("tables", c_void_p), ("free_pages", c_void_p), ("state", c_void_p), ("state_out", c_void_p),
+        ("new_lens", c_void_p), ("pos_off", c_void_p), ("cu_q", c_void_p), ("slots", c_void_p), ("pos3", c_void_p),
+        ("plan", c_void_p), ("plan_ints", c_size_t),
+    ]
+
+
+class Kv8Args(ctypes.Structure):
+    _fields_ = [
+        ("nh", c_int), ("nkv", c_int), ("hd", c_int), ("n_rot", c_int), ("eps", c_float), ("scale", c_float),
+        ("T", c_int), ("row", c_int), ("n_seq", c_int), ("max_pages", c_int), ("n_pages", c_int), ("max_new", c_int),
+        ("qkv", c_void_p), ("q_norm", c_void_p), ("k_norm", c_void_p), ("pos3", c_void_p), ("inv_freq", c_void_p),
+        ("tables", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("plan", c_void_p), ("gate", c_int), ("out", c_void_p), ("out_type", c_int), ("f16_lim", c_float),
+        ("ovf", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class Kv8ReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("nkv", c_int), ("hd", c_int), ("n_seq", c_int), ("max_pages", c_int), ("n_pages", c_int), ("kvT", c_int),
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("tables", c_void_p), ("state", c_void_p), ("first_page", c_void_p), ("cu", c_void_p),
+        ("k_plane", c_void_p), ("vt_plane", c_void_p),
     ]
 
 
@@ -174,6 +206,12 @@ def load():
     lib.clef_hip_vis_positions.argtypes = [POINTER(c_int32), c_int, POINTER(c_int32), c_int,
                                            POINTER(c_int32), c_char_p, c_size_t]
     lib.clef_hip_vis_positions.restype = c_bool
+    lib.clef_hip_kv8_sizes.argtypes = [c_int, c_int, c_int, c_int, c_int, POINTER(c_size_t), POINTER(c_size_t), c_char_p, c_size_t]
+    lib.clef_hip_kv8_sizes.restype = c_bool
+    for name, args in (("plan", Kv8PlanArgs), ("append", Kv8Args), ("attention", Kv8Args), ("read", Kv8ReadArgs)):
+        fn = getattr(lib, "clef_hip_kv8_" + name)
+        fn.argtypes = [POINTER(args), c_void_p, c_char_p, c_size_t]
+        fn.restype = c_bool
     for name in ("clef_hip_attn_prep_kv", "clef_hip_attn_core", "clef_hip_attn_prefill"):
         fn = getattr(lib, name)
         fn.argtypes = [POINTER(AttnArgs), c_void_p, c_char_p, c_size_t]

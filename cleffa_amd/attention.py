@@ -70,6 +70,26 @@ def _stream_handle(stream):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+class _on:
+    """The stream handle to launch on for a device: the given stream's, or the device's current stream, with that
+    device current for the time of the call (another one's stream would take its launches elsewhere)."""
+
+    def __init__(self, device, stream):
+        if device.type != "cuda":
+            raise RuntimeError(f"hip: the call needs tensors on a GPU, not on {device}")
+        self.device, self.stream, self.before = device, stream, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.device.index:
+            self.before = torch.cuda.current_device()
+            torch.cuda.set_device(self.device)
+        return _stream_handle(self.stream)
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
 _initialised = set()
 
 
@@ -362,6 +382,57 @@ class TextAttention:
                                                  _ptr(plan.tok_kv) if prologue else None,
                                                  _stream_handle(stream), err, len(err)), err)
         return qkv
+
+
+    def forward_kv8(self, qkv, q_norm, k_norm, pos3, plan, cache, layer=0, out=None, out_dtype="bf16", gate=True, ovf=None,
+                    f16_lim=65504.0, stream=None, stage="prefill"):
+        """One layer's attention of a planned pass over an 8-bit paged cache (kv8_cache.Kv8Cache, Kv8Plan): the new
+        tokens' keys and values are appended to layer ``layer``'s pages, and their queries attend to all keys of
+        their sequences. qkv [T][row] bf16, pass rows in the plan's order (plan.cu_q); pos3 [T][3], the plan's own
+        or the caller's. Rows behind the last sequence are left out: their outputs stay as they were. stage:
+        "prefill" (append and attention), "append", or "core" (attention alone). Returns out (None for "append")."""
+        dev, T = self.device, plan.T
+        if plan.cache is not cache:
+            raise ValueError("the plan belongs to another cache")
+        if (plan.nh, cache.nkv, cache.hd) != (self.nh, self.nkv, self.hd) or cache.device != dev:
+            raise ValueError("cache and plan do not fit the layer's heads or device")
+        if stage not in ("prefill", "append", "core"):
+            raise ValueError(f"stage {stage!r}")
+        cache.check_layer(layer)
+        _check(qkv, "qkv", (T, qkv.shape[1] if qkv.dim() == 2 else -1), torch.bfloat16, dev)
+        if qkv.shape[1] < self.row or qkv.shape[1] % 8:
+            raise ValueError(f"qkv row {qkv.shape[1]} must be >= {self.row} and a multiple of 8")
+        if (q_norm is None) != (k_norm is None):
+            raise ValueError("q_norm and k_norm must both be given or both be None")
+        if q_norm is not None:
+            _check(q_norm, "q_norm", (self.hd,), torch.float32, dev)
+            _check(k_norm, "k_norm", (self.hd,), torch.float32, dev)
+        if self.n_rot:
+            _check(pos3, "pos3", (T, 3), torch.int32, dev)
+        if ovf is not None:
+            _check(ovf, "ovf", (T,), torch.int32, dev)
+        out_type, odt = _OUT_TYPES[out_dtype]
+        if stage != "append":
+            if out is None:
+                out = torch.empty((T, self.nh * self.hd), dtype=odt, device=dev)
+            _check(out, "out", (T, self.nh * self.hd), odt, dev)
+        a = _lib.Kv8Args()
+        a.nh, a.nkv, a.hd, a.n_rot, a.eps, a.scale = self.nh, self.nkv, self.hd, self.n_rot, self.eps, self.scale
+        a.T, a.row = T, qkv.shape[1]
+        a.n_seq, a.max_pages, a.n_pages, a.max_new = cache.max_seqs, cache.max_pages, cache.n_pages, plan.max_new
+        a.qkv, a.q_norm, a.k_norm, a.pos3, a.inv_freq = _ptr(qkv), _ptr(q_norm), _ptr(k_norm), _ptr(pos3), _ptr(self.inv_freq)
+        a.tables, a.plan = _ptr(cache.tables), _ptr(plan.work)
+        a.k_pages, a.v_pages = _ptr(cache.k[layer]), _ptr(cache.v[layer])
+        a.k_scale, a.v_scale = _ptr(cache.k_scale[layer]), _ptr(cache.v_scale[layer])
+        a.gate, a.out, a.out_type, a.f16_lim, a.ovf = int(gate), _ptr(out) if stage != "append" else None, out_type, f16_lim, _ptr(ovf)
+        a.workspace, a.workspace_bytes = _ptr(plan.workspace), plan.workspace.numel()
+        lib, err = _lib.load(), _err()
+        with _on(dev, stream) as s:
+            if stage != "core":
+                _lib.check(lib.clef_hip_kv8_append(ctypes.byref(a), s, err, len(err)), err)
+            if stage != "append":
+                _lib.check(lib.clef_hip_kv8_attention(ctypes.byref(a), s, err, len(err)), err)
+        return out if stage != "append" else None
 
 
 class VisionAttention:

@@ -6,14 +6,16 @@ from pathlib import Path
 ROOT = Path(__file__).resolve().parent
 REPO = ROOT.parent
 LIB = ROOT / "libclef_hip_attn.so"
-SOURCES = [ROOT / "csrc" / "attn_api.hip", ROOT / "csrc" / "prefix_cache.hip", ROOT / "csrc" / "omni_api.hip", ROOT / "csrc" / "records.cpp",
+SOURCES = [ROOT / "csrc" / "attn_api.hip", ROOT / "csrc" / "prefix_cache.hip", ROOT / "csrc" / "omni_api.hip",
+           ROOT / "csrc" / "kv8_api.hip", ROOT / "csrc" / "records.cpp",
            ROOT / "csrc" / "gemm_api.cpp", ROOT / "csrc" / "gguf_layer.cpp"]
 # the measurement utility bench.py uses, kept out of the engine-facing library
 BENCH_LIB = ROOT / "libclef_hip_bench.so"
 BENCH_SOURCES = [ROOT / "csrc" / "mfma_ceiling.hip"]
 DEPS = SOURCES + BENCH_SOURCES + [ROOT / "csrc" / "attn_kernels.h", ROOT / "csrc" / "attn_params.h", ROOT / "csrc" / "attn_text.h",
                   ROOT / "csrc" / "attn_vis.h", ROOT / "csrc" / "omni_attn.h", ROOT / "csrc" / "attn_text_f32.h", ROOT / "csrc" / "bf16_ops.h", ROOT / "csrc" / "split32.h",
-                  ROOT / "csrc" / "gemm_kernel.h", ROOT / "csrc" / "kv_rows.h", ROOT / "csrc" / "gguf_view.h",
+                  ROOT / "csrc" / "gemm_kernel.h", ROOT / "csrc" / "kv_rows.h", ROOT / "csrc" / "text_ops.h",
+                  *(ROOT / "csrc" / f"kv8_{part}.h" for part in ("attn", "pages", "params", "plan")), ROOT / "csrc" / "gguf_view.h",
                   REPO / "include" / "clef_hip_attn.h"]
 
 

@@ -55,21 +55,6 @@ __device__ __forceinline__ int s_row_key(int kt, int r) {
 __device__ __forceinline__ int k_swz(int key) { return (key & 15) ^ ((key >> 4) << 2); }
 // XOR swizzle of a V^T row's chunks (rows of 8 chunks, two rows per 256-byte bank line)
 __device__ __forceinline__ int v_swz(int d) { return ((d >> 1) & 1) | (((d >> 3) & 3) << 1); }
-// Sum / max over the four 16-lane rows of a wave (v_permlane16_swap / v_permlane32_swap, VALU
-// only, so no LDS traffic). Every lane gets the same bits.
-__device__ __forceinline__ float xrow_max(float x) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-}
-__device__ __forceinline__ float xrow_sum(float x) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float m = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
-}
-
 // LDS operand reads issued as ds_read_b128 with an explicit lgkmcnt wait per use. The compiler
 // would otherwise wait for every outstanding LDS access (lgkmcnt(0)) before each use while the
 // global_load_lds fills of the other buffer are in flight. lds_wait ties the wait to the value

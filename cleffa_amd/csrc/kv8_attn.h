@@ -1,0 +1,349 @@
+// Grouped-query attention of a pass's new tokens over the 8-bit paged cache, with the Q prologue
+// (RMSNorm, rotary) and the sigmoid gate fused in.
+//
+// Rows are (token, q head of the kv group), token-major, so that the q heads that share a kv head share its
+// pages: one token of 24/4 heads is 6 rows of a 16-row matrix tile. Per 16-row tile and 64-token page
+//   S^T = K . Q^T     v_mfma_f32_16x16x32_f16: A = K codes as f16 (exact), B = Q (f16)
+//   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16: A = V codes as bf16 (exact), B = P * 2^ev (bf16)
+// The page's K scale multiplies the f32 scores together with the softmax scale; its V scale 2^ev goes into the
+// exponent of P, so neither costs an instruction per element. Row r of A tile t (of four that make up 64
+// rows) is token / dim 16 (r / 4) + 4 t + r % 4: then a lane's 16 scores of a page are 16 consecutive tokens,
+// which are the k indexes of the next product's B operand with no exchange, and its 16 outputs of a dim
+// group are consecutive dims. A lane reads 16-byte pieces (row, 16 dims or tokens) of the page, each two
+// operands' worth.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "bf16_ops.h"
+#include "kv8_pages.h"
+#include "kv8_params.h"
+#include "text_ops.h"
+
+namespace clef_hip {
+namespace kv8 {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+constexpr float kNone = -1e30f;   // a running maximum before any key: below every score, and finite
+
+__device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
+    const f16x2 x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false), y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
+    const f16x2 z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
+    return f16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+__device__ __forceinline__ bf16x8 codes_bf16(unsigned a, unsigned b) {
+    const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
+    const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
+    return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+
+// One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
+// 2c (e < 8) and 2c + 1. Norm and rotary in f32; f16 with split16's saturation (flagged).
+__device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, f16x8 (&q)[8], int32_t *flag) {
+    const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 16 * g;
+    float x[4][16];
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const u32x4 a = *(const u32x4 *)(src + 64 * c), b = *(const u32x4 *)(src + 64 * c + 8);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[c][2 * i] = bf_lo(a[i]);
+            x[c][2 * i + 1] = bf_hi(a[i]);
+            x[c][8 + 2 * i] = bf_lo(b[i]);
+            x[c][9 + 2 * i] = bf_hi(b[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) ss += x[c][i] * x[c][i];
+    }
+    if (p.q_norm) {
+        const float inv = rsqrtf(text::xrow_sum(ss) / (float)HD + p.eps);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[c][i] *= inv * p.q_norm[64 * c + 16 * g + i];
+    }
+    if (p.n_rot) {   // dims 16g + e of the first 64: pair (16g + e) % 32, whose other half is lane g ^ 2
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int i = (16 * g + e) & 31;
+            float sn, cn;
+            rope_sincos((float)p.pos3[3 * (size_t)t + i % 3] * p.inv_freq[i], &sn, &cn);
+            const float other = __shfl_xor(x[0][e], 32);
+            x[0][e] = g < 2 ? x[0][e] * cn - other * sn : x[0][e] * cn + other * sn;
+        }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            bad |= saturate(x[c][i], p.f16_lim);
+            q[2 * c + (i >> 3)][i & 7] = (_Float16)x[c][i];
+        }
+    if (bad && flag) __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Sixteen finished outputs (dims d0 ..) of a row: times the gate's sigmoid, converted and stored.
+__device__ __forceinline__ void finish16(const Params &p, int t, int head, int d0, float (&o)[16], int32_t *flag) {
+    if (p.gate) {
+        const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + d0;
+        const u32x4 a = *(const u32x4 *)src, b = *(const u32x4 *)(src + 8);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            o[2 * i] *= sigmoidf(bf_lo(a[i]));
+            o[2 * i + 1] *= sigmoidf(bf_hi(a[i]));
+            o[8 + 2 * i] *= sigmoidf(bf_lo(b[i]));
+            o[9 + 2 * i] *= sigmoidf(bf_hi(b[i]));
+        }
+    }
+    const size_t idx = ((size_t)t * p.nh + head) * HD + d0;
+    store_out8(p.out, idx, o, p.out_type, p.f16_lim, flag);
+    store_out8(p.out, idx + 8, o + 8, p.out_type, p.f16_lim, flag);
+}
+
+// Partial results of a cut block: [split slot][kv head][row][256] unnormalised outputs, then
+// [split slot][kv head][row][2] running maximum (log2 units) and sum.
+__device__ __forceinline__ size_t partial_row(const Params &p, int slot, int kh, int row) {
+    return ((size_t)slot * p.nkv + kh) * p.l.bm + row;
+}
+__device__ __forceinline__ float *partial_ml(const Params &p) {
+    return p.partial + (size_t)p.l.max_slots * p.nkv * p.l.bm * HD;
+}
+
+// Few rows (decoding): a workgroup takes an item's 16 MT rows over its pages, wave w the pages w, w + 4, ...
+// Each wave reads its pages straight into registers, all of one page's K and V ahead of their use, so 32 KB
+// per wave are in flight; the four waves' results join through LDS.
+constexpr int kRowsThreads = 256, kRowsWaves = 4;
+template <int MT>
+__global__ __launch_bounds__(kRowsThreads) void kv8_attn_rows_kernel(Params p) {
+    constexpr int BM = 16 * MT, OS = HD + 4;   // LDS row stride of the outputs
+    __shared__ float os[kRowsWaves][16][OS], ml[kRowsWaves][BM][2];
+    const int32_t *h = p.plan;
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm)) return;
+    const int units = h[H_ITEMS] * p.nkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q16 = lane & 15, g = lane >> 4;
+    const int lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;   // the lane's piece of tile 0
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int item = u / p.nkv, kh = u - item * p.nkv;
+        const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
+        const int4 e0 = it[0], e1 = it[1];
+        const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
+        const int pg0 = e1.z, pg1 = e1.w;
+        const int32_t *table = p.tables + (size_t)seq * p.max_pages;
+        u32x4 kr[16], vr[16];
+        auto base = [&](int pg) {
+            const unsigned id = (unsigned)table[pg];
+            return ((size_t)(id < (unsigned)p.n_pages ? id : 0u) * p.nkv + kh);
+        };
+        auto load = [&](u32x4 (&r)[16], const uint8_t *pages, size_t at) {
+            const uint8_t *src = pages + at * PAGE_BYTES + lofs;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) r[4 * c + t] = *(const u32x4 *)(src + 4096 * c + 256 * t);
+        };
+        size_t at = 0;
+        float ks = 0.f, vs = 0.f;
+        if (pg0 + wave < pg1) {
+            at = base(pg0 + wave);
+            load(kr, p.k_pages, at);
+            load(vr, p.v_pages, at);
+            ks = p.k_scale[at];
+            vs = p.v_scale[at];
+        }
+        f16x8 q[MT][8];
+        int last[MT];   // the last key the lane's row sees
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int fr = row0 + min(16 * m + q16, rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
+            load_q(p, q0 + t, head, g, q[m], p.ovf ? p.ovf + q0 : nullptr);
+            last[m] = L + t;
+        }
+        f32x4 o[MT][16];
+        float mx[MT], sum[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            mx[m] = kNone;
+            sum[m] = 0.f;
+#pragma unroll
+            for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int pg = pg0 + wave; pg < pg1; pg += kRowsWaves) {
+            const bool more = pg + kRowsWaves < pg1;
+            f32x4 s[MT][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int m = 0; m < MT; m++) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const u32x4 w = kr[4 * c + t];
+                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * c], s[m][t], 0, 0, 0);
+                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, q[m][2 * c + 1], s[m][t], 0, 0, 0);
+                    }
+                }
+            }
+            const float kf = ks * p.scale_log2;
+            const int ev = (int)(__float_as_uint(vs) >> 23) - 127;   // vs = 2^ev
+            size_t next = 0;
+            if (more) {
+                next = base(pg + kRowsWaves);
+                load(kr, p.k_pages, next);
+                ks = p.k_scale[next];
+                vs = p.v_scale[next];
+            }
+            // keys behind the last one hold whatever the page held: their scores and V codes are cut off
+            const int key0 = pg * PAGE + 16 * g;
+            bf16x8 pb[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                if ((pg + 1) * PAGE > L + 1) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (key0 + 4 * t + i > last[m]) s[m][t][i] = -INFINITY;
+                }
+                float top = s[m][0][0];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[m][t][i]);
+                const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
+                const float f = __builtin_amdgcn_exp2f(mx[m] - now);
+                mx[m] = now;
+                float add = 0.f;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][i], kf, -now));
+                        add += x;
+                        pb[m][t >> 1][4 * (t & 1) + i] = (__bf16)ldexpf(x, ev);
+                    }
+                sum[m] = sum[m] * f + add;
+#pragma unroll
+                for (int d = 0; d < 16; d++) o[m][d] *= f;
+            }
+            if ((pg + 1) * PAGE > n_keys) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int v = n_keys - key0 - 4 * w;   // valid bytes of the word
+                    const unsigned keep = v >= 4 ? ~0u : v <= 0 ? 0u : (1u << 8 * v) - 1;
+#pragma unroll
+                    for (int d = 0; d < 16; d++) vr[d][w] &= keep;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 16; d++) {
+                const u32x4 w = vr[d];
+                const bf16x8 a = codes_bf16(w[0], w[1]), b = codes_bf16(w[2], w[3]);
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[m][0], o[m][d], 0, 0, 0);
+                    o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, pb[m][1], o[m][d], 0, 0, 0);
+                }
+            }
+            if (more) load(vr, p.v_pages, next);
+        }
+        // join the waves: each scales its outputs to the common maximum
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            sum[m] = text::xrow_sum(sum[m]);
+            if (g == 0) {
+                ml[wave][16 * m + q16][0] = mx[m];
+                ml[wave][16 * m + q16][1] = sum[m];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            float top = kNone;
+#pragma unroll
+            for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][16 * m + q16][0]);
+            const float f = __builtin_amdgcn_exp2f(mx[m] - top);
+#pragma unroll
+            for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
+            __syncthreads();
+            const int r = tid >> 4, d0 = 16 * (tid & 15), row = 16 * m + r;
+            if (row < rows) {
+                float x[16], l = 0.f;
+                float mrow = kNone;
+#pragma unroll
+                for (int w = 0; w < kRowsWaves; w++) mrow = fmaxf(mrow, ml[w][row][0]);
+#pragma unroll
+                for (int w = 0; w < kRowsWaves; w++) l += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - mrow);
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] = os[0][r][d0 + i] + os[1][r][d0 + i] + os[2][r][d0 + i] + os[3][r][d0 + i];
+                if (slot < 0) {
+                    const int fr = row0 + row, t = fr / p.group, head = kh * p.group + fr - t * p.group;
+                    const float inv = 1.f / l;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[i] *= inv;
+                    finish16(p, q0 + t, head, d0, x, p.ovf ? p.ovf + q0 : nullptr);
+                } else {
+                    const size_t pr = partial_row(p, slot, kh, row);
+                    float *dst = p.partial + pr * HD + d0;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) *(f32x4 *)(dst + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+                    if ((tid & 15) == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Joins the items of cut blocks. Workgroup unit (pass row, q head): wave w takes items w, w + 4, ..., a lane
+// four dims; the items are added in a fixed order, so results do not change from run to run.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64;
+__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
+    __shared__ float os[kJoinWaves][HD], ls[kJoinWaves];
+    const int32_t *h = p.plan;
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || h[H_SPLIT] == 0) return;
+    const int units = h[H_TOKENS] * p.nh, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int t = u / p.nh, head = u - t * p.nh, kh = head / p.group;
+        const int2 tok = ((const int2 *)(p.plan + p.l.tok))[t];
+        const int fr = tok.y * p.group + head - kh * p.group, b = tok.x + fr / p.l.bm;
+        const int4 blk = ((const int4 *)(p.plan + p.l.blk))[b];
+        const int n = blk.y, row = fr - blk.z;
+        if (n <= 1) continue;   // the whole workgroup skips it
+        const int q0 = t - tok.y;
+        const float *ml = partial_ml(p);
+        float top = kNone;
+        for (int k = lane; k < n; k += 64) top = fmaxf(top, ml[2 * partial_row(p, blk.w + k, kh, row)]);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll 4
+        for (int k = wave; k < n; k += kJoinWaves) {
+            const size_t pr = partial_row(p, blk.w + k, kh, row);
+            const float2 e = *(const float2 *)(ml + 2 * pr);
+            const f32x4 x = *(const f32x4 *)(p.partial + pr * HD + 4 * lane);
+            const float f = __builtin_amdgcn_exp2f(e.x - top);
+            l += e.y * f;
+            o += x * f;
+        }
+        *(f32x4 *)&os[wave][4 * lane] = o;
+        if (lane == 0) ls[wave] = l;
+        __syncthreads();
+        if (tid < 16) {
+            float x[16];
+            const float inv = 1.f / (ls[0] + ls[1] + ls[2] + ls[3]);
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = (os[0][16 * tid + i] + os[1][16 * tid + i] + os[2][16 * tid + i] + os[3][16 * tid + i]) * inv;
+            finish16(p, t, head, 16 * tid, x, p.ovf ? p.ovf + q0 : nullptr);
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace kv8
+}  // namespace clef_hip

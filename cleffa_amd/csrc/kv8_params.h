@@ -1,0 +1,90 @@
+// The 8-bit paged prefix cache: its formats, the pass plan's layout and the kernels' argument
+// blocks (internal; the interface is documented in include/clef_hip_attn.h).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "clef_hip_attn.h"
+
+namespace clef_hip {
+namespace kv8 {
+
+constexpr int HD = 256;                        // head dim
+constexpr int PAGE = CLEF_HIP_KV8_PAGE;        // tokens per page
+constexpr int PAGE_BYTES = PAGE * HD;          // codes of one page and kv head, K or V
+constexpr int kMaxSeq = CLEF_HIP_KV8_MAX_SEQ;
+constexpr int kMaxRows = CLEF_HIP_KV8_MAX_ROWS;
+constexpr int kMaxTablePages = 1 << 16;        // entries of a table row: token indexes stay below 2^22
+constexpr int kMaxGroup = 128;                 // q heads per kv head
+constexpr int32_t kPlanMagic = 0x4b563850;     // 'KV8P'
+
+// Plan header words. A failed plan leaves counts of 0, so the kernels that follow do nothing.
+enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_ITEMS, H_BLOCKS, H_SPLIT, H_WORDS = 16 };
+
+// Where the parts of a plan buffer lie (in int32) and how many entries each can need:
+//  append items {page, pass row of its first new token, slot of that token in the page | count << 8, first
+//  pass row of its sequence}, one for each page that a sequence's new tokens touch: at most one per
+//  token and (n - 1) / 64 + 2 per sequence of n;
+//  token entries {first block of the token's sequence, index in the sequence};
+//  block entries {first item, items, first row, split slot of the first item}: BM rows of a sequence,
+//  a row being one q head of the kv group for one token (token-major);
+//  attention items {sequence, its first pass row, its cached tokens, its keys, first row, rows |
+//  (split slot + 1) << 8, first page, end page}: a block's rows over a run of its pages.
+// A block of p pages is cut when p exceeds the chunk C = max(least, ceil(W / budget)), W the pages of
+// all blocks: ceil(p / C) < p / C + 1, so items <= blocks + budget, and items of cut blocks (split
+// slots) < 2 W / C <= 2 budget.
+struct Layout {
+    int bm, budget, least, max_app, max_blk, max_items, max_slots;
+    long app, tok, blk, items, ints;
+    size_t ws_bytes;
+};
+inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
+    Layout l;
+    const int G = nh / nkv;
+    const long rows = (long)(max_new > 0 && max_new < T ? max_new : T) * G;
+    l.bm = rows <= 16 ? 16 : 32;
+    l.budget = (2 * n_cu + nkv - 1) / nkv;
+    l.least = 4;
+    const long app = (long)T / PAGE + 2L * n_seq;
+    l.max_app = (int)(app < T ? app : T);
+    l.max_blk = (int)((long)T * G / l.bm) + (n_seq < T ? n_seq : T);
+    l.max_items = l.max_blk + l.budget;
+    l.max_slots = 2 * l.budget;
+    l.app = H_WORDS;
+    l.tok = l.app + 4L * l.max_app;
+    l.blk = (l.tok + 2L * T + 3) / 4 * 4;
+    l.items = (l.blk + 4L * l.max_blk + 7) / 8 * 8;
+    l.ints = l.items + 8L * l.max_items;
+    l.ws_bytes = (size_t)l.max_slots * nkv * l.bm * (HD + 2) * sizeof(float);
+    return l;
+}
+
+struct PlanParams {
+    int n_seq, max_pages, n_pages, T, group;
+    Layout l;
+    int32_t *tables, *free_pages;
+    const int32_t *state, *new_lens, *pos_off;
+    int32_t *state_out, *cu_q, *slots, *pos3, *work;
+};
+
+struct Params {
+    const uint16_t *qkv;
+    const float *q_norm, *k_norm, *inv_freq;
+    const int32_t *pos3, *tables, *plan;
+    uint8_t *k_pages, *v_pages;
+    float *k_scale, *v_scale, *partial;
+    void *out;
+    int32_t *ovf;
+    int nh, nkv, group, n_rot, row, T, n_seq, max_pages, n_pages, gate, out_type;
+    float eps, scale_log2, f16_lim;
+    Layout l;
+};
+
+// A plan is run only with the sizes it was made for.
+__device__ __forceinline__ bool plan_fits(const int32_t *h, int n_seq, int T, int group, int bm) {
+    return h[H_MAGIC] == kPlanMagic && h[H_SEQ] == n_seq && h[H_ROWS] == T && h[H_GROUP] == group && h[H_BM] == bm;
+}
+
+}  // namespace kv8
+}  // namespace clef_hip

@@ -388,6 +388,111 @@ bool clef_hip_prefix_copy(const uint16_t *k_src, const uint16_t *vt_src, int src
                           uint16_t *k_dst, uint16_t *vt_dst, int dst_cap, int nkv, int hd, int keep,
                           void *stream, char *err, size_t errlen);
 
+/* ---- 8-bit paged prefix cache. No reference counterpart: the reference's entries are 16-bit planes
+ * that grow by copying (above), and a prefix request runs alone against one of them. Here keys and
+ * values are held as e4m3 codes in pages of CLEF_HIP_KV8_PAGE tokens, which sequences take from one
+ * pool, so that many sequences continue in one pass, a sequence grows without a copy, and a token
+ * takes half the memory. A pass is planned on the device from the sequences' lengths, so a serving
+ * loop can be captured into a graph: plan, then per layer append and attention.
+ *
+ * Per layer:
+ *   K pages [n_pages][nkv][4][64][64] (dim group of 64, token, dim), V pages [n_pages][nkv][256][64]
+ *   (dim, token): OCP e4m3 codes; k_scale, v_scale [n_pages][nkv] f32. value = code * scale. A scale
+ *   is 2^e, e the least integer from -64 on with max|x| <= 448 * 2^e over the page's tokens; it does not
+ *   shrink while tokens are appended. Where it has to grow, the page's older codes are rounded again
+ *   (exact but for codes that become subnormal).
+ * For all layers:
+ *   tables [n_seq][max_pages] int32: the pages of each sequence, in token order.
+ *   free_pages [n_pages] int32: a stack of free pages, entry 0 at the bottom.
+ *   state [2 + 2 n_seq] int32: {free pages on the stack, status of the last plan, then tokens and
+ *   pages held of each sequence}. A caller may lower a sequence's tokens (a new request that shares only
+ *   part of a cached text); its pages stay with it. Pages that several table rows share may be read, not
+ *   appended to or released. */
+#define CLEF_HIP_KV8_PAGE 64
+#define CLEF_HIP_KV8_MAX_SEQ 4096     /* sequences of a table */
+#define CLEF_HIP_KV8_MAX_ROWS 262143  /* rows of a pass */
+/* status of a plan, a sum of */
+#define CLEF_HIP_KV8_NO_PAGES 1   /* too few free pages */
+#define CLEF_HIP_KV8_ROWS 2       /* more new tokens than the pass has rows */
+#define CLEF_HIP_KV8_TOO_LONG 4   /* a sequence would pass max_pages pages */
+#define CLEF_HIP_KV8_BAD_STATE 8  /* lengths, counts or page numbers that cannot be */
+
+/* The int32 of a plan buffer and the bytes of an attention workspace for passes of T rows over a table
+ * of n_seq sequences. max_new: the most new tokens of a sequence in such a pass, or 0 if that is not
+ * known; it selects the attention's form (any pass runs, one of longer runs than max_new more slowly).
+ * nkv at most 1024, nh / nkv at most 128. Either output may be NULL. */
+bool clef_hip_kv8_sizes(int n_seq, int T, int nh, int nkv, int max_new, size_t *plan_ints, size_t *workspace_bytes,
+                        char *err, size_t errlen);
+
+/* Plans a pass on the device. new_lens [n_seq]: new tokens of each sequence (0: it rests; -1 or less:
+ * it has ended, and its pages go back on the stack before any are taken). A sequence of L tokens, h pages
+ * and n new tokens takes max(0, ceil((L + n) / 64) - h) pages off the stack, sequences in order. Writes
+ *   state_out: the state after the pass (may be state itself; tables and free_pages are always
+ *   changed in place, so a plan made again from the same state, with other memory for state_out, does the same);
+ *   cu_q [n_seq + 1]: the pass rows of each sequence's new tokens;
+ *   slots [T]: page * 64 + token in page of each pass row, -1 behind the last sequence's rows;
+ *   pos3 [T][3] (or NULL): text positions, the token's index in its sequence + pos_off[sequence]
+ *   (pos_off NULL: 0) in all three; 0 behind the last sequence's rows;
+ *   plan: the work lists of the append and attention kernels (opaque).
+ * All or nothing: where status (state_out[1]) is not 0, state_out is the state otherwise unchanged, no
+ * page has changed hands, cu_q is 0, slots -1, and append and attention with this plan do nothing. */
+typedef struct {
+    int n_seq, max_pages, n_pages;   /* max_pages at most 65,536 */
+    int T, nh, nkv, max_new;
+    int32_t *tables, *free_pages;
+    const int32_t *state;
+    int32_t *state_out;
+    const int32_t *new_lens, *pos_off;
+    int32_t *cu_q, *slots, *pos3;
+    int32_t *plan;                   /* [plan_ints], 16-byte aligned */
+    size_t plan_ints;                /* at least clef_hip_kv8_sizes' */
+} clef_hip_kv8_plan_args;
+bool clef_hip_kv8_plan(const clef_hip_kv8_plan_args *a, void *stream, char *err, size_t errlen);
+
+/* One full-attention layer of a planned pass. n_seq, T, nh, nkv and max_new are the plan's (a plan made for
+ * others is not run: nothing is written). */
+typedef struct {
+    int nh, nkv, hd, n_rot;   /* hd 256; n_rot 64 or 0 */
+    float eps, scale;
+    int T, row;               /* pass rows; qkv row stride in elements (multiple of 8) */
+    int n_seq, max_pages, n_pages, max_new;
+    const uint16_t *qkv;      /* [T][row] bf16, as in clef_hip_attn_args */
+    const float *q_norm, *k_norm;   /* [hd] f32, or both NULL */
+    const int32_t *pos3;      /* [T][3] */
+    const float *inv_freq;    /* [n_rot / 2] */
+    const int32_t *tables;
+    uint8_t *k_pages, *v_pages;
+    float *k_scale, *v_scale;
+    const int32_t *plan;
+    int gate;
+    void *out;                /* [T][nh*hd]; rows behind the last sequence are left as they are */
+    int out_type;             /* CLEF_HIP_OUT_*; f32 is a store width */
+    float f16_lim;            /* as in clef_hip_attn_args: a query, key or value element with |x| > f16_lim
+                                 or NaN is taken as +-65504 and flags its record, and so does an f16 output */
+    int32_t *ovf;             /* [T] flags at each sequence's first pass row, or NULL */
+    void *workspace;          /* attention only; calls that overlap need one each */
+    size_t workspace_bytes;
+} clef_hip_kv8_args;
+/* The new tokens' keys (RMSNorm, rotary) and values into the pages that the plan names. Rows of a page
+ * that hold no token of its sequence are left as they are. */
+bool clef_hip_kv8_append(const clef_hip_kv8_args *a, void *stream, char *err, size_t errlen);
+/* Causal attention of the new tokens over their sequences' pages (their own keys appended before), Q
+ * prologue and gate fused: out = softmax(scale q k^T) v * sigmoid(gate). */
+bool clef_hip_kv8_attention(const clef_hip_kv8_args *a, void *stream, char *err, size_t errlen);
+
+/* Pages back into 16-bit planes, K [nkv][kvT][hd] f16 (the one value beyond f16, 65536, becomes 65504) and
+ * V^T [nkv][hd][kvT] bf16, as a prefix pass of clef_hip_attn_prefill takes them: sequence r's tokens from
+ * page first_page[r] on (NULL: 0) go to plane rows cu[r] .. cu[r + 1] (device int32 [n_seq + 1],
+ * ascending multiples of 8 up to kvT), as many as it has and the rows hold. Other rows are left as they are. */
+typedef struct {
+    int nkv, hd, n_seq, max_pages, n_pages, kvT;
+    const uint8_t *k_pages, *v_pages;
+    const float *k_scale, *v_scale;
+    const int32_t *tables, *state, *first_page, *cu;
+    uint16_t *k_plane, *vt_plane;
+} clef_hip_kv8_read_args;
+bool clef_hip_kv8_read(const clef_hip_kv8_read_args *a, void *stream, char *err, size_t errlen);
+
 /* Host-only producers of the path's inputs. */
 
 /* M-RoPE positions pos3 [T][3] of one record (clef_record.c:938-962, clef_record_positions).
