@@ -132,9 +132,8 @@ bool clef_hip_kv8_attention(const clef_hip_kv8_args *a, void *stream, char *err,
     kv8::Params p;
     if (!fill(a, true, &p, err, errlen)) return false;
     if (a->T == 0) return true;
-    // persistent grids: the plan's counts are on the device
-    const long units = (long)p.l.max_items * p.nkv;
-    const unsigned grid = (unsigned)(units < 2L * kCus ? units : 2L * kCus);
+    // a workgroup for every item the plan may hold: the plan's counts are on the device
+    const unsigned grid = (unsigned)(p.l.max_items * p.nkv);
     if (p.l.bm == 16) hipLaunchKernelGGL(kv8::kv8_attn_rows_kernel<1>, dim3(grid), dim3(kv8::kRowsThreads), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL(kv8::kv8_attn_rows_kernel<2>, dim3(grid), dim3(kv8::kRowsThreads), 0, (hipStream_t)stream, p);
     if (!launch_ok("kv8_attn", err, errlen)) return false;

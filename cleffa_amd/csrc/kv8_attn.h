@@ -4,9 +4,12 @@
 // Rows are (token, q head of the kv group), token-major, so that the q heads that share a kv head share its
 // pages: one token of 24/4 heads is 6 rows of a 16-row matrix tile. Per 16-row tile and 64-token page
 //   S^T = K . Q^T     v_mfma_f32_16x16x32_f16: A = K codes as f16 (exact), B = Q (f16)
-//   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16: A = V codes as bf16 (exact), B = P * 2^ev (bf16)
-// The page's K scale multiplies the f32 scores together with the softmax scale; its V scale 2^ev goes into the
-// exponent of P, so neither costs an instruction per element. Row r of A tile t (of four that make up 64
+//   O^T += V^T . P^T  v_mfma_f32_16x16x32_f16: A = V codes as f16 (exact), B = 2^15 P (f16)
+// The page's K scale multiplies the f32 scores together with the softmax scale, at no cost per element. The
+// accumulated O is kept in units of the current page's V scale times 2^-15: where that changes, so does the factor
+// that rescales O for a new maximum. P in f16 rounds by 2^-11 of itself (bf16: 2^-8); 2^15 P keeps that down
+// to P = 2^-29, and what falls below 2^-40 of the row's largest weight is lost. Units of 2^-64 to 2^8 leave O
+// within 2^113 and 2^-100. Row r of A tile t (of four that make up 64
 // rows) is token / dim 16 (r / 4) + 4 t + r % 4: then a lane's 16 scores of a page are 16 consecutive tokens,
 // which are the k indexes of the next product's B operand with no exchange, and its 16 outputs of a dim
 // group are consecutive dims. A lane reads 16-byte pieces (row, 16 dims or tokens) of the page, each two
@@ -31,27 +34,39 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
     const f16x2 z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
     return f16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
-__device__ __forceinline__ bf16x8 codes_bf16(unsigned a, unsigned b) {
-    const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
-    const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
-    return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
-}
-
 // One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
-// 2c (e < 8) and 2c + 1. Norm and rotary in f32; f16 with split16's saturation (flagged).
-__device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, f16x8 (&q)[8], int32_t *flag) {
+// 2c (e < 8) and 2c + 1. Two steps, so that other loads can go out between them: the row as it is, then norm and
+// rotary in f32 and f16 with split16's saturation (flagged).
+struct QRow {
+    u32x4 w[8];
+    float pos[3];
+};
+__device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, QRow &r) {
     const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 16 * g;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        r.w[2 * c] = *(const u32x4 *)(src + 64 * c);
+        r.w[2 * c + 1] = *(const u32x4 *)(src + 64 * c + 8);
+    }
+    if (p.n_rot)
+#pragma unroll
+        for (int i = 0; i < 3; i++) r.pos[i] = (float)p.pos3[3 * (size_t)t + i];
+}
+__device__ __forceinline__ float other_half(float x) {   // lane ^ 32's value
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f16x8 (&q)[8], int32_t *flag) {
     float x[4][16];
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        const u32x4 a = *(const u32x4 *)(src + 64 * c), b = *(const u32x4 *)(src + 64 * c + 8);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            x[c][2 * i] = bf_lo(a[i]);
-            x[c][2 * i + 1] = bf_hi(a[i]);
-            x[c][8 + 2 * i] = bf_lo(b[i]);
-            x[c][9 + 2 * i] = bf_hi(b[i]);
+            x[c][2 * i] = bf_lo(r.w[2 * c][i]);
+            x[c][2 * i + 1] = bf_hi(r.w[2 * c][i]);
+            x[c][8 + 2 * i] = bf_lo(r.w[2 * c + 1][i]);
+            x[c][9 + 2 * i] = bf_hi(r.w[2 * c + 1][i]);
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) ss += x[c][i] * x[c][i];
@@ -61,16 +76,36 @@ __device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, 
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[c][i] *= inv * p.q_norm[64 * c + 16 * g + i];
+            for (int i = 0; i < 16; i += 4) {
+                const float4 w = *(const float4 *)(p.q_norm + 64 * c + 16 * g + i);
+                x[c][i] *= inv * w.x;
+                x[c][i + 1] *= inv * w.y;
+                x[c][i + 2] *= inv * w.z;
+                x[c][i + 3] *= inv * w.w;
+            }
     }
-    if (p.n_rot) {   // dims 16g + e of the first 64: pair (16g + e) % 32, whose other half is lane g ^ 2
+    if (p.n_rot) {
+        // dims 16g + e of the first 64: pair (16g + e) % 32, whose other half lane ^ 32 holds; the two lanes share
+        // their 16 pairs' sin and cos, eight each
+        float sn[16], cn[16];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = 16 * (g & 1) + 8 * (g >> 1) + e;
+            const int axis = i % 3;
+            rope_sincos((axis == 0 ? r.pos[0] : axis == 1 ? r.pos[1] : r.pos[2]) * p.inv_freq[i], &sn[e], &cn[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float s1 = other_half(sn[e]), c1 = other_half(cn[e]), s0 = sn[e], c0 = cn[e];
+            sn[e] = g < 2 ? s0 : s1;
+            sn[e + 8] = g < 2 ? s1 : s0;
+            cn[e] = g < 2 ? c0 : c1;
+            cn[e + 8] = g < 2 ? c1 : c0;
+        }
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            const int i = (16 * g + e) & 31;
-            float sn, cn;
-            rope_sincos((float)p.pos3[3 * (size_t)t + i % 3] * p.inv_freq[i], &sn, &cn);
-            const float other = __shfl_xor(x[0][e], 32);
-            x[0][e] = g < 2 ? x[0][e] * cn - other * sn : x[0][e] * cn + other * sn;
+            const float o = other_half(x[0][e]);
+            x[0][e] = g < 2 ? x[0][e] * cn[e] - o * sn[e] : x[0][e] * cn[e] + o * sn[e];
         }
     }
     bool bad = false;
@@ -112,190 +147,208 @@ __device__ __forceinline__ float *partial_ml(const Params &p) {
 }
 
 // Few rows (decoding): a workgroup takes an item's 16 MT rows over its pages, wave w the pages w, w + 4, ...
-// Each wave reads its pages straight into registers, all of one page's K and V ahead of their use, so 32 KB
-// per wave are in flight; the four waves' results join through LDS.
+// Bound by memory: each page is read once, straight into registers, 4 KB pieces (four 1 KB loads) in a ring of
+// four that K and V share: as a piece is used up, the one four later is loaded into its registers, so 16 KB a
+// wave are always in flight, and with 16 rows two workgroups fit a CU, one's prologue and joins behind the
+// other's stream. Page numbers and scales of a wave's next 64 pages are held one per lane. The four waves'
+// results join through LDS.
 constexpr int kRowsThreads = 256, kRowsWaves = 4;
 template <int MT>
-__global__ __launch_bounds__(kRowsThreads) void kv8_attn_rows_kernel(Params p) {
+__global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_kernel(Params p) {
     constexpr int BM = 16 * MT, OS = HD + 4;   // LDS row stride of the outputs
     __shared__ float os[kRowsWaves][16][OS], ml[kRowsWaves][BM][2];
     const int32_t *h = p.plan;
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm)) return;
-    const int units = h[H_ITEMS] * p.nkv;
+    const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
+    const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
+    const int4 e0 = it[0], e1 = it[1];
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_ITEMS]) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q16 = lane & 15, g = lane >> 4;
     const int lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;   // the lane's piece of tile 0
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int item = u / p.nkv, kh = u - item * p.nkv;
-        const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
-        const int4 e0 = it[0], e1 = it[1];
-        const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
-        const int pg0 = e1.z, pg1 = e1.w;
-        const int32_t *table = p.tables + (size_t)seq * p.max_pages;
-        u32x4 kr[16], vr[16];
-        auto base = [&](int pg) {
-            const unsigned id = (unsigned)table[pg];
-            return ((size_t)(id < (unsigned)p.n_pages ? id : 0u) * p.nkv + kh);
-        };
-        auto load = [&](u32x4 (&r)[16], const uint8_t *pages, size_t at) {
-            const uint8_t *src = pages + at * PAGE_BYTES + lofs;
+    const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
+    const int pg0 = e1.z, pg1 = e1.w;
+    const int32_t *table = p.tables + (size_t)seq * p.max_pages;
+    QRow raw[MT];
+    int last[MT];   // the last key the lane's row sees
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+    for (int m = 0; m < MT; m++) {
+        const int fr = row0 + min(16 * m + q16, rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
+        load_q(p, q0 + t, head, g, raw[m]);
+        last[m] = L + t;
+    }
+    // the wave's pages i = 0, 1, ... are pg0 + wave + 4 i; lane j holds number and scales of page (i & ~63) + j
+    const int n_mine = (pg1 - pg0 - wave + kRowsWaves - 1) / kRowsWaves;   // 0 or less: none
+    unsigned ids = 0;
+    float kss = 0.f, vss = 0.f;
+    auto look_up = [&](int i0) {
+        const int pg = pg0 + wave + kRowsWaves * (i0 + lane);
+        ids = pg < pg1 ? (unsigned)table[pg] : 0u;
+        if (ids >= (unsigned)p.n_pages) ids = 0;
+        ids = ids * p.nkv + kh;
+        kss = p.k_scale[ids];
+        vss = p.v_scale[ids];
+    };
+    u32x4 ring[4][4];
+    auto load = [&](const uint8_t *pages, unsigned at, int c) {
+        const uint8_t *src = pages + (size_t)at * PAGE_BYTES + 4096 * c + lofs;
 #pragma unroll
-                for (int t = 0; t < 4; t++) r[4 * c + t] = *(const u32x4 *)(src + 4096 * c + 256 * t);
-        };
-        size_t at = 0;
-        float ks = 0.f, vs = 0.f;
-        if (pg0 + wave < pg1) {
-            at = base(pg0 + wave);
-            load(kr, p.k_pages, at);
-            load(vr, p.v_pages, at);
-            ks = p.k_scale[at];
-            vs = p.v_scale[at];
-        }
-        f16x8 q[MT][8];
-        int last[MT];   // the last key the lane's row sees
+        for (int t = 0; t < 4; t++) ring[c][t] = *(const u32x4 *)(src + 256 * t);
+    };
+    unsigned at = 0;
+    if (n_mine > 0) {
+        look_up(0);
+        at = __builtin_amdgcn_readlane(ids, 0);
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int fr = row0 + min(16 * m + q16, rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
-            load_q(p, q0 + t, head, g, q[m], p.ovf ? p.ovf + q0 : nullptr);
-            last[m] = L + t;
-        }
-        f32x4 o[MT][16];
-        float mx[MT], sum[MT];
+        for (int c = 0; c < 4; c++) load(p.k_pages, at, c);
+    }
+    f16x8 q[MT][8];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            mx[m] = kNone;
-            sum[m] = 0.f;
+    for (int m = 0; m < MT; m++) make_q(p, raw[m], g, q[m], p.ovf ? p.ovf + q0 : nullptr);
+    f32x4 o[MT][16];
+    float mx[MT], sum[MT];
+    int unit = 0;   // o is in units of 2^(unit - 15)
 #pragma unroll
-            for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        for (int pg = pg0 + wave; pg < pg1; pg += kRowsWaves) {
-            const bool more = pg + kRowsWaves < pg1;
-            f32x4 s[MT][4];
+    for (int m = 0; m < MT; m++) {
+        mx[m] = kNone;
+        sum[m] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int i = 0; i < n_mine; i++) {
+        const int pg = pg0 + wave + kRowsWaves * i;
+        const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
+        const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;   // the V scale is 2^ev
+        f32x4 s[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
 #pragma unroll
             for (int t = 0; t < 4; t++) {
+                const u32x4 w = ring[c][t];
+                const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
 #pragma unroll
-                for (int m = 0; m < MT; m++) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const u32x4 w = kr[4 * c + t];
-                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * c], s[m][t], 0, 0, 0);
-                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, q[m][2 * c + 1], s[m][t], 0, 0, 0);
-                    }
+                for (int m = 0; m < MT; m++) {
+                    s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * c], s[m][t], 0, 0, 0);
+                    s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, q[m][2 * c + 1], s[m][t], 0, 0, 0);
                 }
             }
-            const float kf = ks * p.scale_log2;
-            const int ev = (int)(__float_as_uint(vs) >> 23) - 127;   // vs = 2^ev
-            size_t next = 0;
-            if (more) {
-                next = base(pg + kRowsWaves);
-                load(kr, p.k_pages, next);
-                ks = p.k_scale[next];
-                vs = p.v_scale[next];
-            }
-            // keys behind the last one hold whatever the page held: their scores and V codes are cut off
-            const int key0 = pg * PAGE + 16 * g;
-            bf16x8 pb[MT][2];
+            load(p.v_pages, at, c);
+        }
+        const int key0 = pg * PAGE + 16 * g;
+        f16x8 pb[MT][2];
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                if ((pg + 1) * PAGE > L + 1) {
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (key0 + 4 * t + i > last[m]) s[m][t][i] = -INFINITY;
-                }
-                float top = s[m][0][0];
+        for (int m = 0; m < MT; m++) {
+            // keys behind the row's last one hold whatever the page holds: their scores are cut off
+            if ((pg + 1) * PAGE > L + 1) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[m][t][i]);
-                const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
-                const float f = __builtin_amdgcn_exp2f(mx[m] - now);
-                mx[m] = now;
-                float add = 0.f;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][i], kf, -now));
-                        add += x;
-                        pb[m][t >> 1][4 * (t & 1) + i] = (__bf16)ldexpf(x, ev);
-                    }
-                sum[m] = sum[m] * f + add;
-#pragma unroll
-                for (int d = 0; d < 16; d++) o[m][d] *= f;
+                    for (int e = 0; e < 4; e++)
+                        if (key0 + 4 * t + e > last[m]) s[m][t][e] = -INFINITY;
             }
-            if ((pg + 1) * PAGE > n_keys) {
+            float top = s[m][0][0];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
+            const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
+            const float f = __builtin_amdgcn_exp2f(mx[m] - now);
+            mx[m] = now;
+            float add = 0.f;
+            const float shift = 15.f - now;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][e], kf, shift));
+                    add += x;
+                    pb[m][t >> 1][4 * (t & 1) + e] = (_Float16)x;
+                }
+            sum[m] = sum[m] * f + add;
+            const float fo = ldexpf(f, unit - ev);
+            if (__any(fo != 1.f))
+#pragma unroll
+                for (int d = 0; d < 16; d++) o[m][d] *= fo;
+        }
+        unit = ev;
+        const bool more = i + 1 < n_mine;
+        unsigned next = 0;
+        if (more) {
+            if (((i + 1) & 63) == 0) look_up(i + 1);
+            next = __builtin_amdgcn_readlane(ids, (i + 1) & 63);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if ((pg + 1) * PAGE > n_keys) {   // V codes behind the last key, which may be NaN
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     const int v = n_keys - key0 - 4 * w;   // valid bytes of the word
                     const unsigned keep = v >= 4 ? ~0u : v <= 0 ? 0u : (1u << 8 * v) - 1;
 #pragma unroll
-                    for (int d = 0; d < 16; d++) vr[d][w] &= keep;
+                    for (int t = 0; t < 4; t++) ring[c][t][w] &= keep;
                 }
             }
 #pragma unroll
-            for (int d = 0; d < 16; d++) {
-                const u32x4 w = vr[d];
-                const bf16x8 a = codes_bf16(w[0], w[1]), b = codes_bf16(w[2], w[3]);
+            for (int t = 0; t < 4; t++) {
+                const u32x4 w = ring[c][t];
+                const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
-                    o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[m][0], o[m][d], 0, 0, 0);
-                    o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, pb[m][1], o[m][d], 0, 0, 0);
+                    o[m][4 * c + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[m][0], o[m][4 * c + t], 0, 0, 0);
+                    o[m][4 * c + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pb[m][1], o[m][4 * c + t], 0, 0, 0);
                 }
             }
-            if (more) load(vr, p.v_pages, next);
+            if (more) load(p.k_pages, next, c);
         }
-        // join the waves: each scales its outputs to the common maximum
+        at = next;
+    }
+    // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^15 P)
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            sum[m] = text::xrow_sum(sum[m]);
-            if (g == 0) {
-                ml[wave][16 * m + q16][0] = mx[m];
-                ml[wave][16 * m + q16][1] = sum[m];
-            }
+    for (int m = 0; m < MT; m++) {
+        sum[m] = text::xrow_sum(sum[m]);
+        if (g == 0) {
+            ml[wave][16 * m + q16][0] = mx[m];
+            ml[wave][16 * m + q16][1] = sum[m];
         }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][16 * m + q16][0]);
+        const float f = ldexpf(__builtin_amdgcn_exp2f(mx[m] - top), unit);
+#pragma unroll
+        for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
         __syncthreads();
+        const int r = tid >> 4, d0 = 16 * (tid & 15), row = 16 * m + r;
+        if (row < rows) {
+            float x[16], l = 0.f;
+            float mrow = kNone;
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            float top = kNone;
+            for (int w = 0; w < kRowsWaves; w++) mrow = fmaxf(mrow, ml[w][row][0]);
 #pragma unroll
-            for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][16 * m + q16][0]);
-            const float f = __builtin_amdgcn_exp2f(mx[m] - top);
+            for (int w = 0; w < kRowsWaves; w++) l += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - mrow);
 #pragma unroll
-            for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
-            __syncthreads();
-            const int r = tid >> 4, d0 = 16 * (tid & 15), row = 16 * m + r;
-            if (row < rows) {
-                float x[16], l = 0.f;
-                float mrow = kNone;
+            for (int i = 0; i < 16; i++) x[i] = os[0][r][d0 + i] + os[1][r][d0 + i] + os[2][r][d0 + i] + os[3][r][d0 + i];
+            if (slot < 0) {
+                const int fr = row0 + row, t = fr / p.group, head = kh * p.group + fr - t * p.group;
+                const float inv = 1.f / l;
 #pragma unroll
-                for (int w = 0; w < kRowsWaves; w++) mrow = fmaxf(mrow, ml[w][row][0]);
+                for (int i = 0; i < 16; i++) x[i] *= inv;
+                finish16(p, q0 + t, head, d0, x, p.ovf ? p.ovf + q0 : nullptr);
+            } else {
+                const size_t pr = partial_row(p, slot, kh, row);
+                float *dst = p.partial + pr * HD + d0;
 #pragma unroll
-                for (int w = 0; w < kRowsWaves; w++) l += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - mrow);
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = os[0][r][d0 + i] + os[1][r][d0 + i] + os[2][r][d0 + i] + os[3][r][d0 + i];
-                if (slot < 0) {
-                    const int fr = row0 + row, t = fr / p.group, head = kh * p.group + fr - t * p.group;
-                    const float inv = 1.f / l;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) x[i] *= inv;
-                    finish16(p, q0 + t, head, d0, x, p.ovf ? p.ovf + q0 : nullptr);
-                } else {
-                    const size_t pr = partial_row(p, slot, kh, row);
-                    float *dst = p.partial + pr * HD + d0;
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) *(f32x4 *)(dst + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-                    if ((tid & 15) == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
-                }
+                for (int i = 0; i < 16; i += 4) *(f32x4 *)(dst + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+                if ((tid & 15) == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
             }
-            __syncthreads();
         }
+        if (m + 1 < MT) __syncthreads();
     }
 }
 

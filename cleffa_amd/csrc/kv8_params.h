@@ -44,7 +44,7 @@ inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
     const int G = nh / nkv;
     const long rows = (long)(max_new > 0 && max_new < T ? max_new : T) * G;
     l.bm = rows <= 16 ? 16 : 32;
-    l.budget = (2 * n_cu + nkv - 1) / nkv;
+    l.budget = ((l.bm == 16 ? 2 : 1) * n_cu + nkv - 1) / nkv;   // items of one round of workgroups, two or one to a CU
     l.least = 4;
     const long app = (long)T / PAGE + 2L * n_seq;
     l.max_app = (int)(app < T ? app : T);

@@ -184,7 +184,15 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanParams p) {
         if (small) v[0] = (int)mine;
         block_scan(v, total, (int(*)[1])waves);
         const long W = small ? (long)total[0] : (long)total[0] << 8;
-        const int C = (int)max((long)p.l.least, (W + p.l.budget - 1) / p.l.budget);
+        int C = (int)max((long)p.l.least, (W + p.l.budget - 1) / p.l.budget);
+        // few blocks: the chunk grows until the items fit the budget, which is one round of workgroups
+        for (int again = 0; again < 4 && 2 * n_blk <= p.l.budget; again++) {
+            int c[1] = {0}, all[1];
+            if (tid < n_blk) c[0] = (block(tid, r, row0, rows) + C - 1) / C;
+            block_scan(c, all, (int(*)[1])waves);
+            if (all[0] <= p.l.budget) break;
+            C = max(C + 1, (int)((long)C * all[0] / p.l.budget));
+        }
         int at = 0, at_slot = 0;
         for (int b0 = 0; b0 < n_blk; b0 += kPlanThreads) {
             const int b = b0 + tid;
