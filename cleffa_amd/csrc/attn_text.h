@@ -82,14 +82,6 @@ __device__ __forceinline__ void lds_wait4(bf16x8 &r0, bf16x8 &r1, bf16x8 &r2, bf
 __device__ __forceinline__ unsigned lds_addr(const uint16_t *p) {
     return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)p;
 }
-template <typename F, int... I>
-__device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void static_for(F &&f) {
-    static_for_impl(f, std::make_integer_sequence<int, N>{});
-}
 }  // namespace text
 
 // Work items are (query block, q head) pairs. Workgroup b takes items get(0), get(1), ... With a

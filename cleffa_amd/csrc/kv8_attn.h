@@ -18,6 +18,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "bf16_ops.h"
 #include "kv8_pages.h"
 #include "kv8_params.h"
@@ -34,6 +36,9 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
     const f16x2 z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
     return f16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
+// The first n bytes of a word (n below 0 or above 4: none, all).
+__device__ __forceinline__ unsigned keep_bytes(int n) { return n <= 0 ? 0u : ~0u >> 8 * (4 - min(n, 4)); }
+
 // One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
 // 2c (e < 8) and 2c + 1. Two steps, so that other loads can go out between them: the row as it is, then norm and
 // rotary in f32 and f16 with split16's saturation (flagged).
@@ -187,6 +192,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
         ids = ids * p.nkv + kh;
         kss = p.k_scale[ids];
         vss = p.v_scale[ids];
+        asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here: the loop's waits are for its own loads
     };
     u32x4 ring[4][4];
     auto load = [&](const uint8_t *pages, unsigned at, int c) {
@@ -214,7 +220,11 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 #pragma unroll
         for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int i = 0; i < n_mine; i++) {
+    // Only a wave's last page can hold keys that a row does not see or that are not there: an item's rows are of at
+    // most 32 tokens, whose keys lie in its last two pages. It runs apart, so that the others' loads are unconditional
+    // (the compiler's waits would otherwise count on none being in flight).
+    auto page = [&](int i, auto more_t) {
+        constexpr bool MORE = decltype(more_t)::value;
         const int pg = pg0 + wave + kRowsWaves * i;
         const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
         const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;   // the V scale is 2^ev
@@ -236,13 +246,13 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
                 }
             }
             load(p.v_pages, at, c);
+            __builtin_amdgcn_sched_barrier(0);   // pieces are used, and asked for, in this order
         }
         const int key0 = pg * PAGE + 16 * g;
         f16x8 pb[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            // keys behind the row's last one hold whatever the page holds: their scores are cut off
-            if ((pg + 1) * PAGE > L + 1) {
+            if (!MORE && (pg + 1) * PAGE > L + 1) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -274,23 +284,20 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
                 for (int d = 0; d < 16; d++) o[m][d] *= fo;
         }
         unit = ev;
-        const bool more = i + 1 < n_mine;
         unsigned next = 0;
-        if (more) {
+        if constexpr (MORE) {
             if (((i + 1) & 63) == 0) look_up(i + 1);
             next = __builtin_amdgcn_readlane(ids, (i + 1) & 63);
+        } else if ((pg + 1) * PAGE > n_keys) {   // V codes behind the last key may be NaN, whose product with 0 is NaN
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const unsigned keep = keep_bytes(n_keys - key0 - 4 * w);
+#pragma unroll
+                for (int d = 0; d < 16; d++) ring[d >> 2][d & 3][w] &= keep;
+            }
         }
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            if ((pg + 1) * PAGE > n_keys) {   // V codes behind the last key, which may be NaN
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int v = n_keys - key0 - 4 * w;   // valid bytes of the word
-                    const unsigned keep = v >= 4 ? ~0u : v <= 0 ? 0u : (1u << 8 * v) - 1;
-#pragma unroll
-                    for (int t = 0; t < 4; t++) ring[c][t][w] &= keep;
-                }
-            }
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const u32x4 w = ring[c][t];
@@ -301,10 +308,13 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
                     o[m][4 * c + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pb[m][1], o[m][4 * c + t], 0, 0, 0);
                 }
             }
-            if (more) load(p.k_pages, next, c);
+            if constexpr (MORE) load(p.k_pages, next, c);
+            __builtin_amdgcn_sched_barrier(0);
         }
         at = next;
-    }
+    };
+    for (int i = 0; i + 1 < n_mine; i++) page(i, std::true_type{});
+    if (n_mine > 0) page(n_mine - 1, std::false_type{});
     // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^15 P)
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -349,6 +359,239 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
             }
         }
         if (m + 1 < MT) __syncthreads();
+    }
+}
+
+// Many rows (prompts, questions): 128 rows an item, 16 MT per wave, the pages shared through LDS. Pages come in as
+// they are by DMA (global_load_lds), already in operand order, three stages of 32 KB ahead of one barrier a
+// page; every wave turns the codes it needs into f16 after the read. Codes in LDS halve its traffic against
+// f16 tiles (8 waves x 32 KB a page: 2,048 clocks, as long as the page's matrix products), for 256 conversions
+// per wave and page.
+constexpr int kTileStages = 3, kTileStage = 2 * PAGE_BYTES;
+typedef __attribute__((address_space(3))) void lds_ptr;
+template <int OFF>
+__device__ __forceinline__ u32x4 lds_read(unsigned addr) {
+    u32x4 r;
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF) : "memory");
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void lds_wait(u32x4 (&r)[4]) {
+    asm volatile("s_waitcnt lgkmcnt(%4)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]) : "i"(N));
+}
+template <int C>
+__device__ __forceinline__ void lds_piece(u32x4 (&r)[4], unsigned addr) {
+    r[0] = lds_read<4096 * C>(addr);
+    r[1] = lds_read<4096 * C + 1024>(addr);
+    r[2] = lds_read<4096 * C + 2048>(addr);
+    r[3] = lds_read<4096 * C + 3072>(addr);
+}
+
+template <int MT>
+__global__ __launch_bounds__(512 / MT, 2 / MT) void kv8_attn_tile_kernel(Params p) {
+    constexpr int WAVES = 8 / MT, PIECES = 32 / WAVES, NS = kTileStages;
+    __shared__ __attribute__((aligned(16))) uint8_t stage[NS * kTileStage];
+    const int32_t *h = p.plan;
+    const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
+    const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
+    const int4 e0 = it[0], e1 = it[1];
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_ITEMS]) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q16 = lane & 15, g = lane >> 4;
+    const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
+    const int pg0 = e1.z, n_pages = e1.w - e1.z;
+    const int32_t *table = p.tables + (size_t)seq * p.max_pages;
+    const int w0 = 16 * MT * wave;   // the wave's first row in the block
+    const bool active = w0 < rows;
+    QRow raw[MT];
+    int last[MT], head[MT], tok[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int fr = row0 + min(w0 + 16 * m + q16, rows - 1);
+        tok[m] = fr / p.group;
+        head[m] = kh * p.group + fr - tok[m] * p.group;
+        load_q(p, q0 + tok[m], head[m], g, raw[m]);
+        last[m] = L + tok[m];
+    }
+    // keys that every row of the wave sees, and the last that any sees
+    const int all_see = L + (row0 + min(w0, rows - 1)) / p.group, any_sees = L + (row0 + min(w0 + 16 * MT, rows) - 1) / p.group;
+    unsigned ids = 0;   // lane j: page (i & ~63) + j
+    float kss = 0.f, vss = 0.f;
+    auto look_up = [&](int i0) {
+        const int i = i0 + lane;
+        ids = i < n_pages ? (unsigned)table[pg0 + i] : 0u;
+        if (ids >= (unsigned)p.n_pages) ids = 0;
+        ids = ids * p.nkv + kh;
+    };
+    unsigned pofs[PIECES];   // the lane's byte in the page of each piece its wave loads
+#pragma unroll
+    for (int j = 0; j < PIECES; j++) {
+        const int piece = (wave * PIECES + j) & 15;
+        pofs[j] = (piece >> 2) * 4096 + (piece & 3) * 256 + (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;
+    }
+    auto fill = [&](int i) {   // page i into its stage; i & 63 must lie in the looked-up run
+        const size_t at = (size_t)__builtin_amdgcn_readlane(ids, i & 63) * PAGE_BYTES;
+        const uint8_t *src = (wave * PIECES < 16 ? p.k_pages : p.v_pages) + at;
+        uint8_t *dst = stage + (i % NS) * kTileStage + wave * PIECES * 1024;
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            unsigned off = pofs[j];
+            asm volatile("" : "+v"(off));
+            __builtin_amdgcn_global_load_lds((const void *)(src + off), (lds_ptr *)(dst + 1024 * j), 16, 0, 0);
+        }
+    };
+    look_up(0);
+    const unsigned ids0 = ids;
+    kss = p.k_scale[ids0];
+    vss = p.v_scale[ids0];
+    for (int i = 0; i < NS - 1 && i < n_pages; i++) fill(i);
+    f16x8 q[MT][8];
+#pragma unroll
+    for (int m = 0; m < MT; m++) make_q(p, raw[m], g, q[m], p.ovf ? p.ovf + q0 : nullptr);
+    asm volatile("" : "+v"(kss), "+v"(vss));
+    f32x4 o[MT][16];
+    float mx[MT], sum[MT];
+    int unit = 0;   // o is in units of 2^(unit - 15)
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        mx[m] = kNone;
+        sum[m] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const unsigned lds0 = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)stage + 16 * lane;
+    for (int i = 0; i < n_pages; i++) {
+        if (i && (i & 63) == 0) {   // the scales of this page's run (its numbers were looked up with the fills)
+            const int j = i + lane;
+            unsigned id = j < n_pages ? (unsigned)table[pg0 + j] : 0u;
+            if (id >= (unsigned)p.n_pages) id = 0;
+            kss = p.k_scale[(size_t)id * p.nkv + kh];
+            vss = p.v_scale[(size_t)id * p.nkv + kh];
+            asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here, or every page would wait for all fills
+        }
+        // the page has come once at most the fills of the pages behind it are in flight, in every wave
+        if (i + 1 < n_pages) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PIECES * (NS - 2)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int ahead = i + NS - 1;   // its stage held page i - 1, which every wave is done with
+        if (ahead < n_pages) {
+            if ((ahead & 63) == 0) look_up(ahead);
+            fill(ahead);
+        }
+        const int pg = pg0 + i;
+        if (active && pg * PAGE <= any_sees) {
+            const unsigned kl = lds0 + (i % NS) * kTileStage;
+            u32x4 r[2][4];
+            f32x4 s[MT][4];
+            lds_piece<0>(r[0], kl);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            auto k_step = [&](auto c) {
+                constexpr int C = decltype(c)::value;
+                lds_piece<C + 1>(r[(C + 1) & 1], kl);   // behind K piece 3 lies V piece 0
+                lds_wait<4>(r[C & 1]);
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const u32x4 w = r[C & 1][t];
+                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * C], s[m][t], 0, 0, 0);
+                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, q[m][2 * C + 1], s[m][t], 0, 0, 0);
+                    }
+                }
+            };
+            text::static_for<4>(k_step);
+            const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
+            const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;
+            const int key0 = pg * PAGE + 16 * g;
+            f16x8 pb[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                if ((pg + 1) * PAGE > all_see + 1) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (key0 + 4 * t + e > last[m]) s[m][t][e] = -INFINITY;
+                }
+                float top = s[m][0][0];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
+                const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
+                const float f = __builtin_amdgcn_exp2f(mx[m] - now);
+                mx[m] = now;
+                float add = 0.f;
+                const float shift = 15.f - now;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][e], kf, shift));
+                        add += x;
+                        pb[m][t >> 1][4 * (t & 1) + e] = (_Float16)x;
+                    }
+                sum[m] = sum[m] * f + add;
+                const float fo = ldexpf(f, unit - ev);
+                if (__any(fo != 1.f))
+#pragma unroll
+                    for (int d = 0; d < 16; d++) o[m][d] *= fo;
+            }
+            unit = ev;
+            const bool tail = (pg + 1) * PAGE > n_keys;
+            auto v_step = [&](auto c) {
+                constexpr int C = decltype(c)::value;
+                if constexpr (C < 3) {
+                    lds_piece<C + 5>(r[(C + 1) & 1], kl);
+                    lds_wait<4>(r[C & 1]);
+                } else lds_wait<0>(r[C & 1]);
+                if (tail) {   // V codes behind the last key, which may be NaN
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const unsigned keep = keep_bytes(n_keys - key0 - 4 * w);
+#pragma unroll
+                        for (int t = 0; t < 4; t++) r[C & 1][t][w] &= keep;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const u32x4 w = r[C & 1][t];
+                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        o[m][4 * C + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[m][0], o[m][4 * C + t], 0, 0, 0);
+                        o[m][4 * C + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pb[m][1], o[m][4 * C + t], 0, 0, 0);
+                    }
+                }
+            };
+            text::static_for<4>(v_step);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int row = w0 + 16 * m + q16;
+        const float l = text::xrow_sum(sum[m]);
+        if (row >= rows) continue;
+        const float f = slot < 0 ? ldexpf(1.f / l, unit) : ldexpf(1.f, unit);
+        const size_t pr = slot < 0 ? 0 : partial_row(p, slot, kh, row);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            float x[16];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * t + e] = o[m][4 * c + t][e] * f;
+            if (slot < 0) finish16(p, q0 + tok[m], head[m], 64 * c + 16 * g, x, p.ovf ? p.ovf + q0 : nullptr);
+            else
+#pragma unroll
+                for (int t = 0; t < 4; t++) *(f32x4 *)(p.partial + pr * HD + 64 * c + 16 * g + 4 * t) = f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+        }
+        if (slot >= 0 && g == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mx[m], l);
     }
 }
 

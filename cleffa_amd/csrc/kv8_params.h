@@ -31,9 +31,8 @@ enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_IT
 //  a row being one q head of the kv group for one token (token-major);
 //  attention items {sequence, its first pass row, its cached tokens, its keys, first row, rows |
 //  (split slot + 1) << 8, first page, end page}: a block's rows over a run of its pages.
-// A block of p pages is cut when p exceeds the chunk C = max(least, ceil(W / budget)), W the pages of
-// all blocks: ceil(p / C) < p / C + 1, so items <= blocks + budget, and items of cut blocks (split
-// slots) < 2 W / C <= 2 budget.
+// A block of p pages makes max(1, floor(p / C + 1/2)) items, C at least W / budget, W the pages of all
+// blocks: items <= blocks + budget, and those of cut blocks (split slots; p >= 1.5 C) <= 4 W / (3 C) < 2 budget.
 struct Layout {
     int bm, budget, least, max_app, max_blk, max_items, max_slots;
     long app, tok, blk, items, ints;
@@ -43,7 +42,7 @@ inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
     Layout l;
     const int G = nh / nkv;
     const long rows = (long)(max_new > 0 && max_new < T ? max_new : T) * G;
-    l.bm = rows <= 16 ? 16 : 32;
+    l.bm = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     l.budget = ((l.bm == 16 ? 2 : 1) * n_cu + nkv - 1) / nkv;   // items of one round of workgroups, two or one to a CU
     l.least = 4;
     const long app = (long)T / PAGE + 2L * n_seq;

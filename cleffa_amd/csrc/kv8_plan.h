@@ -185,10 +185,12 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanParams p) {
         block_scan(v, total, (int(*)[1])waves);
         const long W = small ? (long)total[0] : (long)total[0] << 8;
         int C = (int)max((long)p.l.least, (W + p.l.budget - 1) / p.l.budget);
+        // a block below 1.5 chunks stays whole, others are cut into the nearest number of pieces
+        auto pieces = [&](int pages) { return max(1, (2 * pages + C) / (2 * C)); };
         // few blocks: the chunk grows until the items fit the budget, which is one round of workgroups
         for (int again = 0; again < 4 && 2 * n_blk <= p.l.budget; again++) {
             int c[1] = {0}, all[1];
-            if (tid < n_blk) c[0] = (block(tid, r, row0, rows) + C - 1) / C;
+            if (tid < n_blk) c[0] = pieces(block(tid, r, row0, rows));
             block_scan(c, all, (int(*)[1])waves);
             if (all[0] <= p.l.budget) break;
             C = max(C + 1, (int)((long)C * all[0] / p.l.budget));
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanParams p) {
             int pages = 0, c[2] = {0, 0}, sum[2];
             if (b < n_blk) {
                 pages = block(b, r, row0, rows);
-                c[0] = (pages + C - 1) / C;
+                c[0] = pieces(pages);
                 c[1] = c[0] > 1 ? c[0] : 0;
             }
             const int items = c[0], cut = c[1];

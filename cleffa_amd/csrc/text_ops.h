@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 #include "bf16_ops.h"
 #include "clef_hip_attn.h"
 
@@ -122,6 +124,14 @@ __device__ __forceinline__ float xrow_sum(float x) {
     const float m = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F &&f) {
+    static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 }  // namespace text
 
