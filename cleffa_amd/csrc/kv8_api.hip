@@ -12,9 +12,6 @@
 #include "kv8_plan.h"
 
 using namespace clef_hip;
-#ifndef KV8_TILE_MT
-#define KV8_TILE_MT 1
-#endif
 
 namespace {
 
@@ -138,7 +135,7 @@ bool clef_hip_kv8_attention(const clef_hip_kv8_args *a, void *stream, char *err,
     // a workgroup for every item the plan may hold: the plan's counts are on the device
     const unsigned grid = (unsigned)(p.l.max_items * p.nkv);
     if (p.l.bm == 16) hipLaunchKernelGGL(kv8::kv8_attn_rows_kernel<1>, dim3(grid), dim3(kv8::kRowsThreads), 0, (hipStream_t)stream, p);
-    else if (p.l.bm == 128) hipLaunchKernelGGL(kv8::kv8_attn_tile_kernel<KV8_TILE_MT>, dim3(grid), dim3(512 / KV8_TILE_MT), 0, (hipStream_t)stream, p);
+    else if (p.l.bm == 128) hipLaunchKernelGGL(kv8::kv8_attn_tile_kernel, dim3(grid), dim3(kv8::kTileThreads), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL(kv8::kv8_attn_rows_kernel<2>, dim3(grid), dim3(kv8::kRowsThreads), 0, (hipStream_t)stream, p);
     if (!launch_ok("kv8_attn", err, errlen)) return false;
     const long rows = (long)p.T * p.nh;

@@ -4,12 +4,11 @@
 // Rows are (token, q head of the kv group), token-major, so that the q heads that share a kv head share its
 // pages: one token of 24/4 heads is 6 rows of a 16-row matrix tile. Per 16-row tile and 64-token page
 //   S^T = K . Q^T     v_mfma_f32_16x16x32_f16: A = K codes as f16 (exact), B = Q (f16)
-//   O^T += V^T . P^T  v_mfma_f32_16x16x32_f16: A = V codes as f16 (exact), B = 2^15 P (f16)
-// The page's K scale multiplies the f32 scores together with the softmax scale, at no cost per element. The
-// accumulated O is kept in units of the current page's V scale times 2^-15: where that changes, so does the factor
-// that rescales O for a new maximum. P in f16 rounds by 2^-11 of itself (bf16: 2^-8); 2^15 P keeps that down
-// to P = 2^-29, and what falls below 2^-40 of the row's largest weight is lost. Units of 2^-64 to 2^8 leave O
-// within 2^113 and 2^-100. Row r of A tile t (of four that make up 64
+//   O^T += V^T . P^T  v_mfma_f32_16x16x32_f16: A = V codes as f16 (exact), B = P (f16)
+// The page's K scale multiplies the f32 scores together with the softmax scale, its V scale is a unit of O or goes
+// into the exponent of P: neither costs an instruction per element. P in f16 rounds by 2^-11 of itself (bf16:
+// 2^-8); against the row's largest it is held from 2^3 on, which keeps that down to P = 2^-17, with steps of
+// 2^-27 below. Units of 2^-64 to 2^8 leave O within 2^113 and 2^-100. Row r of A tile t (of four that make up 64
 // rows) is token / dim 16 (r / 4) + 4 t + r % 4: then a lane's 16 scores of a page are 16 consecutive tokens,
 // which are the k indexes of the next product's B operand with no exchange, and its 16 outputs of a dim
 // group are consecutive dims. A lane reads 16-byte pieces (row, 16 dims or tokens) of the page, each two
@@ -31,6 +30,21 @@ namespace kv8 {
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 constexpr float kNone = -1e30f;   // a running maximum before any key: below every score, and finite
 
+// The running maximum m is one that later pages may pass by up to 2^8: it, and what has been summed under it, is
+// only moved for a page that passes it by more (most pages of most rows do not, which saves the products that
+// rescale O). Likewise the unit of O, a V scale 2^unit, stays for pages whose scale is within 2^2 of it: the
+// difference goes into P's exponent. P is then held as 2^(5 + ev - unit) P in f16, 2^15 at most.
+constexpr float kPUnit = 5.f, kSlack = 8.f;
+constexpr int kUnitSlack = 2;
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+// Moves m for a page whose largest score is top; returns the factor that sums under the old m take.
+__device__ __forceinline__ float new_max(float &m, float top) {
+    const float now = top > m + kSlack ? top : m;
+    const float f = __builtin_amdgcn_exp2f(m - now);
+    m = now;
+    return f;
+}
+
 __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
     const f16x2 x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false), y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
     const f16x2 z = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false), w = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
@@ -39,12 +53,24 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
 // The first n bytes of a word (n below 0 or above 4: none, all).
 __device__ __forceinline__ unsigned keep_bytes(int n) { return n <= 0 ? 0u : ~0u >> 8 * (4 - min(n, 4)); }
 
+// sin and cos of an angle by the hardware functions of revolutions, the fraction exact in two products: 4e-7 off at
+// most up to 10^6 (measured over 4 million angles), against 5e-4 of an f16 operand.
+__device__ __forceinline__ void rope_turns(float x, float *s, float *c) {
+    constexpr double kTurn = 0.15915494309189535;   // 1 / (2 pi)
+    constexpr float C1 = (float)kTurn, C2 = (float)(kTurn - (double)C1);
+    const float j = __builtin_rintf(x * C1);
+    const float r = fmaf(x, C2, fmaf(x, C1, -j));
+    *s = __builtin_amdgcn_sinf(r);
+    *c = __builtin_amdgcn_cosf(r);
+}
+
 // One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
 // 2c (e < 8) and 2c + 1. Two steps, so that other loads can go out between them: the row as it is, then norm and
 // rotary in f32 and f16 with split16's saturation (flagged).
 struct QRow {
     u32x4 w[8];
-    float pos[3];
+    float4 norm[16], freq[2];
+    int pos[3];
 };
 __device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, QRow &r) {
     const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 16 * g;
@@ -53,9 +79,16 @@ __device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, 
         r.w[2 * c] = *(const u32x4 *)(src + 64 * c);
         r.w[2 * c + 1] = *(const u32x4 *)(src + 64 * c + 8);
     }
-    if (p.n_rot)
+    if (p.q_norm)
 #pragma unroll
-        for (int i = 0; i < 3; i++) r.pos[i] = (float)p.pos3[3 * (size_t)t + i];
+        for (int i = 0; i < 16; i++) r.norm[i] = *(const float4 *)(p.q_norm + 64 * (i >> 2) + 16 * g + 4 * (i & 3));
+    if (p.n_rot) {   // pairs 16 (g & 1) + 8 (g >> 1) + e
+        const int i0 = 16 * (g & 1) + 8 * (g >> 1);
+        r.freq[0] = *(const float4 *)(p.inv_freq + i0);
+        r.freq[1] = *(const float4 *)(p.inv_freq + i0 + 4);
+#pragma unroll
+        for (int i = 0; i < 3; i++) r.pos[i] = p.pos3[3 * (size_t)t + i];
+    }
 }
 __device__ __forceinline__ float other_half(float x) {   // lane ^ 32's value
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -82,7 +115,7 @@ __device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f1
         for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-                const float4 w = *(const float4 *)(p.q_norm + 64 * c + 16 * g + i);
+                const float4 w = r.norm[4 * c + i / 4];
                 x[c][i] *= inv * w.x;
                 x[c][i + 1] *= inv * w.y;
                 x[c][i + 2] *= inv * w.z;
@@ -95,9 +128,10 @@ __device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f1
         float sn[16], cn[16];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int i = 16 * (g & 1) + 8 * (g >> 1) + e;
-            const int axis = i % 3;
-            rope_sincos((axis == 0 ? r.pos[0] : axis == 1 ? r.pos[1] : r.pos[2]) * p.inv_freq[i], &sn[e], &cn[e]);
+            const int axis = (16 * (g & 1) + 8 * (g >> 1) + e) % 3;
+            const float4 f4 = r.freq[e >> 2];
+            const float f = (e & 3) == 0 ? f4.x : (e & 3) == 1 ? f4.y : (e & 3) == 2 ? f4.z : f4.w;
+            rope_turns((float)(axis == 0 ? r.pos[0] : axis == 1 ? r.pos[1] : r.pos[2]) * f, &sn[e], &cn[e]);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -113,22 +147,46 @@ __device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f1
             x[0][e] = g < 2 ? x[0][e] * cn[e] - o * sn[e] : x[0][e] * cn[e] + o * sn[e];
         }
     }
-    bool bad = false;
+    // split16's saturation: the largest magnitude decides (NaN passes through the maximum and fails the compare)
+    float most = 0.f;
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            bad |= saturate(x[c][i], p.f16_lim);
-            q[2 * c + (i >> 3)][i & 7] = (_Float16)x[c][i];
+        for (int i = 0; i < 16; i += 2)
+            most = __builtin_elementwise_maximum(most, __builtin_elementwise_maximum(fabsf(x[c][i]), fabsf(x[c][i + 1])));
+    if (!(most <= p.f16_lim)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) saturate(x[c][i], p.f16_lim);
+        if (flag) __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const f16x2 h = __builtin_bit_cast(f16x2, pack_f16(x[c][i], x[c][i + 1]));
+            q[2 * c + (i >> 3)][i & 7] = h[0];
+            q[2 * c + (i >> 3)][(i & 7) + 1] = h[1];
         }
-    if (bad && flag) __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Sixteen finished outputs (dims d0 ..) of a row: times the gate's sigmoid, converted and stored.
-__device__ __forceinline__ void finish16(const Params &p, int t, int head, int d0, float (&o)[16], int32_t *flag) {
+// Sixteen finished outputs (dims d0 ..) of a row: times the sigmoid of their gates (loaded ahead), converted and stored.
+struct Gate16 {
+    u32x4 a, b;
+};
+__device__ __forceinline__ Gate16 load_gate(const Params &p, int t, int head, int d0) {
+    Gate16 w = {};
     if (p.gate) {
         const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + d0;
-        const u32x4 a = *(const u32x4 *)src, b = *(const u32x4 *)(src + 8);
+        w.a = *(const u32x4 *)src;
+        w.b = *(const u32x4 *)(src + 8);
+    }
+    return w;
+}
+__device__ __forceinline__ void finish16(const Params &p, int t, int head, int d0, const Gate16 &w, float (&o)[16], int32_t *flag) {
+    if (p.gate) {
+        const u32x4 a = w.a, b = w.b;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             o[2 * i] *= sigmoidf(bf_lo(a[i]));
@@ -212,7 +270,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     for (int m = 0; m < MT; m++) make_q(p, raw[m], g, q[m], p.ovf ? p.ovf + q0 : nullptr);
     f32x4 o[MT][16];
     float mx[MT], sum[MT];
-    int unit = 0;   // o is in units of 2^(unit - 15)
+    int unit = 0;   // o is in units of 2^(unit - 5)
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         mx[m] = kNone;
@@ -249,6 +307,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
             __builtin_amdgcn_sched_barrier(0);   // pieces are used, and asked for, in this order
         }
         const int key0 = pg * PAGE + 16 * g;
+        const int now_unit = abs(ev - unit) <= kUnitSlack ? unit : ev;
         f16x8 pb[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -264,11 +323,9 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
-            const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
-            const float f = __builtin_amdgcn_exp2f(mx[m] - now);
-            mx[m] = now;
+            const float f = new_max(mx[m], text::xrow_max(top) * kf);
             float add = 0.f;
-            const float shift = 15.f - now;
+            const float shift = kPUnit + (float)(ev - now_unit) - mx[m];
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -277,13 +334,13 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
                     add += x;
                     pb[m][t >> 1][4 * (t & 1) + e] = (_Float16)x;
                 }
-            sum[m] = sum[m] * f + add;
-            const float fo = ldexpf(f, unit - ev);
+            sum[m] = sum[m] * f + add * pow2(now_unit - ev);
+            const float fo = ldexpf(f, unit - now_unit);
             if (__any(fo != 1.f))
 #pragma unroll
                 for (int d = 0; d < 16; d++) o[m][d] *= fo;
         }
-        unit = ev;
+        unit = now_unit;
         unsigned next = 0;
         if constexpr (MORE) {
             if (((i + 1) & 63) == 0) look_up(i + 1);
@@ -315,7 +372,14 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     };
     for (int i = 0; i + 1 < n_mine; i++) page(i, std::true_type{});
     if (n_mine > 0) page(n_mine - 1, std::false_type{});
-    // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^15 P)
+    Gate16 gate[MT];   // of the outputs that the thread will finish
+    if (slot < 0)
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int fr = row0 + min(16 * m + (tid >> 4), rows - 1), t = fr / p.group;
+            gate[m] = load_gate(p, q0 + t, kh * p.group + fr - t * p.group, 16 * (tid & 15));
+        }
+    // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^5 P)
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         sum[m] = text::xrow_sum(sum[m]);
@@ -349,7 +413,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
                 const float inv = 1.f / l;
 #pragma unroll
                 for (int i = 0; i < 16; i++) x[i] *= inv;
-                finish16(p, q0 + t, head, d0, x, p.ovf ? p.ovf + q0 : nullptr);
+                finish16(p, q0 + t, head, d0, gate[m], x, p.ovf ? p.ovf + q0 : nullptr);
             } else {
                 const size_t pr = partial_row(p, slot, kh, row);
                 float *dst = p.partial + pr * HD + d0;
@@ -362,236 +426,311 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     }
 }
 
-// Many rows (prompts, questions): 128 rows an item, 16 MT per wave, the pages shared through LDS. Pages come in as
-// they are by DMA (global_load_lds), already in operand order, three stages of 32 KB ahead of one barrier a
-// page; every wave turns the codes it needs into f16 after the read. Codes in LDS halve its traffic against
-// f16 tiles (8 waves x 32 KB a page: 2,048 clocks, as long as the page's matrix products), for 256 conversions
-// per wave and page.
-constexpr int kTileStages = 3, kTileStage = 2 * PAGE_BYTES;
-typedef __attribute__((address_space(3))) void lds_ptr;
+// Many rows (prompts, questions): 128 rows an item, the pages' codes turned into f16 once and shared through LDS.
+// On this chip conversions and the matrix products they feed hardly overlap (four conversions and a product take
+// 25 clocks of a SIMD, a product 16), so no wave converts what another has: each of the eight takes an eighth of a
+// page, and what is left to the inner loops is products and their LDS reads. Waves w and w + 4 share 32 rows: each
+// takes the scores of half of a page's tokens, and O of half of the dims, so that an operand read from LDS serves
+// two products and O and Q of 32 rows fit 128 registers, two waves a SIMD; the weights P go through LDS.
+// Two phases a page, a barrier behind each: scores and softmax of page i while its V is written to LDS, then
+// O += P V while K of page i + 1 is; so one slot of 32 KB is enough for each. Codes come into registers a page ahead.
+//
+// The maximum of a row is common to its two waves. A wave whose page passes it by more than the slack says so in a
+// flag; behind the barrier all waves then take the pairs' new maxima and make that page's P again (the first page,
+// and hardly ever after).
+constexpr int kTileThreads = 512;
+struct TileLds {
+    u32x4 k[32][64], v[32][64];   // operand [2 (4 c + t) + h][lane]
+    u32x4 p[4][2][2][64];         // row group, half of the tokens, tile
+    float top[4][2][32], sum[4][2][32];
+    int flag[2];
+};
+// Operand reads and slot writes are issued by hand and waited for by count, so that reads run four operands ahead of
+// the products and behind the conversions.
+__device__ __forceinline__ unsigned lds_at(const void *ptr) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)ptr; }
 template <int OFF>
 __device__ __forceinline__ u32x4 lds_read(unsigned addr) {
     u32x4 r;
     asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF) : "memory");
     return r;
 }
+template <int OFF, int STEP>
+__device__ __forceinline__ void lds_read4(u32x4 (&r)[4], unsigned addr) {
+    r[0] = lds_read<OFF>(addr);
+    r[1] = lds_read<OFF + STEP>(addr);
+    r[2] = lds_read<OFF + 2 * STEP>(addr);
+    r[3] = lds_read<OFF + 3 * STEP>(addr);
+}
+template <int OFF>
+__device__ __forceinline__ void lds_write(unsigned addr, f16x8 v) {
+    asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(addr), "v"(v), "i"(OFF) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void lds_wait(u32x4 (&r)[4]) {
     asm volatile("s_waitcnt lgkmcnt(%4)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]) : "i"(N));
 }
-template <int C>
-__device__ __forceinline__ void lds_piece(u32x4 (&r)[4], unsigned addr) {
-    r[0] = lds_read<4096 * C>(addr);
-    r[1] = lds_read<4096 * C + 1024>(addr);
-    r[2] = lds_read<4096 * C + 2048>(addr);
-    r[3] = lds_read<4096 * C + 3072>(addr);
-}
+// A barrier whose LDS accesses before it are done; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int MT>
-__global__ __launch_bounds__(512 / MT, 2 / MT) void kv8_attn_tile_kernel(Params p) {
-    constexpr int WAVES = 8 / MT, PIECES = 32 / WAVES, NS = kTileStages;
-    __shared__ __attribute__((aligned(16))) uint8_t stage[NS * kTileStage];
+__global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p) {
+    __shared__ __attribute__((aligned(16))) TileLds sm;
     const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
     const int4 e0 = it[0], e1 = it[1];
     if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_ITEMS]) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = wave & 3, half = wave >> 2;   // rows 32 rg .. 32 rg + 31, half of the tokens or dims
     const int q16 = lane & 15, g = lane >> 4;
     const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
-    const int pg0 = e1.z, n_pages = e1.w - e1.z;
+    const int pg0 = e1.z, n = e1.w - e1.z;
     const int32_t *table = p.tables + (size_t)seq * p.max_pages;
-    const int w0 = 16 * MT * wave;   // the wave's first row in the block
-    const bool active = w0 < rows;
-    QRow raw[MT];
-    int last[MT], head[MT], tok[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const int fr = row0 + min(w0 + 16 * m + q16, rows - 1);
-        tok[m] = fr / p.group;
-        head[m] = kh * p.group + fr - tok[m] * p.group;
-        load_q(p, q0 + tok[m], head[m], g, raw[m]);
-        last[m] = L + tok[m];
+    int32_t *const flag_row = p.ovf ? p.ovf + q0 : nullptr;
+    auto row_at = [&](int m, int &t, int &head) {
+        const int fr = row0 + min(32 * rg + 16 * m + q16, rows - 1);
+        t = fr / p.group;
+        head = kh * p.group + fr - t * p.group;
+    };
+    // the wave makes the operands of one of its group's two tiles and takes the other's through LDS
+    QRow raw;
+    {
+        int t, head;
+        row_at(half, t, head);
+        load_q(p, q0 + t, head, g, raw);
     }
-    // keys that every row of the wave sees, and the last that any sees
-    const int all_see = L + (row0 + min(w0, rows - 1)) / p.group, any_sees = L + (row0 + min(w0 + 16 * MT, rows) - 1) / p.group;
-    unsigned ids = 0;   // lane j: page (i & ~63) + j
-    float kss = 0.f, vss = 0.f;
+    // lane j: page (i & ~63) + j of the run that is being loaded (ids), or being scored (scales)
+    unsigned ids = 0;
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
-        ids = i < n_pages ? (unsigned)table[pg0 + i] : 0u;
-        if (ids >= (unsigned)p.n_pages) ids = 0;
-        ids = ids * p.nkv + kh;
+        unsigned id = i < n ? (unsigned)table[pg0 + i] : 0u;
+        if (id >= (unsigned)p.n_pages) id = 0;
+        return id * p.nkv + kh;
     };
-    unsigned pofs[PIECES];   // the lane's byte in the page of each piece its wave loads
-#pragma unroll
-    for (int j = 0; j < PIECES; j++) {
-        const int piece = (wave * PIECES + j) & 15;
-        pofs[j] = (piece >> 2) * 4096 + (piece & 3) * 256 + (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;
-    }
-    auto fill = [&](int i) {   // page i into its stage; i & 63 must lie in the looked-up run
-        const size_t at = (size_t)__builtin_amdgcn_readlane(ids, i & 63) * PAGE_BYTES;
-        const uint8_t *src = (wave * PIECES < 16 ? p.k_pages : p.v_pages) + at;
-        uint8_t *dst = stage + (i % NS) * kTileStage + wave * PIECES * 1024;
-#pragma unroll
-        for (int j = 0; j < PIECES; j++) {
-            unsigned off = pofs[j];
-            asm volatile("" : "+v"(off));
-            __builtin_amdgcn_global_load_lds((const void *)(src + off), (lds_ptr *)(dst + 1024 * j), 16, 0, 0);
-        }
+    const unsigned lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;
+    const unsigned pofs = (wave >> 1) * 4096 + (wave & 1) * 512 + lofs;   // pieces 2 wave and 2 wave + 1 of a page
+    u32x4 kr[2], vr[2];
+    auto load = [&](u32x4 (&r)[2], const uint8_t *pages, unsigned at) {
+        const uint8_t *src = pages + (size_t)at * PAGE_BYTES + pofs;
+        r[0] = *(const u32x4 *)src;
+        r[1] = *(const u32x4 *)(src + 256);
     };
-    look_up(0);
-    const unsigned ids0 = ids;
-    kss = p.k_scale[ids0];
-    vss = p.v_scale[ids0];
-    for (int i = 0; i < NS - 1 && i < n_pages; i++) fill(i);
-    f16x8 q[MT][8];
+    auto store = [&](unsigned dst, const u32x4 &r) {   // two LDS writes
+        lds_write<0>(dst, codes_f16(r[0], r[1]));
+        lds_write<1024>(dst, codes_f16(r[2], r[3]));
+    };
+    const unsigned k_out = lds_at(sm.k[4 * wave]) + 16 * lane, v_out = lds_at(sm.v[4 * wave]) + 16 * lane;
+    ids = look_up(0);
+    float kss = p.k_scale[ids], vss = p.v_scale[ids];
+    unsigned id_next = __builtin_amdgcn_readlane(ids, n > 1 ? 1 : 0);   // of page i + 1
+    load(kr, p.k_pages, __builtin_amdgcn_readlane(ids, 0));
+    load(vr, p.v_pages, __builtin_amdgcn_readlane(ids, 0));
+    f16x8 q[2][8];
+    {
+        f16x8 mine[8];
+        make_q(p, raw, g, mine, flag_row);
+        u32x4(*const ex)[64] = sm.k;   // exchanged in the 64 KB of the K and V slots
 #pragma unroll
-    for (int m = 0; m < MT; m++) make_q(p, raw[m], g, q[m], p.ovf ? p.ovf + q0 : nullptr);
-    asm volatile("" : "+v"(kss), "+v"(vss));
-    f32x4 o[MT][16];
-    float mx[MT], sum[MT];
-    int unit = 0;   // o is in units of 2^(unit - 15)
+        for (int c = 0; c < 8; c++) ex[8 * wave + c][lane] = __builtin_bit_cast(u32x4, mine[c]);
+        if (tid < 2) sm.flag[tid] = 0;
+        lds_barrier();
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        mx[m] = kNone;
-        sum[m] = 0.f;
-#pragma unroll
-        for (int d = 0; d < 16; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < 8; c++) {
+            const f16x8 other = __builtin_bit_cast(f16x8, ex[8 * (wave ^ 4) + c][lane]);
+            q[0][c] = half ? other : mine[c];
+            q[1][c] = half ? mine[c] : other;
+        }
+        lds_barrier();
     }
-    const unsigned lds0 = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)stage + 16 * lane;
-    for (int i = 0; i < n_pages; i++) {
-        if (i && (i & 63) == 0) {   // the scales of this page's run (its numbers were looked up with the fills)
-            const int j = i + lane;
-            unsigned id = j < n_pages ? (unsigned)table[pg0 + j] : 0u;
-            if (id >= (unsigned)p.n_pages) id = 0;
-            kss = p.k_scale[(size_t)id * p.nkv + kh];
-            vss = p.v_scale[(size_t)id * p.nkv + kh];
-            asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here, or every page would wait for all fills
-        }
-        // the page has come once at most the fills of the pages behind it are in flight, in every wave
-        if (i + 1 < n_pages) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PIECES * (NS - 2)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const int ahead = i + NS - 1;   // its stage held page i - 1, which every wave is done with
-        if (ahead < n_pages) {
-            if ((ahead & 63) == 0) look_up(ahead);
-            fill(ahead);
-        }
+    store(k_out, kr[0]);
+    store(k_out + 2048, kr[1]);
+    load(kr, p.k_pages, id_next);
+    int last[2];   // the last key that the lane's row of each tile sees
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        int t, head;
+        row_at(m, t, head);
+        last[m] = L + t;
+    }
+    const int all_see = L + (row0 + min(32 * rg, rows - 1)) / p.group;   // keys up to this one are seen by all of the group's rows
+    f32x4 o[2][8], s[2][2];
+    float mx[2] = {kNone, kNone}, sum[2] = {0.f, 0.f}, sum_before[2];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int d = 0; d < 8; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int unit = 0;   // o is in units of 2^(unit - 5)
+    // operand 2 (4 c + t) + h of K: the group's tokens are tiles t = 2 half, 2 half + 1; of V: its dims groups c likewise
+    const unsigned k_in = lds_at(sm.k) + 16 * lane + 4096 * half, v_in = lds_at(sm.v) + 16 * lane + 16384 * half;
+    const unsigned p_in = lds_at(sm.p[rg]) + 16 * lane, flag_in = lds_at(sm.flag);
+    for (int i = 0; i < n; i++) {
         const int pg = pg0 + i;
-        if (active && pg * PAGE <= any_sees) {
-            const unsigned kl = lds0 + (i % NS) * kTileStage;
-            u32x4 r[2][4];
-            f32x4 s[MT][4];
-            lds_piece<0>(r[0], kl);
+        u32x4 r[2][4];
+        lds_barrier();   // K of page i is there, V of page i - 1 is used up
+        lds_read4<0, 1024>(r[0], k_in);       // dims 0-63: tiles' operands (t, h)
+        lds_read4<8192, 1024>(r[1], k_in);    // dims 64-127
+        if ((pg + 1) * PAGE > n_keys) {   // V codes behind the last key may be NaN, whose product with 0 is NaN
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            auto k_step = [&](auto c) {
-                constexpr int C = decltype(c)::value;
-                lds_piece<C + 1>(r[(C + 1) & 1], kl);   // behind K piece 3 lies V piece 0
-                lds_wait<4>(r[C & 1]);
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const u32x4 w = r[C & 1][t];
-                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * C], s[m][t], 0, 0, 0);
-                        s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, q[m][2 * C + 1], s[m][t], 0, 0, 0);
-                    }
-                }
-            };
-            text::static_for<4>(k_step);
-            const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
-            const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;
-            const int key0 = pg * PAGE + 16 * g;
-            f16x8 pb[MT][2];
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                if ((pg + 1) * PAGE > all_see + 1) {
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (key0 + 4 * t + e > last[m]) s[m][t][e] = -INFINITY;
-                }
-                float top = s[m][0][0];
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
-                const float now = fmaxf(mx[m], text::xrow_max(top) * kf);
-                const float f = __builtin_amdgcn_exp2f(mx[m] - now);
-                mx[m] = now;
-                float add = 0.f;
-                const float shift = 15.f - now;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][e], kf, shift));
-                        add += x;
-                        pb[m][t >> 1][4 * (t & 1) + e] = (_Float16)x;
-                    }
-                sum[m] = sum[m] * f + add;
-                const float fo = ldexpf(f, unit - ev);
-                if (__any(fo != 1.f))
-#pragma unroll
-                    for (int d = 0; d < 16; d++) o[m][d] *= fo;
+            for (int w = 0; w < 4; w++) {
+                const unsigned keep = keep_bytes(n_keys - pg * PAGE - 16 * g - 4 * w);
+                vr[0][w] &= keep;
+                vr[1][w] &= keep;
             }
-            unit = ev;
-            const bool tail = (pg + 1) * PAGE > n_keys;
-            auto v_step = [&](auto c) {
-                constexpr int C = decltype(c)::value;
-                if constexpr (C < 3) {
-                    lds_piece<C + 5>(r[(C + 1) & 1], kl);
-                    lds_wait<4>(r[C & 1]);
-                } else lds_wait<0>(r[C & 1]);
-                if (tail) {   // V codes behind the last key, which may be NaN
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const unsigned keep = keep_bytes(n_keys - key0 - 4 * w);
-#pragma unroll
-                        for (int t = 0; t < 4; t++) r[C & 1][t][w] &= keep;
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const u32x4 w = r[C & 1][t];
-                    const f16x8 a = codes_f16(w[0], w[1]), b = codes_f16(w[2], w[3]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        o[m][4 * C + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[m][0], o[m][4 * C + t], 0, 0, 0);
-                        o[m][4 * C + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pb[m][1], o[m][4 * C + t], 0, 0, 0);
-                    }
-                }
-            };
-            text::static_for<4>(v_step);
         }
-    }
+        if (i && (i & 63) == 0) {   // the scales of the next run
+            const unsigned id = look_up(i);
+            kss = p.k_scale[id];
+            vss = p.v_scale[id];
+            asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here and not at every page
+        }
+        const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
+        const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;   // the V scale is 2^ev
+        const int now_unit = abs(ev - unit) <= kUnitSlack ? unit : ev;
+        const float in_unit = kPUnit + (float)(ev - now_unit), out_unit = pow2(now_unit - ev);
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const int row = w0 + 16 * m + q16;
-        const float l = text::xrow_sum(sum[m]);
+        for (int m = 0; m < 2; m++) s[m][0] = s[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // dims 64 c ..: four operands, eight products; V's codes go to LDS between them. Waits count what lies behind
+        // the operands: the next four, and the writes of a piece (two)
+        auto k_part = [&](auto c_t) {
+            constexpr int C = decltype(c_t)::value;
+            lds_wait<C == 0 ? 4 : C == 1 ? 6 : C == 2 ? 8 : 2>(r[C & 1]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const f16x8 a = __builtin_bit_cast(f16x8, r[C & 1][e]);
+#pragma unroll
+                for (int m = 0; m < 2; m++) s[m][e >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[m][2 * C + (e & 1)], s[m][e >> 1], 0, 0, 0);
+            }
+            if constexpr (C < 2) {
+                lds_read4<8192 * (C + 2), 1024>(r[C & 1], k_in);
+                store(v_out + 2048 * C, vr[C]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        text::static_for<4>(k_part);
+        load(vr, p.v_pages, id_next);
+        // P of the page from the scores and the maxima, into LDS; the sum takes it
+        auto make_p = [&]() {
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const float shift = in_unit - mx[m];
+                float x[8], add = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], kf, shift));
+                    add += x[e];
+                }
+                sum_before[m] = sum[m];
+                sum[m] = fmaf(add, out_unit, sum[m]);
+                sm.p[rg][half][m][lane] = u32x4{pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7])};
+            }
+        };
+        const int key0 = pg * PAGE + 16 * g + 8 * half;
+        bool over = false;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            if ((pg + 1) * PAGE > all_see + 1)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (key0 + e > last[m]) s[m][e >> 2][e & 3] = -INFINITY;
+            float top = s[m][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top = fmaxf(top, s[m][e >> 2][e & 3]);
+            top = text::xrow_max(top) * kf;
+            over |= top > mx[m] + kSlack;
+            if (g == 0) sm.top[rg][half][16 * m + q16] = top;
+        }
+        if (__any(over)) sm.flag[i & 1] = 1;
+        make_p();
+        lds_barrier();   // V and P of page i are there, K of it is used up
+        u32x4 pr[4];
+        unsigned moved;
+        asm volatile("ds_read_b32 %0, %1" : "=v"(moved) : "v"(flag_in + 4 * (i & 1)) : "memory");
+        lds_read4<0, 1024>(pr, p_in);         // P operand (half of the tokens, tile)
+        lds_read4<0, 1024>(r[0], v_in);
+        asm volatile("s_waitcnt lgkmcnt(8)" : "+v"(moved));
+        if (__builtin_amdgcn_readfirstlane(moved)) {
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const float f = new_max(mx[m], fmaxf(sm.top[rg][0][16 * m + q16], sm.top[rg][1][16 * m + q16]));
+                sum[m] = sum_before[m] * f;   // without what the first make_p added
+#pragma unroll
+                for (int d = 0; d < 8; d++) o[m][d] *= f;
+            }
+            lds_wait<0>(pr);
+            make_p();
+            lds_barrier();
+            lds_read4<0, 1024>(pr, p_in);
+            lds_read4<0, 1024>(r[0], v_in);
+            lds_wait<0>(pr);
+        }
+        if (unit != now_unit) {
+            const float f = pow2(unit - now_unit);
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int d = 0; d < 8; d++) o[m][d] *= f;
+        }
+        unit = now_unit;
+        lds_wait<4>(pr);
+        lds_read4<4096, 1024>(r[1], v_in);
+        auto v_part = [&](auto c_t) {   // tiles 2 c, 2 c + 1 of the wave's eight: four operands, eight products
+            constexpr int C = decltype(c_t)::value;
+            lds_wait<C == 0 ? 4 : C == 1 ? 6 : C == 2 ? 8 : 2>(r[C & 1]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const f16x8 a = __builtin_bit_cast(f16x8, r[C & 1][e]);
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+                    o[m][2 * C + (e >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, pr[2 * (e & 1) + m]), o[m][2 * C + (e >> 1)], 0, 0, 0);
+            }
+            if constexpr (C < 2) {
+                lds_read4<4096 * (C + 2), 1024>(r[C & 1], v_in);
+                store(k_out + 2048 * C, kr[C]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        text::static_for<4>(v_part);
+        const int ahead = min(i + 2, n - 1);
+        if (ahead == i + 2 && (ahead & 63) == 0) ids = look_up(ahead);
+        id_next = __builtin_amdgcn_readlane(ids, ahead & 63);
+        load(kr, p.k_pages, id_next);
+        if (tid == 0) sm.flag[(i + 1) & 1] = 0;
+    }
+    Gate16 gate[2][2];
+    if (slot < 0)
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            int t, head;
+            row_at(m, t, head);
+#pragma unroll
+            for (int c = 0; c < 2; c++) gate[m][c] = load_gate(p, q0 + t, head, 128 * half + 64 * c + 16 * g);
+        }
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        sum[m] = text::xrow_sum(sum[m]);
+        if (g == 0) sm.sum[rg][half][16 * m + q16] = sum[m];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        const int row = 32 * rg + 16 * m + q16;
         if (row >= rows) continue;
-        const float f = slot < 0 ? ldexpf(1.f / l, unit) : ldexpf(1.f, unit);
+        int t, head;
+        row_at(m, t, head);
+        const float l = sm.sum[rg][0][16 * m + q16] + sm.sum[rg][1][16 * m + q16];
+        const float f = slot < 0 ? pow2(unit) / l : pow2(unit);
         const size_t pr = slot < 0 ? 0 : partial_row(p, slot, kh, row);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
+        for (int c = 0; c < 2; c++) {
+            const int d0 = 128 * half + 64 * c + 16 * g;
             float x[16];
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * t + e] = o[m][4 * c + t][e] * f;
-            if (slot < 0) finish16(p, q0 + tok[m], head[m], 64 * c + 16 * g, x, p.ovf ? p.ovf + q0 : nullptr);
+            for (int e = 0; e < 16; e++) x[e] = o[m][4 * c + (e >> 2)][e & 3] * f;
+            if (slot < 0) finish16(p, q0 + t, head, d0, gate[m][c], x, flag_row);
             else
 #pragma unroll
-                for (int t = 0; t < 4; t++) *(f32x4 *)(p.partial + pr * HD + 64 * c + 16 * g + 4 * t) = f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                for (int e = 0; e < 16; e += 4) *(f32x4 *)(p.partial + pr * HD + d0 + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
         }
-        if (slot >= 0 && g == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mx[m], l);
+        if (slot >= 0 && g == 0 && half == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mx[m], l);
     }
 }
 
@@ -610,6 +749,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
         const int4 blk = ((const int4 *)(p.plan + p.l.blk))[b];
         const int n = blk.y, row = fr - blk.z;
         if (n <= 1) continue;   // the whole workgroup skips it
+        const Gate16 gate = load_gate(p, t, head, 16 * (tid & 15));
         const int q0 = t - tok.y;
         const float *ml = partial_ml(p);
         float top = kNone;
@@ -635,7 +775,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
             const float inv = 1.f / (ls[0] + ls[1] + ls[2] + ls[3]);
 #pragma unroll
             for (int i = 0; i < 16; i++) x[i] = (os[0][16 * tid + i] + os[1][16 * tid + i] + os[2][16 * tid + i] + os[3][16 * tid + i]) * inv;
-            finish16(p, t, head, 16 * tid, x, p.ovf ? p.ovf + q0 : nullptr);
+            finish16(p, t, head, 16 * tid, gate, x, p.ovf ? p.ovf + q0 : nullptr);
         }
         __syncthreads();
     }

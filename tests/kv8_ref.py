@@ -64,8 +64,8 @@ def attend(q, gate, k, v, first, scale, use_gate):
     """Causal attention of queries at tokens first, first + 1, ... ([n][nh][256]) over keys [nkv][N][256]: the outputs
     [n][nh][256], and how far f16 queries and f16 weights may move each: a query element is off by at most half
     a step, 2^-11 of itself (2^-18 more for the f32 norm, rotary and sums), which moves a score by at most
-    that share of sum |q k| * scale = d and a weight by exp(2 d); a weight's own rounding is 2^-11 of it. The
-    output's rounding comes on top."""
+    that share of sum |q k| * scale = d and a weight by exp(2 d); a weight's own rounding is 2^-11 of it, or 2^-28 of
+    the row's largest where that is more (half of f16's smallest step, of weights held times 2^3 at least). The output's rounding comes on top."""
     n, nh = q.shape[:2]
     group = nh // k.shape[0]
     out, off = np.zeros_like(q), np.zeros_like(q)
@@ -78,7 +78,8 @@ def attend(q, gate, k, v, first, scale, use_gate):
             w /= w.sum()
             out[i, h] = w @ vv[:m]
             d = (np.abs(kk[:m]) @ np.abs(q[i, h])).max() * scale * (2.0 ** -11 + 2.0 ** -18)
-            off[i, h] = (w @ np.abs(vv[:m])) * (np.expm1(2 * d) + 2.0 ** -11 * np.exp(2 * d) + 2.0 ** -16)
+            off[i, h] = (w @ np.abs(vv[:m])) * (np.expm1(2 * d) + 2.0 ** -11 * np.exp(2 * d) + 2.0 ** -16) \
+                + 2.0 ** -28 * w.max() * np.abs(vv[:m]).sum(0)
     if use_gate:
         g = 1 / (1 + np.exp(-gate))
         out, off = out * g, off * g + np.abs(out * g) * 2.0 ** -20

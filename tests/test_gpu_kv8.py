@@ -92,7 +92,8 @@ def _run(nh, nkv, passes, seed=0, n_rot=64, norm=True, gate=True, out_dtype="bf1
         assert np.array_equal(_np(cache.free)[:model.n_free], model.free[:model.n_free])
         q, k, v, g = ref.rows(_np(qkv.float()), nh, nkv, n_rot, None if qn is None else _np(qn), None if kn is None else _np(kn), pos3, theta)
         values = _cache_values(cache)
-        for r, n in enumerate(new):   # the new tokens' codes: half a step of their page's scale (2^-12 more for f32 arithmetic before them)
+        for r, n in enumerate(new):   # the new tokens' codes: half a step of their page's scale (and f32 arithmetic before them: 2^-12
+            # of it, and 2^-19 of the row for the rotation)
             if n <= 0:
                 continue
             L = before[r]
@@ -100,7 +101,7 @@ def _run(nh, nkv, passes, seed=0, n_rot=64, norm=True, gate=True, out_dtype="bf1
             page = model.tables[r, np.arange(L, L + n) // PAGE]
             for got, x, s in ((kk[:, L:], k[cu[r]:cu[r + 1]], values[2][page]), (vv[:, L:], v[cu[r]:cu[r + 1]], values[3][page])):
                 x = x.transpose(1, 0, 2)
-                room = np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s.T[..., None]) * (1 + 2.0 ** -12) + 2.0 ** -20 * np.abs(x)
+                room = np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s.T[..., None]) * (1 + 2.0 ** -12) + 2.0 ** -19 * np.abs(x).max(-1, keepdims=True)
                 assert (np.abs(got - x) <= room).all(), f"codes of sequence {r}"
         _check_attention(out, before, new, cu, q, g, cache, model, values, HD ** -0.5, gate, out_dtype)
         assert (out[T - 2:] == 7.0).all(), "rows behind the last sequence changed"
@@ -137,6 +138,39 @@ def test_variants(out_dtype, n_rot, norm, gate):
 def test_sharp_rows_and_row_stride():
     """Keys that dominate their rows (large queries and keys, no norm), and rows wider than needed."""
     _run(8, 4, [[90], [1], [7]], n_rot=0, norm=False, scale=4.0, extra=24, seed=8)
+
+
+@pytest.mark.parametrize("new", [[1], [40]])
+@pytest.mark.parametrize("where", ["first", "last"])
+def test_many_small_weights(new, where):
+    """One key outweighs each other one by 2^23, and together they make 0.4% of the output: weights far below the
+    largest still count, whether the largest comes before or behind them."""
+    nh, nkv, n = 2, 1, 32768
+    _say("small weights", new, where)
+    cache, model = Kv8Cache(1, nkv, 520, 1, 520), ref.Cache(520, 1, 520)
+    att = TextAttention(nh, nkv, HD, 0)
+    plan = Kv8Plan(cache, n, nh)
+    plan.update(_int([n]))
+    model.plan([n], n)
+    qkv = torch.zeros(n, att.row, dtype=torch.bfloat16, device="cuda")
+    qkv[:, 2 * nh * HD + HD:] = 1.0                                   # every value 1
+    at = 5 if where == "first" else n - 3
+    qkv[at, 2 * nh * HD] = 16.0                                       # one key of length 16, its value 0
+    qkv[at, 2 * nh * HD + HD:] = 0
+    att.forward_kv8(qkv, None, None, None, plan, cache, 0, stage="append")
+    T = new[0]
+    plan = Kv8Plan(cache, T, nh, T)
+    plan.update(_int(new))
+    model.plan(new, T)
+    q = torch.zeros(T, att.row, dtype=torch.bfloat16, device="cuda")
+    q[:, 0] = q[:, 2 * HD] = 16.0                                     # scores 16 = 23.08 in log2, and 0
+    out = att.forward_kv8(q, None, None, None, plan, cache, 0, gate=False)
+    torch.cuda.synchronize()
+    rest = np.arange(T)[:, None] + n - 1                              # other keys of value 1 (the new ones' values are 0)
+    w = np.exp(-16.0)
+    want = (n - 1) * w / (1 + rest * w + w)
+    # each weight w is off by at most 2^-11 of itself (f16), the output by 2^-8
+    assert (np.abs(_np(out.float()) - want) <= want * (2.0 ** -11 + 2.0 ** -8 + 2.0 ** -16)).all()
 
 
 @pytest.mark.parametrize("magnitude", [2.0 ** -90, 2.0 ** -40, 1.0, 2.0 ** 9])
