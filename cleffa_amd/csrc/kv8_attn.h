@@ -36,10 +36,11 @@ constexpr float kNone = -1e30f;   // a running maximum before any key: below eve
 // difference goes into P's exponent. P is then held as 2^(5 + ev - unit) P in f16, 2^15 at most.
 constexpr float kPUnit = 5.f, kSlack = 8.f;
 constexpr int kUnitSlack = 2;
+constexpr float kPMost = 8192.f;   // 2^(5 + 8): a weight as large as the slack allows, of a page in its own unit
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
-// Moves m for a page whose largest score is top; returns the factor that sums under the old m take.
-__device__ __forceinline__ float new_max(float &m, float top) {
-    const float now = top > m + kSlack ? top : m;
+// Moves m for a page whose largest score top passes it by more than the slack; returns the factor that sums under the old m take.
+__device__ __forceinline__ float new_max(float &m, float top, float slack) {
+    const float now = top > m + slack ? top : m;
     const float f = __builtin_amdgcn_exp2f(m - now);
     m = now;
     return f;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
-            const float f = new_max(mx[m], text::xrow_max(top) * kf);
+            const float f = new_max(mx[m], text::xrow_max(top) * kf, kSlack);
             float add = 0.f;
             const float shift = kPUnit + (float)(ev - now_unit) - mx[m];
 #pragma unroll
@@ -435,9 +436,9 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 // Two phases a page, a barrier behind each: scores and softmax of page i while its V is written to LDS, then
 // O += P V while K of page i + 1 is; so one slot of 32 KB is enough for each. Codes come into registers a page ahead.
 //
-// The maximum of a row is common to its two waves. A wave whose page passes it by more than the slack says so in a
-// flag; behind the barrier all waves then take the pairs' new maxima and make that page's P again (the first page,
-// and hardly ever after).
+// The maximum of a row is common to its two waves, and no page's own maximum is looked for while weights stay small: a
+// wave whose sums of eight weights pass what the slack allows says so in a flag; behind the barrier all waves then
+// take the pairs' new maxima and make that page's P again (the first page, and hardly ever after).
 constexpr int kTileThreads = 512;
 struct TileLds {
     u32x4 k[32][64], v[32][64];   // operand [2 (4 c + t) + h][lane]
@@ -468,6 +469,10 @@ __device__ __forceinline__ void lds_write(unsigned addr, f16x8 v) {
 template <int N>
 __device__ __forceinline__ void lds_wait(u32x4 (&r)[4]) {
     asm volatile("s_waitcnt lgkmcnt(%4)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]) : "i"(N));
+}
+template <int N>
+__device__ __forceinline__ void lds_wait2(u32x4 (&r)[4], u32x4 &a, u32x4 &b) {
+    asm volatile("s_waitcnt lgkmcnt(%6)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(a), "+v"(b) : "i"(N));
 }
 // A barrier whose LDS accesses before it are done; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -553,15 +558,16 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
     }
     const int all_see = L + (row0 + min(32 * rg, rows - 1)) / p.group;   // keys up to this one are seen by all of the group's rows
     f32x4 o[2][8], s[2][2];
-    float mx[2] = {kNone, kNone}, sum[2] = {0.f, 0.f}, sum_before[2];
+    float mx[2] = {kNone, kNone}, sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int d = 0; d < 8; d++) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     int unit = 0;   // o is in units of 2^(unit - 5)
     // operand 2 (4 c + t) + h of K: the group's tokens are tiles t = 2 half, 2 half + 1; of V: its dims groups c likewise
-    const unsigned k_in = lds_at(sm.k) + 16 * lane + 4096 * half, v_in = lds_at(sm.v) + 16 * lane + 16384 * half;
-    const unsigned p_in = lds_at(sm.p[rg]) + 16 * lane, flag_in = lds_at(sm.flag);
+    const unsigned k_in = lds_at(sm.k) + 16 * lane + 4096 * half;
+    const unsigned v_own = lds_at(sm.v) + 16 * lane + (16384 + 1024) * half, v_other = lds_at(sm.v) + 16 * lane + 16384 * half + 1024 * (half ^ 1);
+    const unsigned p_in = lds_at(sm.p[rg][half ^ 1]) + 16 * lane, flag_in = lds_at(sm.flag);
     for (int i = 0; i < n; i++) {
         const int pg = pg0 + i;
         u32x4 r[2][4];
@@ -607,60 +613,63 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
         };
         text::static_for<4>(k_part);
         load(vr, p.v_pages, id_next);
-        // P of the page from the scores and the maxima, into LDS; the sum takes it
+        const int key0 = pg * PAGE + 16 * g + 8 * half;
+        if ((pg + 1) * PAGE > all_see + 1)
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (key0 + e > last[m]) s[m][e >> 2][e & 3] = -INFINITY;
+        // P of the page from the scores and the maxima: the own half stays in registers, both lie in LDS
+        f16x8 pb[2];
+        float add[2];
         auto make_p = [&]() {
 #pragma unroll
             for (int m = 0; m < 2; m++) {
                 const float shift = in_unit - mx[m];
-                float x[8], add = 0.f;
+                float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], kf, shift));
-                    add += x[e];
-                }
-                sum_before[m] = sum[m];
-                sum[m] = fmaf(add, out_unit, sum[m]);
-                sm.p[rg][half][m][lane] = u32x4{pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7])};
+                for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], kf, shift));
+                add[m] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+                pb[m] = __builtin_bit_cast(f16x8, u32x4{pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7])});
+                sm.p[rg][half][m][lane] = __builtin_bit_cast(u32x4, pb[m]);
             }
         };
-        const int key0 = pg * PAGE + 16 * g + 8 * half;
-        bool over = false;
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            if ((pg + 1) * PAGE > all_see + 1)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (key0 + e > last[m]) s[m][e >> 2][e & 3] = -INFINITY;
-            float top = s[m][0][0];
-#pragma unroll
-            for (int e = 1; e < 8; e++) top = fmaxf(top, s[m][e >> 2][e & 3]);
-            top = text::xrow_max(top) * kf;
-            over |= top > mx[m] + kSlack;
-            if (g == 0) sm.top[rg][half][16 * m + q16] = top;
-        }
-        if (__any(over)) sm.flag[i & 1] = 1;
         make_p();
+        // no weight of the page is past the slack while the sums of eight are not
+        if (__any(fmaxf(add[0], add[1]) > kPMost)) sm.flag[i & 1] = 1;
         lds_barrier();   // V and P of page i are there, K of it is used up
-        u32x4 pr[4];
+        u32x4 pr[2];     // the other half's P operands
         unsigned moved;
         asm volatile("ds_read_b32 %0, %1" : "=v"(moved) : "v"(flag_in + 4 * (i & 1)) : "memory");
-        lds_read4<0, 1024>(pr, p_in);         // P operand (half of the tokens, tile)
-        lds_read4<0, 1024>(r[0], v_in);
-        asm volatile("s_waitcnt lgkmcnt(8)" : "+v"(moved));
+        pr[0] = lds_read<0>(p_in);
+        pr[1] = lds_read<1024>(p_in);
+        lds_read4<0, 2048>(r[0], v_own);
+        asm volatile("s_waitcnt lgkmcnt(6)" : "+v"(moved));
         if (__builtin_amdgcn_readfirstlane(moved)) {
+            lds_wait2<0>(r[0], pr[0], pr[1]);   // no read may land in a register that is used anew
+            float top[2];
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                const float f = new_max(mx[m], fmaxf(sm.top[rg][0][16 * m + q16], sm.top[rg][1][16 * m + q16]));
-                sum[m] = sum_before[m] * f;   // without what the first make_p added
+                top[m] = s[m][0][0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) top[m] = fmaxf(top[m], s[m][e >> 2][e & 3]);
+                top[m] = text::xrow_max(top[m]) * kf;
+                if (g == 0) sm.top[rg][half][16 * m + q16] = top[m];
+            }
+            lds_barrier();
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const float f = new_max(mx[m], fmaxf(sm.top[rg][0][16 * m + q16], sm.top[rg][1][16 * m + q16]), 0.f);
+                sum[m] *= f;
 #pragma unroll
                 for (int d = 0; d < 8; d++) o[m][d] *= f;
             }
-            lds_wait<0>(pr);
             make_p();
             lds_barrier();
-            lds_read4<0, 1024>(pr, p_in);
-            lds_read4<0, 1024>(r[0], v_in);
-            lds_wait<0>(pr);
+            pr[0] = lds_read<0>(p_in);
+            pr[1] = lds_read<1024>(p_in);
+            lds_read4<0, 2048>(r[0], v_own);
         }
         if (unit != now_unit) {
             const float f = pow2(unit - now_unit);
@@ -670,20 +679,25 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
                 for (int d = 0; d < 8; d++) o[m][d] *= f;
         }
         unit = now_unit;
-        lds_wait<4>(pr);
-        lds_read4<4096, 1024>(r[1], v_in);
-        auto v_part = [&](auto c_t) {   // tiles 2 c, 2 c + 1 of the wave's eight: four operands, eight products
+#pragma unroll
+        for (int m = 0; m < 2; m++) sum[m] = fmaf(add[m], out_unit, sum[m]);
+        lds_read4<8192, 2048>(r[1], v_own);
+        // first the own tokens' products (tiles 4 c ..), then the other half's; K's codes go to LDS between them
+        auto v_part = [&](auto c_t) {
             constexpr int C = decltype(c_t)::value;
-            lds_wait<C == 0 ? 4 : C == 1 ? 6 : C == 2 ? 8 : 2>(r[C & 1]);
+            if constexpr (C == 2) lds_wait2<8>(r[0], pr[0], pr[1]);
+            else lds_wait<C == 0 ? 4 : C == 1 ? 6 : 2>(r[C & 1]);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const f16x8 a = __builtin_bit_cast(f16x8, r[C & 1][e]);
 #pragma unroll
-                for (int m = 0; m < 2; m++)
-                    o[m][2 * C + (e >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, pr[2 * (e & 1) + m]), o[m][2 * C + (e >> 1)], 0, 0, 0);
+                for (int m = 0; m < 2; m++) {
+                    const f16x8 w = C < 2 ? pb[m] : __builtin_bit_cast(f16x8, pr[m]);
+                    o[m][4 * (C & 1) + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w, o[m][4 * (C & 1) + e], 0, 0, 0);
+                }
             }
             if constexpr (C < 2) {
-                lds_read4<4096 * (C + 2), 1024>(r[C & 1], v_in);
+                lds_read4<8192 * C, 2048>(r[C & 1], v_other);
                 store(k_out + 2048 * C, kr[C]);
             }
             __builtin_amdgcn_sched_barrier(0);
