@@ -159,8 +159,12 @@ bool clef_hip_kv8_read(const clef_hip_kv8_read_args *a, void *stream, char *err,
     p.tables = a->tables; p.state = a->state; p.first_page = a->first_page; p.cu = a->cu;
     p.k_plane = a->k_plane; p.vt_plane = a->vt_plane;
     p.n_seq = a->n_seq; p.max_pages = a->max_pages; p.n_pages = a->n_pages; p.nkv = a->nkv; p.kvT = a->kvT;
-    const long pieces = (long)a->kvT / CLEF_HIP_KV8_PAGE + a->n_seq;
-    hipLaunchKernelGGL(kv8::kv8_read_kernel, dim3((unsigned)(pieces * a->nkv)), dim3(kv8::kReadThreads), 0, (hipStream_t)stream, p);
+    const long pages = (long)a->kvT / CLEF_HIP_KV8_PAGE + a->n_seq;
+    if (pages * a->nkv < 8L * kCus)
+        hipLaunchKernelGGL(kv8::kv8_read_kernel<1>, dim3((unsigned)(pages * a->nkv)), dim3(256), 0, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL(kv8::kv8_read_kernel<2>, dim3((unsigned)(((long)a->kvT / (2 * CLEF_HIP_KV8_PAGE) + a->n_seq) * a->nkv)), dim3(512), 0,
+                           (hipStream_t)stream, p);
     return launch_ok("kv8_read", err, errlen);
 }
 

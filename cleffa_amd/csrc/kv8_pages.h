@@ -240,57 +240,63 @@ __device__ __forceinline__ u32x4 to_bf16(unsigned a, unsigned b, float s) {
     return o;
 }
 
-// Pages back into 16-bit planes. Workgroup (piece, kv head): piece i belongs to the last sequence r with
-// cu[r] / 64 + r <= i and is that sequence's page i - cu[r] / 64 - r (from first_page on): sequence r has
-// cu[r + 1] / 64 - cu[r] / 64 + 1 pieces, enough for its (cu[r + 1] - cu[r] + 63) / 64 pages.
-constexpr int kReadThreads = 256;
-__global__ __launch_bounds__(kReadThreads) void kv8_read_kernel(ReadParams p) {
+// Pages back into 16-bit planes. Workgroup (piece, kv head): NP pages, N = 64 NP tokens. Piece i belongs to the last
+// sequence r with cu[r] / N + r <= i and is its pages NP (i - cu[r] / N - r) and up (from first_page on): sequence r
+// has cu[r + 1] / N - cu[r] / N + 1 pieces, enough for its cu[r + 1] - cu[r] rows. The sequence is found by all threads
+// counting at once, a search's loads one after the other would take longer than the copy. Bound by memory (a byte
+// in, two out): every load and store instruction of a wave covers whole lines, a lane taking eight codes to sixteen
+// bytes. Two pages make 256 bytes of a V^T row (79,000 tokens, 4 heads: 120.5 -> 106.6 us, 4.6 TB/s), which small reads
+// lack the workgroups for (4,091 tokens: 7.3 -> 9.1 us): the launch takes two from 8 workgroups a CU on.
+template <int NP>
+__global__ __launch_bounds__(256 * NP) void kv8_read_kernel(ReadParams p) {
+    constexpr int kReadThreads = 256 * NP, kReadTokens = PAGE * NP, LANES = 8 * NP;   // lanes a V^T row
     const int kh = blockIdx.x % p.nkv, piece = blockIdx.x / p.nkv, tid = threadIdx.x;
-    int r = 0, end = p.n_seq;
-    while (end - r > 1) {
-        const int mid = (r + end) >> 1;
-        if ((p.cu[mid] >> 6) + mid <= piece) r = mid;
-        else end = mid;
+    int r = -1;
+    for (int r0 = 0; r0 < p.n_seq; r0 += kReadThreads) {
+        const int i = r0 + tid;
+        r += __syncthreads_count(i < p.n_seq && p.cu[i] / kReadTokens + i <= piece);
     }
-    const int row0 = p.cu[r], j = piece - (row0 >> 6) - r;
+    if (r < 0) return;
+    const int row0 = p.cu[r], j = piece - row0 / kReadTokens - r;
     const int first = p.first_page ? p.first_page[r] : 0;
-    const long pg = (long)first + j;
+    const long pg = (long)first + NP * j;
     if (j < 0 || row0 < 0 || row0 % 8 || first < 0 || pg >= p.max_pages) return;
-    // rows of this page: the sequence's tokens, the room of its plane rows and the plane's end bound them
-    const long left = (long)min(p.cu[r + 1], p.kvT) - row0 - (long)j * PAGE;
-    const int n = (int)min(min(left, (long)p.state[2 + 2 * r] - pg * PAGE), (long)PAGE);
+    // rows of the piece: the sequence's tokens, the room of its plane rows, the plane's end and the table's bound them
+    const long left = (long)min(p.cu[r + 1], p.kvT) - row0 - (long)j * kReadTokens;
+    const long have = min((long)p.state[2 + 2 * r], (long)p.max_pages * PAGE) - pg * PAGE;
+    const int n = (int)min(min(left, have), (long)kReadTokens);
     if (n <= 0) return;
-    const int page = p.tables[(size_t)r * p.max_pages + pg];
-    if ((unsigned)page >= (unsigned)p.n_pages) return;
-    const size_t at = (size_t)page * p.nkv + kh;
-    const uint8_t *kp = p.k_pages + at * PAGE_BYTES, *vp = p.v_pages + at * PAGE_BYTES;
-    const float ks = p.k_scale[at], vs = p.v_scale[at];
-    const size_t base = (size_t)row0 + (size_t)j * PAGE;
-    // K: thread (token, 16 dims); V: thread (dim, 16 tokens): four of each
-    u32x4 k[4], v[4];
+    const int32_t *table = p.tables + (size_t)r * p.max_pages + pg;
+    const unsigned page0 = (unsigned)table[0], page1 = NP > 1 && n > PAGE ? (unsigned)table[1] : page0;
+    if (page0 >= (unsigned)p.n_pages || page1 >= (unsigned)p.n_pages) return;
+    const size_t at0 = (size_t)page0 * p.nkv + kh, at1 = (size_t)page1 * p.nkv + kh;
+    const float ks0 = p.k_scale[at0], ks1 = p.k_scale[at1], vs0 = p.v_scale[at0], vs1 = p.v_scale[at1];
+    const size_t base = (size_t)row0 + (size_t)j * kReadTokens;
+    // K: thread (token, 8 dims), 32 lanes a row; V: thread (dim, 8 tokens)
+    uint2 k[8], v[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int id = tid + kReadThreads * i, tok = id >> 4, part = id & 15;
-        k[i] = *(const u32x4 *)(kp + (part >> 2) * 4096 + tok * 64 + (part & 3) * 16);
-        v[i] = *(const u32x4 *)(vp + 16 * id);
+    for (int i = 0; i < 8; i++) {
+        const int id = tid + kReadThreads * i, tok = id >> 5, part = id & 31, t8 = id % LANES;
+        k[i] = *(const uint2 *)(p.k_pages + (tok < PAGE ? at0 : at1) * PAGE_BYTES + (part >> 3) * 4096 + (tok & 63) * 64 + (part & 7) * 8);
+        v[i] = *(const uint2 *)(p.v_pages + (t8 < 8 ? at0 : at1) * PAGE_BYTES + id / LANES * PAGE + (t8 & 7) * 8);
+    }
+    uint16_t *const k_dst = p.k_plane + ((size_t)kh * p.kvT + base) * HD;
+    uint16_t *const v_dst = p.vt_plane + (size_t)kh * HD * p.kvT + base;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int id = tid + kReadThreads * i, tok = id >> 5, part = id & 31;
+        if (tok < n) __builtin_nontemporal_store(to_f16(k[i].x, k[i].y, tok < PAGE ? ks0 : ks1), (u32x4 *)(k_dst + tok * HD + 8 * part));
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int id = tid + kReadThreads * i, tok = id >> 4, part = id & 15;
-        if (tok < n) {
-            uint16_t *dst = p.k_plane + ((size_t)kh * p.kvT + base + tok) * HD + 16 * part;
-            *(u32x4 *)dst = to_f16(k[i][0], k[i][1], ks);
-            *(u32x4 *)(dst + 8) = to_f16(k[i][2], k[i][3], ks);
-        }
-        const int d = id >> 2, t0 = (id & 3) * 16;
-        uint16_t *dst = p.vt_plane + ((size_t)kh * HD + d) * p.kvT + base + t0;
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const int m = n - t0 - 8 * q;
-            const u32x4 w = to_bf16(v[i][2 * q], v[i][2 * q + 1], vs);
-            if (m >= 8) *(u32x4 *)(dst + 8 * q) = w;
-            else
-                for (int e = 0; e < m; e++) dst[8 * q + e] = (uint16_t)(w[e / 2] >> 16 * (e & 1));
+    for (int i = 0; i < 8; i++) {
+        const int id = tid + kReadThreads * i, d = id / LANES, t0 = 8 * (id % LANES), m = n - t0;
+        uint16_t *dst = v_dst + (size_t)d * p.kvT + t0;
+        const u32x4 w = to_bf16(v[i].x, v[i].y, t0 < PAGE ? vs0 : vs1);
+        if (m >= 8) __builtin_nontemporal_store(w, (u32x4 *)dst);
+        else if (m > 0) {   // the last tokens: four, two, one
+            if (m & 4) *(uint2 *)dst = make_uint2(w[0], w[1]);
+            if (m & 2) *(unsigned *)(dst + (m & 4)) = m & 4 ? w[2] : w[0];
+            if (m & 1) dst[m - 1] = (uint16_t)(m & 4 ? (m & 2 ? w[3] : w[2]) : (m & 2 ? w[1] : w[0]));
         }
     }
 }
