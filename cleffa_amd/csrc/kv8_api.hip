@@ -116,7 +116,11 @@ bool clef_hip_kv8_plan(const clef_hip_kv8_plan_args *a, void *stream, char *err,
     p.n_seq = a->n_seq; p.max_pages = a->max_pages; p.n_pages = a->n_pages; p.T = a->T; p.group = a->nh / a->nkv;
     p.tables = a->tables; p.free_pages = a->free_pages; p.state = a->state; p.state_out = a->state_out;
     p.new_lens = a->new_lens; p.pos_off = a->pos_off; p.cu_q = a->cu_q; p.slots = a->slots; p.pos3 = a->pos3; p.work = a->plan;
-    hipLaunchKernelGGL(kv8::kv8_plan_kernel, dim3(1), dim3(kv8::kPlanThreads), 0, (hipStream_t)stream, p);
+    if (a->n_seq <= 256 && a->T <= 256) hipLaunchKernelGGL(kv8::kv8_plan_kernel<256>, dim3(1), dim3(256), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL(kv8::kv8_plan_kernel<1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, p);
+    if (!launch_ok("kv8_plan", err, errlen)) return false;
+    if (a->T <= 1024) return true;
+    hipLaunchKernelGGL(kv8::kv8_plan_rows_kernel, dim3((unsigned)((a->T + kv8::kRowThreads - 1) / kv8::kRowThreads)), dim3(kv8::kRowThreads), 0, (hipStream_t)stream, p);
     return launch_ok("kv8_plan", err, errlen);
 }
 

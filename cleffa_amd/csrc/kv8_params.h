@@ -23,6 +23,7 @@ constexpr int32_t kPlanMagic = 0x4b563850;     // 'KV8P'
 enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_ITEMS, H_BLOCKS, H_SPLIT, H_WORDS = 16 };
 
 // Where the parts of a plan buffer lie (in int32) and how many entries each can need:
+//  the first block of each sequence (of passes whose rows a second kernel writes);
 //  append items {page, pass row of its first new token, slot of that token in the page | count << 8, first
 //  pass row of its sequence}, one for each page that a sequence's new tokens touch: at most one per
 //  token and (n - 1) / 64 + 2 per sequence of n;
@@ -35,7 +36,7 @@ enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_IT
 // blocks: items <= blocks + budget, and those of cut blocks (split slots; p >= 1.5 C) <= 4 W / (3 C) < 2 budget.
 struct Layout {
     int bm, budget, least, max_app, max_blk, max_items, max_slots;
-    long app, tok, blk, items, ints;
+    long seq_blk, app, tok, blk, items, ints;
     size_t ws_bytes;
 };
 inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
@@ -50,7 +51,8 @@ inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
     l.max_blk = (int)((long)T * G / l.bm) + (n_seq < T ? n_seq : T);
     l.max_items = l.max_blk + l.budget;
     l.max_slots = 2 * l.budget;
-    l.app = H_WORDS;
+    l.seq_blk = H_WORDS;
+    l.app = (l.seq_blk + n_seq + 3) / 4 * 4;
     l.tok = l.app + 4L * l.max_app;
     l.blk = (l.tok + 2L * T + 3) / 4 * 4;
     l.items = (l.blk + 4L * l.max_blk + 7) / 8 * 8;
