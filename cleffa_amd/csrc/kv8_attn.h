@@ -54,17 +54,6 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
 // The first n bytes of a word (n below 0 or above 4: none, all).
 __device__ __forceinline__ unsigned keep_bytes(int n) { return n <= 0 ? 0u : ~0u >> 8 * (4 - min(n, 4)); }
 
-// sin and cos of an angle by the hardware functions of revolutions, the fraction exact in two products: 4e-7 off at
-// most up to 10^6 (measured over 4 million angles), against 5e-4 of an f16 operand.
-__device__ __forceinline__ void rope_turns(float x, float *s, float *c) {
-    constexpr double kTurn = 0.15915494309189535;   // 1 / (2 pi)
-    constexpr float C1 = (float)kTurn, C2 = (float)(kTurn - (double)C1);
-    const float j = __builtin_rintf(x * C1);
-    const float r = fmaf(x, C2, fmaf(x, C1, -j));
-    *s = __builtin_amdgcn_sinf(r);
-    *c = __builtin_amdgcn_cosf(r);
-}
-
 // One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
 // 2c (e < 8) and 2c + 1. Two steps, so that other loads can go out between them: the row as it is, then norm and
 // rotary in f32 and f16 with split16's saturation (flagged).

@@ -44,6 +44,17 @@ __device__ __forceinline__ bool saturate(float &x, float lim) {
     return bad;
 }
 
+// sin and cos of an angle by the hardware functions of revolutions, the fraction exact in two products: 4e-7 off at
+// most up to 10^6 (measured over 4 million angles), against 5e-4 of an f16 operand and 6e-2 of a code.
+__device__ __forceinline__ void rope_turns(float x, float *s, float *c) {
+    constexpr double kTurn = 0.15915494309189535;   // 1 / (2 pi)
+    constexpr float C1 = (float)kTurn, C2 = (float)(kTurn - (double)C1);
+    const float j = __builtin_rintf(x * C1);
+    const float r = fmaf(x, C2, fmaf(x, C1, -j));
+    *s = __builtin_amdgcn_sinf(r);
+    *c = __builtin_amdgcn_cosf(r);
+}
+
 // The page's new scale from each thread's largest magnitude; old rows keep the page's scale as a floor.
 __device__ __forceinline__ float shared_scale(float most, float before, float *red) {
 #pragma unroll
@@ -61,8 +72,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
     __shared__ float red[4];
     const int kh = blockIdx.x % p.nkv, item = blockIdx.x / p.nkv, tid = threadIdx.x;
     const int32_t *h = p.plan;
+    const int4 it = ((const int4 *)(p.plan + p.l.app))[item];   // with the header, not behind it: the grid ends with the list's room
     if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_APPEND]) return;
-    const int4 it = ((const int4 *)(p.plan + p.l.app))[item];
     const int page = it.x, t0 = it.y, off = it.z & 0xff, n = it.z >> 8, flag = it.w;
     if ((unsigned)page >= (unsigned)p.n_pages) return;
     const size_t at = (size_t)page * p.nkv + kh;
@@ -74,29 +85,37 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
         const int k = tid & 15, rr = tid >> 4;
         const int d0 = k < 4 ? 8 * k : 64 + 16 * (k - 4), d1 = k < 4 ? 32 + 8 * k : d0 + 8;
         const uint16_t *src = p.qkv + (size_t)p.nh * 2 * HD + (size_t)kh * HD;
-        float x[4][16];
+        u32x4 raw[4][2];
+        int pos[4][3];
+        float w[16], freq[8];
 #pragma unroll
         for (int m = 0; m < 4; m++) {
-            const int j = 16 * m + rr;
             if (16 * m >= n) break;
-            const uint16_t *row = src + (size_t)(t0 + min(j, n - 1)) * p.row;
-            const u32x4 a = *(const u32x4 *)(row + d0), b = *(const u32x4 *)(row + d1);
+            const int t = t0 + min(16 * m + rr, n - 1);
+            raw[m][0] = *(const u32x4 *)(src + (size_t)t * p.row + d0);
+            raw[m][1] = *(const u32x4 *)(src + (size_t)t * p.row + d1);
+            if (p.n_rot)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[m][2 * i] = bf_lo(a[i]);
-                x[m][2 * i + 1] = bf_hi(a[i]);
-                x[m][8 + 2 * i] = bf_lo(b[i]);
-                x[m][8 + 2 * i + 1] = bf_hi(b[i]);
-            }
+                for (int c = 0; c < 3; c++) pos[m][c] = p.pos3[3 * (size_t)t + c];
         }
-        float w[16];
         if (p.k_norm)
 #pragma unroll
             for (int i = 0; i < 16; i++) w[i] = p.k_norm[(i < 8 ? d0 : d1) + (i & 7)];
+        if (p.n_rot)
+#pragma unroll
+            for (int e = 0; e < 8; e++) freq[e] = p.inv_freq[(8 * k + e) & 31];
+        const float before = off ? p.k_scale[at] : 0.f;
+        float x[4][16];
 #pragma unroll
         for (int m = 0; m < 4; m++) {
             if (16 * m >= n) break;
-            const int j = 16 * m + rr, t = t0 + min(j, n - 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[m][2 * i] = bf_lo(raw[m][0][i]);
+                x[m][2 * i + 1] = bf_hi(raw[m][0][i]);
+                x[m][8 + 2 * i] = bf_lo(raw[m][1][i]);
+                x[m][9 + 2 * i] = bf_hi(raw[m][1][i]);
+            }
             if (p.k_norm) {
                 float ss = 0.f;
 #pragma unroll
@@ -108,21 +127,27 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
             if (p.n_rot && k < 4) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const int i = 8 * k + e;
+                    const int axis = (8 * k + e) % 3;
                     float sn, cn;
-                    rope_sincos((float)p.pos3[3 * (size_t)t + i % 3] * p.inv_freq[i], &sn, &cn);
+                    rope_turns((float)(axis == 0 ? pos[m][0] : axis == 1 ? pos[m][1] : pos[m][2]) * freq[e], &sn, &cn);
                     const float a = x[m][e], b = x[m][e + 8];
                     x[m][e] = a * cn - b * sn;
                     x[m][e + 8] = b * cn + a * sn;
                 }
             }
+            // split16's saturation: the largest magnitude decides (NaN passes through the maximum and fails the compare)
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                bad |= saturate(x[m][i], p.f16_lim);
-                most = fmaxf(most, fabsf(x[m][i]));
+            for (int i = 0; i < 16; i += 2)
+                top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(fabsf(x[m][i]), fabsf(x[m][i + 1])));
+            if (!(top <= p.f16_lim)) {
+                bad = true;
+                top = 65504.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) saturate(x[m][i], p.f16_lim);
             }
+            most = fmaxf(most, top);
         }
-        const float before = off ? p.k_scale[at] : 0.f;
         const float s = shared_scale(most, before, red), f = inverse_pow2(s);
         uint8_t *pg = p.k_pages + at * PAGE_BYTES;
 #pragma unroll
@@ -158,15 +183,15 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
             v[i] = u32x4{0u, 0u, 0u, 0u};
             if (i >= lo && i < hi) v[i] = *(const u32x4 *)(src + (size_t)(t0 + 8 * a + i - off) * p.row);
         }
+        const float before = off ? p.v_scale[at] : 0.f;
+        // bf16 magnitudes are ordered as integers are, NaN above all others
+        unsigned top = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float x = e & 1 ? bf_hi(v[i][e / 2]) : bf_lo(v[i][e / 2]);
-                bad |= saturate(x, p.f16_lim);
-                most = fmaxf(most, fabsf(x));
-            }
-        const float before = off ? p.v_scale[at] : 0.f;
+            for (int e = 0; e < 4; e++) top = max(top, max(v[i][e] << 16 & 0x7fffffffu, v[i][e] & 0x7fff0000u));
+        bad = !(__uint_as_float(top) <= p.f16_lim);
+        most = bad ? 65504.f : __uint_as_float(top);
         const float s = shared_scale(most, before, red), f = inverse_pow2(s);
         uint8_t *pg = p.v_pages + at * PAGE_BYTES;
         // old tokens: those of this thread's runs, so that no other thread writes them
@@ -180,7 +205,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     x[i] = e & 1 ? bf_hi(v[i][e / 2]) : bf_lo(v[i][e / 2]);
-                    saturate(x[i], p.f16_lim);
+                    if (bad) saturate(x[i], p.f16_lim);
                     x[i] *= f;
                 }
                 uint8_t *run = pg + (8 * c + e) * PAGE + 8 * a;
