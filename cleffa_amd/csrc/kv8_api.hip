@@ -142,8 +142,8 @@ bool clef_hip_kv8_attention(const clef_hip_kv8_args *a, void *stream, char *err,
     else if (p.l.bm == 128) hipLaunchKernelGGL(kv8::kv8_attn_tile_kernel, dim3(grid), dim3(kv8::kTileThreads), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL(kv8::kv8_attn_rows_kernel<2>, dim3(grid), dim3(kv8::kRowsThreads), 0, (hipStream_t)stream, p);
     if (!launch_ok("kv8_attn", err, errlen)) return false;
-    const long rows = (long)p.T * p.nh;
-    hipLaunchKernelGGL(kv8::kv8_join_kernel, dim3((unsigned)(rows < 4L * kCus ? rows : 4L * kCus)), dim3(kv8::kJoinThreads), 0, (hipStream_t)stream, p);
+    const long wgs = (long)p.T * p.nh;   // if every unit takes all of a workgroup's waves
+    hipLaunchKernelGGL(kv8::kv8_join_kernel, dim3((unsigned)(wgs < 8L * kCus ? wgs : 8L * kCus)), dim3(kv8::kJoinThreads), 0, (hipStream_t)stream, p);
     return launch_ok("kv8_join", err, errlen);
 }
 

@@ -737,50 +737,87 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
     }
 }
 
-// Joins the items of cut blocks. Workgroup unit (pass row, q head): wave w takes items w, w + 4, ..., a lane
-// four dims; the items are added in a fixed order, so results do not change from run to run.
-constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64;
+// Joins the items of cut blocks. A unit is a pass row's q head; one or four waves take its items in turn (by the
+// plan's most cut block: what a wave reads is in flight at once), a lane four dims, and the first of them adds
+// them up. The order is fixed, so results do not change from run to run.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kJoinBatch = 8;
 __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
-    __shared__ float os[kJoinWaves][HD], ls[kJoinWaves];
+    __shared__ float os[kJoinWaves][HD], ml[kJoinWaves][2];
     const int32_t *h = p.plan;
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || h[H_SPLIT] == 0) return;
-    const int units = h[H_TOKENS] * p.nh, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int t = u / p.nh, head = u - t * p.nh, kh = head / p.group;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int most = h[H_MOST], units = h[H_TOKENS] * p.nh;
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || most <= 1) return;
+    const int W = most <= kJoinBatch / 2 ? 1 : kJoinWaves, sub = wave & (W - 1), per = kJoinWaves / W;
+    const int rounds = (units + per * (int)gridDim.x - 1) / (per * (int)gridDim.x);
+    for (int round = 0; round < rounds; round++) {
+        const int u = (round * (int)gridDim.x + (int)blockIdx.x) * per + wave / W;
+        const int t = min(u / p.nh, p.T - 1), head = u % p.nh, kh = head / p.group;
         const int2 tok = ((const int2 *)(p.plan + p.l.tok))[t];
         const int fr = tok.y * p.group + head - kh * p.group, b = tok.x + fr / p.l.bm;
-        const int4 blk = ((const int4 *)(p.plan + p.l.blk))[b];
-        const int n = blk.y, row = fr - blk.z;
-        if (n <= 1) continue;   // the whole workgroup skips it
-        const Gate16 gate = load_gate(p, t, head, 16 * (tid & 15));
-        const int q0 = t - tok.y;
-        const float *ml = partial_ml(p);
-        float top = kNone;
-        for (int k = lane; k < n; k += 64) top = fmaxf(top, ml[2 * partial_row(p, blk.w + k, kh, row)]);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        int4 blk = {0, 0, 0, 0};
+        uint2 gate = {0, 0};
+        if (u < units) {
+            blk = ((const int4 *)(p.plan + p.l.blk))[b];
+            if (p.gate) gate = *(const uint2 *)(p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + 4 * lane);
+        }
+        const int n = __builtin_amdgcn_readfirstlane(blk.y), row = fr - blk.z;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
-#pragma unroll 4
-        for (int k = wave; k < n; k += kJoinWaves) {
-            const size_t pr = partial_row(p, blk.w + k, kh, row);
-            const float2 e = *(const float2 *)(ml + 2 * pr);
-            const f32x4 x = *(const f32x4 *)(p.partial + pr * HD + 4 * lane);
-            const float f = __builtin_amdgcn_exp2f(e.x - top);
-            l += e.y * f;
-            o += x * f;
-        }
-        *(f32x4 *)&os[wave][4 * lane] = o;
-        if (lane == 0) ls[wave] = l;
-        __syncthreads();
-        if (tid < 16) {
-            float x[16];
-            const float inv = 1.f / (ls[0] + ls[1] + ls[2] + ls[3]);
+        float m = kNone, l = 0.f;
+        if (n > 1)
+            for (int k0 = sub; k0 < n; k0 += W * kJoinBatch) {
+                float2 e[kJoinBatch];
+                f32x4 x[kJoinBatch];
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = (os[0][16 * tid + i] + os[1][16 * tid + i] + os[2][16 * tid + i] + os[3][16 * tid + i]) * inv;
-            finish16(p, t, head, 16 * tid, gate, x, p.ovf ? p.ovf + q0 : nullptr);
+                for (int j = 0; j < kJoinBatch; j++) {
+                    const size_t pr = partial_row(p, blk.w + min(k0 + W * j, n - 1), kh, row);
+                    e[j] = *(const float2 *)(partial_ml(p) + 2 * pr);
+                    x[j] = *(const f32x4 *)(p.partial + pr * HD + 4 * lane);
+                }
+                float top = m;
+#pragma unroll
+                for (int j = 0; j < kJoinBatch; j++) top = fmaxf(top, e[j].x);
+                const float f = __builtin_amdgcn_exp2f(m - top);
+                o *= f;
+                l *= f;
+                m = top;
+#pragma unroll
+                for (int j = 0; j < kJoinBatch; j++) {
+                    const float w = k0 + W * j < n ? __builtin_amdgcn_exp2f(e[j].x - top) : 0.f;
+                    l += e[j].y * w;
+                    o += x[j] * w;
+                }
+            }
+        if (W > 1) {
+            *(f32x4 *)&os[wave][4 * lane] = o;
+            if (lane == 0) {
+                ml[wave][0] = m;
+                ml[wave][1] = l;
+            }
+            __syncthreads();
+            if (sub == 0) {
+                float top = m;
+                for (int w = 1; w < W; w++) top = fmaxf(top, ml[wave + w][0]);
+                const float f = __builtin_amdgcn_exp2f(m - top);
+                o *= f;
+                l *= f;
+                for (int w = 1; w < W; w++) {
+                    const float g = __builtin_amdgcn_exp2f(ml[wave + w][0] - top);
+                    l += ml[wave + w][1] * g;
+                    o += *(const f32x4 *)&os[wave + w][4 * lane] * g;
+                }
+            }
         }
-        __syncthreads();
+        if (n > 1 && sub == 0) {
+            o *= 1.f / l;
+            if (p.gate) {
+                o[0] *= sigmoidf(bf_lo(gate.x));
+                o[1] *= sigmoidf(bf_hi(gate.x));
+                o[2] *= sigmoidf(bf_lo(gate.y));
+                o[3] *= sigmoidf(bf_hi(gate.y));
+            }
+            store_out4(p.out, ((size_t)t * p.nh + head) * HD + 4 * lane, o, p.out_type, p.f16_lim, p.ovf ? p.ovf + t - tok.y : nullptr);
+        }
+        if (W > 1) __syncthreads();
     }
 }
 

@@ -20,7 +20,7 @@ constexpr int kMaxGroup = 128;                 // q heads per kv head
 constexpr int32_t kPlanMagic = 0x4b563850;     // 'KV8P'
 
 // Plan header words. A failed plan leaves counts of 0, so the kernels that follow do nothing.
-enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_ITEMS, H_BLOCKS, H_SPLIT, H_WORDS = 16 };
+enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_ITEMS, H_BLOCKS, H_SPLIT, H_MOST, H_WORDS = 16 };
 
 // Where the parts of a plan buffer lie (in int32) and how many entries each can need:
 //  the first block of each sequence (of passes whose rows a second kernel writes);

@@ -107,13 +107,13 @@ __global__ __launch_bounds__(kRowThreads) void kv8_plan_rows_kernel(PlanParams p
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
     constexpr int kPlanThreads = THREADS, kPlanWaves = THREADS / 64;
-    __shared__ int cu[kPlanSums][kMaxSeq + 1], len[kMaxSeq], held[kMaxSeq], fresh[kMaxFresh], waves[kChunks][kPlanWaves], bad;
+    __shared__ int cu[kPlanSums][kMaxSeq + 1], len[kMaxSeq], held[kMaxSeq], fresh[kMaxFresh], waves[kChunks][kPlanWaves], bad, most;
     int *const cu_q = cu[0], *const cu_add = cu[1], *const cu_rel = cu[2], *const cu_app = cu[3], *const cu_blk = cu[4];
     const int tid = threadIdx.x, n = p.n_seq;
     const int n_free = p.state[0];
     int status = (unsigned)n_free > (unsigned)p.n_pages ? CLEF_HIP_KV8_BAD_STATE : 0;
     int base[kPlanSums] = {0, 0, 0, 0, 0};
-    if (tid == 0) bad = 0;   // the scans' barriers come before its first use
+    if (tid == 0) bad = most = 0;   // the scans' barriers come before their first use
     for (int r0 = 0; r0 < n; r0 += kPlanThreads) {
         const int r = r0 + tid;
         int v[kPlanSums] = {0, 0, 0, 0, 0}, total[kPlanSums];
@@ -282,6 +282,7 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
             if (b < n_blk) {
                 const int first = at + c[0], slot = at_slot + c[1];
                 ((int4 *)(p.work + p.l.blk))[b] = make_int4(first, items, row0, slot);
+                if (items > 1) atomicMax(&most, items);
                 if (in_lds) fresh[b] = first | slot << 16;   // at most 2^14, 2^11
                 else
                     for (int k = 0; k < items; k++) place(first + k, k, items, pages, r, row0, rows, slot);
@@ -304,6 +305,7 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
         n_items = at;
         n_slots = at_slot;
     }
+    __syncthreads();
     if (tid == 0) {
         p.cu_q[n] = good ? n_tok : 0;
         p.state_out[0] = good ? n_free + n_rel - n_add : n_free;
@@ -320,6 +322,7 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
         h[H_ITEMS] = n_items;
         h[H_BLOCKS] = good ? n_blk : 0;
         h[H_SPLIT] = n_slots;
+        h[H_MOST] = most;   // items of the most cut block
     }
 }
 
