@@ -70,24 +70,26 @@ def _stream_handle(stream):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
-class _on:
-    """The stream handle to launch on for a device: the given stream's, or the device's current stream, with that
-    device current for the time of the call (another one's stream would take its launches elsewhere)."""
+_ERR = ctypes.c_char * 512
 
-    def __init__(self, device, stream):
-        if device.type != "cuda":
-            raise RuntimeError(f"hip: the call needs tensors on a GPU, not on {device}")
-        self.device, self.stream, self.before = device, stream, None
 
-    def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
-            self.before = torch.cuda.current_device()
-            torch.cuda.set_device(self.device)
-        return _stream_handle(self.stream)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def _launch(fn, args, device, stream):
+    """fn(&args, stream, err, errlen) on the given stream, or the device's current one, with that device current for
+    the time of the call (another one's stream would take its launches elsewhere); raises what it refuses."""
+    if device.type != "cuda":
+        raise RuntimeError(f"hip: the call needs tensors on a GPU, not on {device}")
+    err = _ERR()
+    before = torch.cuda.current_device()
+    if before == device.index:
+        ok = fn(ctypes.byref(args), _stream_handle(stream), err, 512)
+    else:
+        torch.cuda.set_device(device)
+        try:
+            ok = fn(ctypes.byref(args), _stream_handle(stream), err, 512)
+        finally:
+            torch.cuda.set_device(before)
+    if not ok:
+        _lib.check(ok, err)
 
 
 _initialised = set()
@@ -236,6 +238,16 @@ def _check(t, name, shape, dtype, device):
         raise ValueError(f"{name} must be contiguous")
     if t.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned")
+
+
+def _arg(t, name, shape, dtype, device):
+    """_check, and the tensor's address."""
+    if t.__class__ is torch.Tensor and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        p = t.data_ptr()
+        if not p & 15:
+            return p
+    _check(t, name, shape, dtype, device)
+    return t.data_ptr()
 
 
 class TextAttention:
@@ -391,48 +403,41 @@ class TextAttention:
         their sequences. qkv [T][row] bf16, pass rows in the plan's order (plan.cu_q); pos3 [T][3], the plan's own
         or the caller's. Rows behind the last sequence are left out: their outputs stay as they were. stage:
         "prefill" (append and attention), "append", or "core" (attention alone). Returns out (None for "append")."""
-        dev, T = self.device, plan.T
+        dev, T, hd = self.device, plan.T, self.hd
         if plan.cache is not cache:
             raise ValueError("the plan belongs to another cache")
-        if (plan.nh, cache.nkv, cache.hd) != (self.nh, self.nkv, self.hd) or cache.device != dev:
+        if plan.nh != self.nh or cache.nkv != self.nkv or cache.hd != hd or cache.device != dev:
             raise ValueError("cache and plan do not fit the layer's heads or device")
         if stage not in ("prefill", "append", "core"):
             raise ValueError(f"stage {stage!r}")
-        cache.check_layer(layer)
-        _check(qkv, "qkv", (T, qkv.shape[1] if qkv.dim() == 2 else -1), torch.bfloat16, dev)
-        if qkv.shape[1] < self.row or qkv.shape[1] % 8:
-            raise ValueError(f"qkv row {qkv.shape[1]} must be >= {self.row} and a multiple of 8")
+        pools = cache.layer_args(layer)
+        row = qkv.shape[1] if qkv.dim() == 2 else -1
+        qkv = _arg(qkv, "qkv", (T, row), torch.bfloat16, dev)
+        if row < self.row or row % 8:
+            raise ValueError(f"qkv row {row} must be >= {self.row} and a multiple of 8")
         if (q_norm is None) != (k_norm is None):
             raise ValueError("q_norm and k_norm must both be given or both be None")
         if q_norm is not None:
-            _check(q_norm, "q_norm", (self.hd,), torch.float32, dev)
-            _check(k_norm, "k_norm", (self.hd,), torch.float32, dev)
-        if self.n_rot:
-            _check(pos3, "pos3", (T, 3), torch.int32, dev)
+            q_norm, k_norm = _arg(q_norm, "q_norm", (hd,), torch.float32, dev), _arg(k_norm, "k_norm", (hd,), torch.float32, dev)
+        pos3 = _arg(pos3, "pos3", (T, 3), torch.int32, dev) if self.n_rot else None
         if ovf is not None:
-            _check(ovf, "ovf", (T,), torch.int32, dev)
+            ovf = _arg(ovf, "ovf", (T,), torch.int32, dev)
         out_type, odt = _OUT_TYPES[out_dtype]
-        if stage != "append":
+        if stage == "append":
+            out = to = None
+        else:
             if out is None:
-                out = torch.empty((T, self.nh * self.hd), dtype=odt, device=dev)
-            _check(out, "out", (T, self.nh * self.hd), odt, dev)
-        a = _lib.Kv8Args()
-        a.nh, a.nkv, a.hd, a.n_rot, a.eps, a.scale = self.nh, self.nkv, self.hd, self.n_rot, self.eps, self.scale
-        a.T, a.row = T, qkv.shape[1]
-        a.n_seq, a.max_pages, a.n_pages, a.max_new = cache.max_seqs, cache.max_pages, cache.n_pages, plan.max_new
-        a.qkv, a.q_norm, a.k_norm, a.pos3, a.inv_freq = _ptr(qkv), _ptr(q_norm), _ptr(k_norm), _ptr(pos3), _ptr(self.inv_freq)
-        a.tables, a.plan = _ptr(cache.tables), _ptr(plan.work)
-        a.k_pages, a.v_pages = _ptr(cache.k[layer]), _ptr(cache.v[layer])
-        a.k_scale, a.v_scale = _ptr(cache.k_scale[layer]), _ptr(cache.v_scale[layer])
-        a.gate, a.out, a.out_type, a.f16_lim, a.ovf = int(gate), _ptr(out) if stage != "append" else None, out_type, f16_lim, _ptr(ovf)
-        a.workspace, a.workspace_bytes = _ptr(plan.workspace), plan.workspace.numel()
-        lib, err = _lib.load(), _err()
-        with _on(dev, stream) as s:
-            if stage != "core":
-                _lib.check(lib.clef_hip_kv8_append(ctypes.byref(a), s, err, len(err)), err)
-            if stage != "append":
-                _lib.check(lib.clef_hip_kv8_attention(ctypes.byref(a), s, err, len(err)), err)
-        return out if stage != "append" else None
+                out = torch.empty((T, self.nh * hd), dtype=odt, device=dev)
+            to = _arg(out, "out", (T, self.nh * hd), odt, dev)
+        a = _lib.Kv8Args(self.nh, self.nkv, hd, self.n_rot, self.eps, self.scale, T, row, cache.max_seqs, cache.max_pages, cache.n_pages,
+                         plan.max_new, qkv, q_norm, k_norm, pos3, self.inv_freq.data_ptr(), *pools, plan.work.data_ptr(), int(gate), to,
+                         out_type, f16_lim, ovf, plan.workspace.data_ptr(), plan.workspace_bytes)
+        lib = _lib.load()
+        if stage != "core":
+            _launch(lib.clef_hip_kv8_append, a, dev, stream)
+        if stage != "append":
+            _launch(lib.clef_hip_kv8_attention, a, dev, stream)
+        return out
 
 
 class VisionAttention:

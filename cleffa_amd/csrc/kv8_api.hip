@@ -49,17 +49,18 @@ bool sizes_ok(int n_seq, int T, int nh, int nkv, char *err, size_t errlen) {
     return true;
 }
 
-bool pool_ok(int max_pages, int n_pages, char *err, size_t errlen) {
+bool pool_ok(int max_pages, int n_pages, int nkv, char *err, size_t errlen) {
     if (max_pages <= 0 || max_pages > kv8::kMaxTablePages)
         return fail(err, errlen, "table rows of %d pages: 1 to %d are supported", max_pages, kv8::kMaxTablePages);
-    if (n_pages <= 0 || n_pages > INT32_MAX / CLEF_HIP_KV8_PAGE) return fail(err, errlen, "pool of %d pages", n_pages);
+    if (n_pages <= 0 || n_pages > INT32_MAX / CLEF_HIP_KV8_PAGE || (long)n_pages * nkv > INT32_MAX)
+        return fail(err, errlen, "pool of %d pages", n_pages);
     return true;
 }
 
 bool fill(const clef_hip_kv8_args *a, bool core, kv8::Params *q, char *err, size_t errlen) {
     if (!a) return fail(err, errlen, "null 8-bit cache arguments");
     if (a->hd != kv8::HD) return fail(err, errlen, "the 8-bit cache supports hd 256 only (got %d)", a->hd);
-    if (!sizes_ok(a->n_seq, a->T, a->nh, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, err, errlen)) return false;
+    if (!sizes_ok(a->n_seq, a->T, a->nh, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, a->nkv, err, errlen)) return false;
     if (a->n_rot != 0 && a->n_rot != 64) return fail(err, errlen, "unsupported n_rot %d", a->n_rot);
     const long need_row = 2L * a->nh * a->hd + 2L * a->nkv * a->hd;
     if (a->row < need_row || a->row % 8) return fail(err, errlen, "qkv row %d must be >= %ld and a multiple of 8", a->row, need_row);
@@ -67,6 +68,7 @@ bool fill(const clef_hip_kv8_args *a, bool core, kv8::Params *q, char *err, size
     if (!aligned16(a->q_norm) || !aligned16(a->k_norm)) return fail(err, errlen, "norm weights must be 16-byte aligned");
     if (!a->k_norm != !a->q_norm) return fail(err, errlen, "q_norm and k_norm must both be set or both be NULL");
     if (a->T && a->n_rot && (!a->pos3 || !a->inv_freq)) return fail(err, errlen, "rotary needs pos3 and inv_freq");
+    if (a->n_rot && !aligned16(a->inv_freq)) return fail(err, errlen, "inv_freq must be 16-byte aligned");
     if (!a->k_pages || !a->v_pages || !aligned16(a->k_pages) || !aligned16(a->v_pages)) return fail(err, errlen, "K / V pages must be 16-byte aligned device pointers");
     if (!a->k_scale || !a->v_scale) return fail(err, errlen, "missing page scales");
     if (!a->tables) return fail(err, errlen, "missing page tables");
@@ -106,7 +108,7 @@ bool clef_hip_kv8_sizes(int n_seq, int T, int nh, int nkv, int max_new, size_t *
 
 bool clef_hip_kv8_plan(const clef_hip_kv8_plan_args *a, void *stream, char *err, size_t errlen) {
     if (!a) return fail(err, errlen, "null plan arguments");
-    if (!sizes_ok(a->n_seq, a->T, a->nh, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, err, errlen)) return false;
+    if (!sizes_ok(a->n_seq, a->T, a->nh, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, a->nkv, err, errlen)) return false;
     if (!a->tables || !a->free_pages || !a->state || !a->state_out || !a->new_lens || !a->cu_q || (a->T && !a->slots))
         return fail(err, errlen, "missing page tables, free pages, state, lengths, cu_q or slots");
     if (!a->plan || !aligned16(a->plan)) return fail(err, errlen, "plan must be a 16-byte aligned device pointer");
@@ -150,7 +152,7 @@ bool clef_hip_kv8_attention(const clef_hip_kv8_args *a, void *stream, char *err,
 bool clef_hip_kv8_read(const clef_hip_kv8_read_args *a, void *stream, char *err, size_t errlen) {
     if (!a) return fail(err, errlen, "null read arguments");
     if (a->hd != kv8::HD) return fail(err, errlen, "the 8-bit cache supports hd 256 only (got %d)", a->hd);
-    if (!sizes_ok(a->n_seq, 0, a->nkv, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, err, errlen)) return false;
+    if (!sizes_ok(a->n_seq, 0, a->nkv, a->nkv, err, errlen) || !pool_ok(a->max_pages, a->n_pages, a->nkv, err, errlen)) return false;
     if (!a->k_pages || !a->v_pages || !aligned16(a->k_pages) || !aligned16(a->v_pages)) return fail(err, errlen, "K / V pages must be 16-byte aligned device pointers");
     if (!a->k_scale || !a->v_scale) return fail(err, errlen, "missing page scales");
     if (!a->tables || !a->state || !a->cu) return fail(err, errlen, "missing page tables, state or cu");

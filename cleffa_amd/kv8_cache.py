@@ -20,7 +20,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _check, _device, _err, _on, _ptr, init_device
+from .attention import _arg, _device, _err, _launch, init_device
 
 _STATUS = {1: "too few free pages", 2: "more new tokens than the pass has rows", 4: "a sequence would pass its table row",
            8: "lengths, counts or page numbers that cannot be"}
@@ -41,11 +41,12 @@ class Kv8Cache:
                              f"(at most {_lib.KV8_MAX_SEQ}) of {max_pages} pages (at most 65536)")
         self.n_layers, self.nkv, self.n_pages, self.max_seqs, self.max_pages, self.hd = n_layers, nkv, n_pages, max_seqs, max_pages, hd
         self.device = _device(device)
+        self._k_shape, self._v_shape = (n_pages, nkv, 4, _lib.KV8_PAGE, 64), (n_pages, nkv, hd, _lib.KV8_PAGE)
         self.k, self.v, self.k_scale, self.v_scale = ([None] * n_layers for _ in range(4))
         if allocate:
             for l in range(n_layers):
-                self.k[l] = torch.empty(self.page_shape("k"), dtype=torch.uint8, device=self.device)
-                self.v[l] = torch.empty(self.page_shape("v"), dtype=torch.uint8, device=self.device)
+                self.k[l] = torch.empty(self._k_shape, dtype=torch.uint8, device=self.device)
+                self.v[l] = torch.empty(self._v_shape, dtype=torch.uint8, device=self.device)
                 self.k_scale[l] = torch.ones((n_pages, nkv), dtype=torch.float32, device=self.device)
                 self.v_scale[l] = torch.ones((n_pages, nkv), dtype=torch.float32, device=self.device)
         self.tables = torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=self.device)
@@ -54,43 +55,31 @@ class Kv8Cache:
         self.state = torch.zeros(2 + 2 * max_seqs, dtype=torch.int32, device=self.device)
         self.state[0] = n_pages
 
-    def page_shape(self, which):
-        return (self.n_pages, self.nkv, 4, _lib.KV8_PAGE, 64) if which == "k" else (self.n_pages, self.nkv, self.hd, _lib.KV8_PAGE)
-
     def nbytes(self):
         """Bytes of all layers' pages and scales."""
         return self.n_layers * self.n_pages * self.nkv * 2 * (_lib.KV8_PAGE * self.hd + 4)
 
-    def check_layer(self, layer):
+    def layer_args(self, layer):
+        """Addresses of the tables and of a layer's pages and scales, their types and shapes checked."""
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
-        dev = self.device
-        _check(self.k[layer], "k pages", self.page_shape("k"), torch.uint8, dev)
-        _check(self.v[layer], "v pages", self.page_shape("v"), torch.uint8, dev)
-        _check(self.k_scale[layer], "k_scale", (self.n_pages, self.nkv), torch.float32, dev)
-        _check(self.v_scale[layer], "v_scale", (self.n_pages, self.nkv), torch.float32, dev)
-        _check(self.tables, "tables", (self.max_seqs, self.max_pages), torch.int32, dev)
+        dev, scales = self.device, (self.n_pages, self.nkv)
+        return (_arg(self.tables, "tables", (self.max_seqs, self.max_pages), torch.int32, dev),
+                _arg(self.k[layer], "k pages", self._k_shape, torch.uint8, dev), _arg(self.v[layer], "v pages", self._v_shape, torch.uint8, dev),
+                _arg(self.k_scale[layer], "k_scale", scales, torch.float32, dev), _arg(self.v_scale[layer], "v_scale", scales, torch.float32, dev))
 
     def read(self, layer, cu, k_plane, vt_plane, first_page=None, stream=None):
         """Brings pages back into 16-bit planes (k_plane [nkv][kvT][256] f16, vt_plane [nkv][256][kvT] bf16): of
         sequence r the tokens from page first_page[r] (0 if None) on, into plane rows cu[r] .. cu[r + 1]
         (device int32 [max_seqs + 1], multiples of 8). Other rows are left as they are."""
-        self.check_layer(layer)
-        dev, kvT = self.device, k_plane.shape[1] if k_plane.dim() == 3 else -1
-        _check(self.state, "state", (2 + 2 * self.max_seqs,), torch.int32, dev)
-        _check(cu, "cu", (self.max_seqs + 1,), torch.int32, dev)
-        if first_page is not None:
-            _check(first_page, "first_page", (self.max_seqs,), torch.int32, dev)
-        _check(k_plane, "k_plane", (self.nkv, kvT, self.hd), torch.float16, dev)
-        _check(vt_plane, "vt_plane", (self.nkv, self.hd, kvT), torch.bfloat16, dev)
-        a = _lib.Kv8ReadArgs()
-        a.nkv, a.hd, a.n_seq, a.max_pages, a.n_pages, a.kvT = self.nkv, self.hd, self.max_seqs, self.max_pages, self.n_pages, kvT
-        a.k_pages, a.v_pages, a.k_scale, a.v_scale = (_ptr(t[layer]) for t in (self.k, self.v, self.k_scale, self.v_scale))
-        a.tables, a.state, a.first_page, a.cu = _ptr(self.tables), _ptr(self.state), _ptr(first_page), _ptr(cu)
-        a.k_plane, a.vt_plane = _ptr(k_plane), _ptr(vt_plane)
-        err = _err()
-        with _on(dev, stream) as s:
-            _lib.check(_lib.load().clef_hip_kv8_read(ctypes.byref(a), s, err, len(err)), err)
+        dev, n, kvT = self.device, self.max_seqs, k_plane.shape[1] if k_plane.dim() == 3 else -1
+        tables, k, v, k_scale, v_scale = self.layer_args(layer)
+        a = _lib.Kv8ReadArgs(self.nkv, self.hd, n, self.max_pages, self.n_pages, kvT, k, v, k_scale, v_scale, tables,
+                             _arg(self.state, "state", (2 + 2 * n,), torch.int32, dev),
+                             None if first_page is None else _arg(first_page, "first_page", (n,), torch.int32, dev),
+                             _arg(cu, "cu", (n + 1,), torch.int32, dev), _arg(k_plane, "k_plane", (self.nkv, kvT, self.hd), torch.float16, dev),
+                             _arg(vt_plane, "vt_plane", (self.nkv, self.hd, kvT), torch.bfloat16, dev))
+        _launch(_lib.load().clef_hip_kv8_read, a, dev, stream)
         return k_plane, vt_plane
 
 
@@ -118,6 +107,7 @@ class Kv8Plan:
         self.pos3 = torch.zeros((max(self.T, 1), 3), dtype=torch.int32, device=dev)[:self.T]
         self.work = torch.zeros(ints.value, dtype=torch.int32, device=dev)
         self.workspace = torch.empty(ws.value, dtype=torch.uint8, device=dev)
+        self.workspace_bytes = ws.value
         self.state = None   # the state that the last update wrote
 
     def update(self, new_lens, pos_off=None, state_out=None, stream=None):
@@ -125,24 +115,15 @@ class Kv8Plan:
         gives its pages back). Without state_out the cache's state moves on in place; with it, the state after
         the pass goes there and the cache's own stays (tables and free pages change in place either way).
         pos_off int32 [max_seqs]: added to the token indexes for pos3. Does not wait: see status()."""
-        c, dev = self.cache, self.device
-        _check(new_lens, "new_lens", (c.max_seqs,), torch.int32, dev)
-        if pos_off is not None:
-            _check(pos_off, "pos_off", (c.max_seqs,), torch.int32, dev)
+        c, dev, n = self.cache, self.device, self.cache.max_seqs
         out = c.state if state_out is None else state_out
-        _check(c.state, "state", (2 + 2 * c.max_seqs,), torch.int32, dev)
-        _check(out, "state_out", (2 + 2 * c.max_seqs,), torch.int32, dev)
-        _check(c.tables, "tables", (c.max_seqs, c.max_pages), torch.int32, dev)
-        _check(c.free, "free", (c.n_pages,), torch.int32, dev)
-        a = _lib.Kv8PlanArgs()
-        a.n_seq, a.max_pages, a.n_pages, a.T, a.nh, a.nkv, a.max_new = c.max_seqs, c.max_pages, c.n_pages, self.T, self.nh, c.nkv, self.max_new
-        a.tables, a.free_pages, a.state, a.state_out = _ptr(c.tables), _ptr(c.free), _ptr(c.state), _ptr(out)
-        a.new_lens, a.pos_off = _ptr(new_lens), _ptr(pos_off)
-        a.cu_q, a.slots, a.pos3 = _ptr(self.cu_q), _ptr(self.slots), _ptr(self.pos3)
-        a.plan, a.plan_ints = _ptr(self.work), self.work.numel()
-        err = _err()
-        with _on(dev, stream) as s:
-            _lib.check(_lib.load().clef_hip_kv8_plan(ctypes.byref(a), s, err, len(err)), err)
+        a = _lib.Kv8PlanArgs(n, c.max_pages, c.n_pages, self.T, self.nh, c.nkv, self.max_new,
+                             _arg(c.tables, "tables", (n, c.max_pages), torch.int32, dev), _arg(c.free, "free", (c.n_pages,), torch.int32, dev),
+                             _arg(c.state, "state", (2 + 2 * n,), torch.int32, dev), _arg(out, "state_out", (2 + 2 * n,), torch.int32, dev),
+                             _arg(new_lens, "new_lens", (n,), torch.int32, dev),
+                             None if pos_off is None else _arg(pos_off, "pos_off", (n,), torch.int32, dev),
+                             self.cu_q.data_ptr(), self.slots.data_ptr(), self.pos3.data_ptr(), self.work.data_ptr(), self.work.numel())
+        _launch(_lib.load().clef_hip_kv8_plan, a, dev, stream)
         self.state = out
         return self
 

@@ -403,7 +403,7 @@ bool clef_hip_prefix_copy(const uint16_t *k_src, const uint16_t *vt_src, int src
  *   (exact but for codes that become subnormal).
  * For all layers:
  *   tables [n_seq][max_pages] int32: the pages of each sequence, in token order.
- *   free_pages [n_pages] int32: a stack of free pages, entry 0 at the bottom.
+ *   free_pages [n_pages] int32: a stack of free pages, entry 0 at the bottom, no page in it twice or in a table.
  *   state [2 + 2 n_seq] int32: {free pages on the stack, status of the last plan, then tokens and
  *   pages held of each sequence}. A caller may lower a sequence's tokens (a new request that shares only
  *   part of a cached text); its pages stay with it. Pages that several table rows share may be read, not
@@ -437,7 +437,7 @@ bool clef_hip_kv8_sizes(int n_seq, int T, int nh, int nkv, int max_new, size_t *
  * All or nothing: where status (state_out[1]) is not 0, state_out is the state otherwise unchanged, no
  * page has changed hands, cu_q is 0, slots -1, and append and attention with this plan do nothing. */
 typedef struct {
-    int n_seq, max_pages, n_pages;   /* max_pages at most 65,536 */
+    int n_seq, max_pages, n_pages;   /* max_pages at most 65,536; n_pages * 64 and n_pages * nkv below 2^31 */
     int T, nh, nkv, max_new;
     int32_t *tables, *free_pages;
     const int32_t *state;
@@ -459,7 +459,7 @@ typedef struct {
     const uint16_t *qkv;      /* [T][row] bf16, as in clef_hip_attn_args */
     const float *q_norm, *k_norm;   /* [hd] f32, or both NULL */
     const int32_t *pos3;      /* [T][3] */
-    const float *inv_freq;    /* [n_rot / 2] */
+    const float *inv_freq;    /* [n_rot / 2], 16-byte aligned */
     const int32_t *tables;
     uint8_t *k_pages, *v_pages;
     float *k_scale, *v_scale;

@@ -140,6 +140,48 @@ def test_sharp_rows_and_row_stride():
     _run(8, 4, [[90], [1], [7]], n_rot=0, norm=False, scale=4.0, extra=24, seed=8)
 
 
+@pytest.mark.parametrize("n_seq,new,group", [(70, 1, 2), (70, 3, 8), (40, 40, 4), (6, 1, 1)])
+def test_items_of_many_pages(n_seq, new, group):
+    """Sequences that share 300 pages (read only) and end in a page of their own: items run over hundreds of pages (with
+    many sequences) or are cut (with few), in each of the attention's forms."""
+    nkv, shared = 8, 300
+    nh = nkv * group
+    _say("shared pages", n_seq, new, group)
+    cache, model = Kv8Cache(1, nkv, shared + n_seq, n_seq, shared + 1), ref.Cache(shared + n_seq, n_seq, shared + 1)
+    g = torch.Generator(device="cuda").manual_seed(n_seq)
+    for codes, scale in ((cache.k[0], cache.k_scale[0]), (cache.v[0], cache.v_scale[0])):
+        codes.copy_(torch.randint(0, 120, codes.shape, generator=g, dtype=torch.uint8, device="cuda")
+                    | torch.randint(0, 2, codes.shape, generator=g, dtype=torch.uint8, device="cuda") << 7)
+        codes[shared:] = 0x7f
+        # scales of 2^-12 to 2^-4: units of the outputs change within a sequence
+        scale.copy_(2.0 ** torch.randint(-12, -3, scale.shape, generator=g, device="cuda"))
+    model.tables[:, :shared], model.len[:], model.held[:] = np.arange(shared), shared * PAGE, shared
+    model.n_free, model.free[:n_seq] = n_seq, shared + np.arange(n_seq)
+    cache.tables.copy_(_int(model.tables))
+    cache.free.copy_(_int(model.free))
+    cache.state.copy_(_int(model.state()))
+    T = n_seq * new
+    plan = Kv8Plan(cache, T, nh, new)
+    plan.update(_int([new] * n_seq))
+    status, cu, _, pos3 = model.plan([new] * n_seq, T)
+    qkv, qn, kn = _qkv(T, nh, nkv, 3)
+    out = TextAttention(nh, nkv).forward_kv8(qkv, qn, kn, plan.pos3, plan, cache, 0)
+    torch.cuda.synchronize()
+    assert status == plan.status() == 0
+    some = [0, n_seq // 2, n_seq - 1]
+    q, _, _, gate = ref.rows(_np(qkv.float()), nh, nkv, 64, _np(qn), _np(kn), pos3)
+    values = _cache_values(cache)
+    for r in some:
+        kk, vv = _sequence(cache, values, model, r, shared * PAGE + new)
+        tokens = [0, new - 1] if new > 3 else list(range(new))
+        for t in sorted(set(tokens)):
+            rows = slice(cu[r] + t, cu[r] + t + 1)
+            want, off = ref.attend(q[rows], gate[rows], kk, vv, shared * PAGE + t, HD ** -0.5, True)
+            off = off + HALF_STEP["bf16"] * (np.abs(want) + off)
+            d = np.abs(_np(out[rows].float()).reshape(want.shape) - want)
+            assert (d <= off).all(), (r, t, float((d / off).max()))
+
+
 @pytest.mark.parametrize("new", [[1], [40]])
 @pytest.mark.parametrize("where", ["first", "last"])
 def test_many_small_weights(new, where):
@@ -210,6 +252,32 @@ def test_codes_exact(magnitude):
         for page, (val, s, m) in held[name].items():
             assert np.array_equal(scale[page], s), (name, page)
             assert np.array_equal((got[page] * scale[page][:, None, None])[:, :m], val[:, :m]), (name, page)
+
+
+@pytest.mark.parametrize("last", [1, 30])
+def test_pages_of_very_different_magnitude(last):
+    """Pages whose keys and values differ by up to 2^75 in one sequence, in both orders: the outputs' units move with them."""
+    nh, nkv, mags = 4, 2, [2.0 ** 13, 2.0 ** -60, 1.0, 2.0 ** -20, 2.0 ** 12, 2.0 ** -62, 2.0 ** -3]
+    for order in (mags, mags[::-1]):
+        _say("magnitudes", order[0], last)
+        cache, model = Kv8Cache(1, nkv, 10, 1, 10), ref.Cache(10, 1, 10)
+        cache.k[0].fill_(0x7f)
+        cache.v[0].fill_(0xff)
+        att = TextAttention(nh, nkv, HD, 0)
+        for i, n in enumerate([PAGE] * len(order) + [last]):
+            before = model.len.copy()
+            plan = Kv8Plan(cache, n, nh, n)
+            plan.update(_int([n]))
+            _, cu, _, _ = model.plan([n], n)
+            qkv, _, _ = _qkv(n, nh, nkv, 60 + i)
+            if i < len(order):
+                x = qkv.float()
+                x[:, 2 * nh * HD:] *= order[i]
+                qkv = x.to(torch.bfloat16)
+            out = att.forward_kv8(qkv, None, None, None, plan, cache, 0)
+            torch.cuda.synchronize()
+            q, _, _, g = ref.rows(_np(qkv.float()), nh, nkv, 0, None, None, None)
+            _check_attention(out, before, [n], cu, q, g, cache, model, _cache_values(cache), HD ** -0.5, True)
 
 
 def test_other_pages_and_rows_untouched():
@@ -297,7 +365,7 @@ def test_plan_over_many_sequences():
 
 
 @pytest.mark.parametrize("new,T,status", [([5, 129, 1], 200, 4), ([64, 64, 64], 191, 2), ([64, 64, 64], 192, 1), ([300, 0, 0], 100, 2),
-                                          ([1, -1, 2 ** 31 - 1], 10, 2)])
+                                          ([1, -1, 2 ** 31 - 1], 10, 2), ([1400, 200, 0], 1500, 2)])
 def test_plan_refuses_whole(new, T, status):
     """A pass that does not fit changes nothing, and append and attention with its plan write nothing."""
     _say("refused plan", new, T)
@@ -360,6 +428,41 @@ def test_plan_again_from_the_same_state():
         assert all(torch.equal(a, b) for a, b in zip(got[0], again))
 
 
+def test_pass_without_rows():
+    """A pass of no rows ends sequences and gives their pages back; a layer's call with it does nothing."""
+    nh, nkv = 4, 2
+    cache, att = Kv8Cache(1, nkv, 8, 2, 4), TextAttention(nh, nkv)
+    plan = Kv8Plan(cache, 200, nh)
+    plan.update(_int([150, 50]))
+    none = Kv8Plan(cache, 0, nh)
+    none.update(_int([-1, 0]))
+    none.check()
+    assert cache.state.tolist() == [7, 0, 0, 0, 50, 1] and sorted(cache.free[:7].tolist()) == sorted(set(range(8)) - {int(cache.tables[1, 0])})
+    out = att.forward_kv8(torch.zeros(0, att.row, dtype=torch.bfloat16, device="cuda"), None, None, none.pos3, none, cache, 0)
+    assert out.shape == (0, nh * HD)
+    none.update(_int([1, 0]))
+    assert none.status() == 2
+
+
+def test_copies_of_a_cache_are_their_own():
+    """A deep copy of a cache and its plan works on its own memory, and leaves the first as it was."""
+    import copy
+    nh, nkv = 4, 2
+    cache, att = Kv8Cache(1, nkv, 8, 1, 4), TextAttention(nh, nkv)
+    plan = Kv8Plan(cache, 20, nh)
+    rows = _qkv(20, nh, nkv, 5)
+    plan.update(_int([20]))
+    want = att.forward_kv8(*rows, plan.pos3, plan, cache, 0)
+    other, other_plan = copy.deepcopy((cache, plan))
+    kept = [t.clone() for t in (cache.state, cache.tables, cache.k[0], cache.v[0])]
+    other_plan.update(_int([20]))
+    att.forward_kv8(*_qkv(20, nh, nkv, 6), other_plan.pos3, other_plan, other, 0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (cache.state, cache.tables, cache.k[0], cache.v[0])))
+    assert int(other.state[2]) == 40 and int(cache.state[2]) == 20
+    assert torch.equal(att.forward_kv8(*rows, plan.pos3, plan, cache, 0, stage="core"), want)
+
+
 # ---- reading back, and the 16-bit path
 
 @pytest.mark.parametrize("lens", [[1], [64], [130, 7, 0, 64], [5, 300]])
@@ -391,6 +494,33 @@ def test_read(lens):
             wk[:, cu[r]:cu[r] + m] = kk[:, skip[r]:skip[r] + m]
             wv[:, :, cu[r]:cu[r] + m] = vv[:, skip[r]:skip[r] + m].transpose(0, 2, 1)
         assert np.array_equal(_np(k), wk.astype(np.float16).astype(np.float64)) and np.array_equal(_np(v), wv)
+
+
+def test_read_of_many_pages():
+    """A read large enough for two pages a workgroup: odd lengths, rows that start anywhere at multiples of 8."""
+    nkv, lens = 16, [5000, 3, 0, 70, 2049, 64, 1500]
+    n, n_pages = len(lens), 150
+    cache, model = Kv8Cache(1, nkv, n_pages, n, 80), ref.Cache(n_pages, n, 80)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    cache.k[0].copy_(torch.randint(0, 127, cache.k[0].shape, generator=g, dtype=torch.uint8, device="cuda"))
+    cache.v[0].copy_(torch.randint(0, 127, cache.v[0].shape, generator=g, dtype=torch.uint8, device="cuda"))
+    cache.k_scale[0].copy_(2.0 ** torch.randint(-9, 9, (n_pages, nkv), generator=g, device="cuda"))
+    cache.v_scale[0].copy_(2.0 ** torch.randint(-9, 9, (n_pages, nkv), generator=g, device="cuda"))
+    plan = Kv8Plan(cache, sum(lens), nkv)
+    plan.update(_int(lens))
+    model.plan(lens, sum(lens))
+    cu = np.concatenate([[0], np.cumsum([-(-m // 8) * 8 + 8 for m in lens])])
+    kvT = int(cu[-1])
+    _say("read", lens, "into", kvT)
+    k, v = torch.full((nkv, kvT, HD), 9.0, dtype=torch.float16, device="cuda"), torch.full((nkv, HD, kvT), 9.0, dtype=torch.bfloat16, device="cuda")
+    cache.read(0, _int(cu), k, v)
+    torch.cuda.synchronize()
+    values = _cache_values(cache)
+    k, v = _np(k), _np(v)
+    for r, m in enumerate(lens):
+        kk, vv = _sequence(cache, values, model, r, m)
+        assert np.array_equal(k[:, cu[r]:cu[r] + m], np.clip(kk, -65504, 65504)) and np.array_equal(v[:, :, cu[r]:cu[r] + m].transpose(0, 2, 1), vv)
+        assert (k[:, cu[r] + m:cu[r + 1]] == 9).all() and (v[:, :, cu[r] + m:cu[r + 1]] == 9).all()
 
 
 def test_against_the_16_bit_path():

@@ -97,7 +97,7 @@ def _args(**over):
 @pytest.mark.parametrize("over,msg", [(dict(hd=128), "hd 256"), (dict(nh=25), "head counts"), (dict(n_rot=32), "n_rot"), (dict(row=14000), "qkv row"),
                                       (dict(row=14337), "qkv row"), (dict(qkv=None), "qkv"), (dict(q_norm=None), "both"), (dict(pos3=None), "rotary"),
                                       (dict(k_pages=ctypes.c_void_p((1 << 20) + 8)), "pages"), (dict(v_scale=None), "scales"), (dict(tables=None), "tables"),
-                                      (dict(plan=None), "plan"), (dict(eps=float("nan")), "eps"), (dict(n_pages=-1), "pool")])
+                                      (dict(plan=None), "plan"), (dict(inv_freq=ctypes.c_void_p((1 << 20) + 4)), "inv_freq"), (dict(n_pages=1 << 30), "pool"), (dict(eps=float("nan")), "eps"), (dict(n_pages=-1), "pool")])
 def test_append_and_attention_refused(over, msg):
     for fn in (_lib.load().clef_hip_kv8_append, _lib.load().clef_hip_kv8_attention):
         err = _err()
@@ -140,7 +140,7 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="T -1"):
         Kv8Plan(cache, -1, 8)
     with pytest.raises(ValueError, match="layer 2"):
-        cache.check_layer(2)
+        cache.layer_args(2)
     with pytest.raises(ValueError, match="hd 256"):
         Kv8Cache(1, 4, 16, 3, 8, hd=128, device="cpu")
     with pytest.raises(ValueError, match="cache sizes"):
@@ -156,7 +156,7 @@ def test_python_refusals():
         cache.read(0, torch.zeros(4, dtype=torch.int32), torch.zeros(4, 64, 256, dtype=torch.float16), torch.zeros(4, 256, 64, dtype=torch.bfloat16))
     cache.k[0] = cache.k[0][:8]
     with pytest.raises(ValueError, match="k pages"):
-        cache.check_layer(0)
+        cache.layer_args(0)
 
 
 def test_reference_codes():
