@@ -161,6 +161,78 @@ __device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f1
         }
 }
 
+// A sixteenth of a q row, for a workgroup whose waves share the making of their rows: lane j takes dims 64c + 4j + e,
+// e < 4, and the finished dims go to the row in LDS. The same arithmetic as QRow's.
+struct QPart {
+    uint2 w[4];
+    float4 norm[4], freq;
+    int pos[3];
+};
+__device__ __forceinline__ void load_part(const Params &p, int t, int head, int j, QPart &r) {
+    const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 4 * j;
+#pragma unroll
+    for (int c = 0; c < 4; c++) r.w[c] = *(const uint2 *)(src + 64 * c);
+    if (p.q_norm)
+#pragma unroll
+        for (int c = 0; c < 4; c++) r.norm[c] = *(const float4 *)(p.q_norm + 64 * c + 4 * j);
+    if (p.n_rot) {   // pairs 4 (j & 7) + e
+        r.freq = *(const float4 *)(p.inv_freq + 4 * (j & 7));
+#pragma unroll
+        for (int i = 0; i < 3; i++) r.pos[i] = p.pos3[3 * (size_t)t + i];
+    }
+}
+__device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j, _Float16 *row, int32_t *flag) {
+    float x[4][4];
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        x[c][0] = bf_lo(r.w[c].x);
+        x[c][1] = bf_hi(r.w[c].x);
+        x[c][2] = bf_lo(r.w[c].y);
+        x[c][3] = bf_hi(r.w[c].y);
+#pragma unroll
+        for (int i = 0; i < 4; i++) ss += x[c][i] * x[c][i];
+    }
+    if (p.q_norm) {
+        const float inv = rsqrtf(row16_sum(ss) / (float)HD + p.eps);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float4 w = r.norm[c];
+            x[c][0] *= inv * w.x;
+            x[c][1] *= inv * w.y;
+            x[c][2] *= inv * w.z;
+            x[c][3] *= inv * w.w;
+        }
+    }
+    if (p.n_rot) {
+        const float freq[4] = {r.freq.x, r.freq.y, r.freq.z, r.freq.w};
+        const int ax = j & 7;   // pair 4 ax + e: axis (4 ax + e) % 3 = (ax + e) % 3
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int axis = (ax + e) % 3;
+            float sn, cn;
+            rope_turns((float)(axis == 0 ? r.pos[0] : axis == 1 ? r.pos[1] : r.pos[2]) * freq[e], &sn, &cn);
+            const float o = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x[0][e]), 0x128, 0xf, 0xf, false));   // lane j ^ 8's
+            x[0][e] = j < 8 ? x[0][e] * cn - o * sn : x[0][e] * cn + o * sn;
+        }
+    }
+    float most = 0.f;   // split16's saturation, as in make_q
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+            most = __builtin_elementwise_maximum(most, __builtin_elementwise_maximum(fabsf(x[c][i]), fabsf(x[c][i + 1])));
+    if (!(most <= p.f16_lim)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) saturate(x[c][i], p.f16_lim);
+        if (flag) __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) *(uint2 *)(row + 64 * c + 4 * j) = make_uint2(pack_f16(x[c][0], x[c][1]), pack_f16(x[c][2], x[c][3]));
+}
+
 // Sixteen finished outputs (dims d0 ..) of a row: times the sigmoid of their gates (loaded ahead), converted and stored.
 struct Gate16 {
     u32x4 a, b;
@@ -199,6 +271,9 @@ __device__ __forceinline__ float *partial_ml(const Params &p) {
     return p.partial + (size_t)p.l.max_slots * p.nkv * p.l.bm * HD;
 }
 
+// A barrier whose LDS accesses before it are done; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Few rows (decoding): a workgroup takes an item's 16 MT rows over its pages, wave w the pages w, w + 4, ...
 // Bound by memory: each page is read once, straight into registers, 4 KB pieces (four 1 KB loads) in a ring of
 // four that K and V share: as a piece is used up, the one four later is loaded into its registers, so 16 KB a
@@ -209,55 +284,69 @@ constexpr int kRowsThreads = 256, kRowsWaves = 4;
 template <int MT>
 __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_kernel(Params p) {
     constexpr int BM = 16 * MT, OS = HD + 4;   // LDS row stride of the outputs
-    __shared__ float os[kRowsWaves][16][OS], ml[kRowsWaves][BM][2];
+    __shared__ __attribute__((aligned(16))) float os[kRowsWaves][16][OS];   // holds the q rows before
+    __shared__ float ml[kRowsWaves][BM][2];
     const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
     const int4 e0 = it[0], e1 = it[1];
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_ITEMS]) return;
+    const int n_items = h[H_ITEMS];
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= n_items) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q16 = lane & 15, g = lane >> 4;
     const int lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;   // the lane's piece of tile 0
     const int seq = e0.x, q0 = e0.y, L = e0.z, n_keys = e0.w, row0 = e1.x, rows = e1.y & 0xff, slot = (e1.y >> 8) - 1;
     const int pg0 = e1.z, pg1 = e1.w;
     const int32_t *table = p.tables + (size_t)seq * p.max_pages;
-    QRow raw[MT];
-    int last[MT];   // the last key the lane's row sees
+    // the wave's pages i = 0, 1, ... are pg0 + wave + 4 i; lane j holds number and scales of page (i & ~63) + j (a page
+    // behind the item's last: the last's)
+    const int n_mine = (pg1 - pg0 - wave + kRowsWaves - 1) / kRowsWaves;   // 0 or less: none
+    auto number = [&](int i0) { return (unsigned)table[min(pg0 + wave + kRowsWaves * (i0 + lane), pg1 - 1)]; };
+    unsigned ids = number(0);
+    // Each wave makes a quarter of the rows. Loads go out in the order of their uses, and none of them conditionally:
+    // a wave without a page loads the item's last.
+    const int part = lane & 15;
+    QPart raw[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        const int fr = row0 + min(16 * m + q16, rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
-        load_q(p, q0 + t, head, g, raw[m]);
-        last[m] = L + t;
+        const int fr = row0 + min(16 * m + 4 * wave + (lane >> 4), rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
+        load_part(p, q0 + t, head, part, raw[m]);
     }
-    // the wave's pages i = 0, 1, ... are pg0 + wave + 4 i; lane j holds number and scales of page (i & ~63) + j
-    const int n_mine = (pg1 - pg0 - wave + kRowsWaves - 1) / kRowsWaves;   // 0 or less: none
-    unsigned ids = 0;
-    float kss = 0.f, vss = 0.f;
-    auto look_up = [&](int i0) {
-        const int pg = pg0 + wave + kRowsWaves * (i0 + lane);
-        ids = pg < pg1 ? (unsigned)table[pg] : 0u;
+    float kss, vss;
+    auto scales = [&] {
         if (ids >= (unsigned)p.n_pages) ids = 0;
         ids = ids * p.nkv + kh;
         kss = p.k_scale[ids];
         vss = p.v_scale[ids];
-        asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here: the loop's waits are for its own loads
     };
+    auto landed = [&] { asm volatile("" : "+v"(kss), "+v"(vss)); };   // waited for here: the loop's waits are for its own loads
     u32x4 ring[4][4];
     auto load = [&](const uint8_t *pages, unsigned at, int c) {
         const uint8_t *src = pages + (size_t)at * PAGE_BYTES + 4096 * c + lofs;
 #pragma unroll
         for (int t = 0; t < 4; t++) ring[c][t] = *(const u32x4 *)(src + 256 * t);
     };
-    unsigned at = 0;
-    if (n_mine > 0) {
-        look_up(0);
-        at = __builtin_amdgcn_readlane(ids, 0);
+    scales();
+    unsigned at = __builtin_amdgcn_readlane(ids, 0);
 #pragma unroll
-        for (int c = 0; c < 4; c++) load(p.k_pages, at, c);
+    for (int c = 0; c < 4; c++) load(p.k_pages, at, c);
+    constexpr int QS = HD + 8;   // LDS row stride of the q rows
+    _Float16 *const qs = (_Float16 *)&os[0][0][0];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int r = 16 * m + 4 * wave + (lane >> 4);
+        make_part(p, raw[m], part, qs + r * QS, p.ovf ? p.ovf + q0 : nullptr);
     }
+    landed();
+    lds_barrier();
     f16x8 q[MT][8];
+    int last[MT];   // the last key the lane's row sees
 #pragma unroll
-    for (int m = 0; m < MT; m++) make_q(p, raw[m], g, q[m], p.ovf ? p.ovf + q0 : nullptr);
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) q[m][c] = *(const f16x8 *)(qs + (16 * m + q16) * QS + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+        last[m] = L + (row0 + min(16 * m + q16, rows - 1)) / p.group;
+    }
     f32x4 o[MT][16];
     float mx[MT], sum[MT];
     int unit = 0;   // o is in units of 2^(unit - 5)
@@ -333,7 +422,11 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
         unit = now_unit;
         unsigned next = 0;
         if constexpr (MORE) {
-            if (((i + 1) & 63) == 0) look_up(i + 1);
+            if (((i + 1) & 63) == 0) {
+                ids = number(i + 1);
+                scales();
+                landed();
+            }
             next = __builtin_amdgcn_readlane(ids, (i + 1) & 63);
         } else if ((pg + 1) * PAGE > n_keys) {   // V codes behind the last key may be NaN, whose product with 0 is NaN
 #pragma unroll
@@ -463,16 +556,14 @@ template <int N>
 __device__ __forceinline__ void lds_wait2(u32x4 (&r)[4], u32x4 &a, u32x4 &b) {
     asm volatile("s_waitcnt lgkmcnt(%6)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(a), "+v"(b) : "i"(N));
 }
-// A barrier whose LDS accesses before it are done; loads from memory stay in flight.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p) {
     __shared__ __attribute__((aligned(16))) TileLds sm;
     const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
     const int4 e0 = it[0], e1 = it[1];
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= h[H_ITEMS]) return;
+    const int n_items = h[H_ITEMS];
+    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= n_items) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave & 3, half = wave >> 2;   // rows 32 rg .. 32 rg + 31, half of the tokens or dims
     const int q16 = lane & 15, g = lane >> 4;

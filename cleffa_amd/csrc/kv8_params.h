@@ -84,7 +84,8 @@ struct Params {
 
 // A plan is run only with the sizes it was made for.
 __device__ __forceinline__ bool plan_fits(const int32_t *h, int n_seq, int T, int group, int bm) {
-    return h[H_MAGIC] == kPlanMagic && h[H_SEQ] == n_seq && h[H_ROWS] == T && h[H_GROUP] == group && h[H_BM] == bm;
+    // one wait for all five words (&& would load each after the one before)
+    return ((h[H_MAGIC] ^ kPlanMagic) | (h[H_SEQ] ^ n_seq) | (h[H_ROWS] ^ T) | (h[H_GROUP] ^ group) | (h[H_BM] ^ bm)) == 0;
 }
 
 }  // namespace kv8
