@@ -170,8 +170,6 @@ struct QPart {
 };
 __device__ __forceinline__ void load_part(const Params &p, int t, int head, int j, QPart &r) {
     const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 4 * j;
-#pragma unroll
-    for (int c = 0; c < 4; c++) r.w[c] = *(const uint2 *)(src + 64 * c);
     if (p.q_norm)
 #pragma unroll
         for (int c = 0; c < 4; c++) r.norm[c] = *(const float4 *)(p.q_norm + 64 * c + 4 * j);
@@ -180,6 +178,8 @@ __device__ __forceinline__ void load_part(const Params &p, int t, int head, int 
 #pragma unroll
         for (int i = 0; i < 3; i++) r.pos[i] = p.pos3[3 * (size_t)t + i];
     }
+#pragma unroll
+    for (int c = 0; c < 4; c++) r.w[c] = *(const uint2 *)(src + 64 * c);
 }
 __device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j, _Float16 *row, int32_t *flag) {
     float x[4][4];
@@ -289,9 +289,8 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
-    const int4 e0 = it[0], e1 = it[1];
-    const int n_items = h[H_ITEMS];
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= n_items) return;
+    int4 e0 = it[0], e1 = it[1];
+    if (!plan_has(h, H_ITEMS, item, p.n_seq, p.T, p.group, p.l.bm, e0, e1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q16 = lane & 15, g = lane >> 4;
     const int lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;   // the lane's piece of tile 0
@@ -312,6 +311,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
         const int fr = row0 + min(16 * m + 4 * wave + (lane >> 4), rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
         load_part(p, q0 + t, head, part, raw[m]);
     }
+    __builtin_amdgcn_sched_barrier(0);
     float kss, vss;
     auto scales = [&] {
         if (ids >= (unsigned)p.n_pages) ids = 0;
@@ -561,9 +561,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
     const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
-    const int4 e0 = it[0], e1 = it[1];
-    const int n_items = h[H_ITEMS];
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= n_items) return;
+    int4 e0 = it[0], e1 = it[1];
+    if (!plan_has(h, H_ITEMS, item, p.n_seq, p.T, p.group, p.l.bm, e0, e1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave & 3, half = wave >> 2;   // rows 32 rg .. 32 rg + 31, half of the tokens or dims
     const int q16 = lane & 15, g = lane >> 4;

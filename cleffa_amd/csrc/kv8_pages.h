@@ -72,9 +72,9 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
     __shared__ float red[4];
     const int kh = blockIdx.x % p.nkv, item = blockIdx.x / p.nkv, tid = threadIdx.x;
     const int32_t *h = p.plan;
-    const int4 it = ((const int4 *)(p.plan + p.l.app))[item];   // with the header, not behind it: the grid ends with the list's room
-    const int n_items = h[H_APPEND];
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || item >= n_items) return;
+    int4 it = ((const int4 *)(p.plan + p.l.app))[item];   // the grid ends with the list's room
+    int4 none = {0, 0, 0, 0};
+    if (!plan_has(h, H_APPEND, item, p.n_seq, p.T, p.group, p.l.bm, it, none)) return;
     const int page = it.x, t0 = it.y, off = it.z & 0xff, n = it.z >> 8, flag = it.w;
     if ((unsigned)page >= (unsigned)p.n_pages) return;
     const size_t at = (size_t)page * p.nkv + kh;
