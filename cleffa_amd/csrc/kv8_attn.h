@@ -54,134 +54,33 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned a, unsigned b) {
 // The first n bytes of a word (n below 0 or above 4: none, all).
 __device__ __forceinline__ unsigned keep_bytes(int n) { return n <= 0 ? 0u : ~0u >> 8 * (4 - min(n, 4)); }
 
-// One q row as the B operand of its 16-row tile: lane (row, g) takes dims 64c + 16g + e, e < 16, as operands
-// 2c (e < 8) and 2c + 1. Two steps, so that other loads can go out between them: the row as it is, then norm and
-// rotary in f32 and f16 with split16's saturation (flagged).
-struct QRow {
-    u32x4 w[8];
-    float4 norm[16], freq[2];
-    int pos[3];
+// The q rows of an item: RMSNorm and rotary in f32, then f16 with split16's saturation (flagged), into LDS rows of QS.
+// The workgroup's waves share them, 16 lanes a row, lane j of them dims 64c + 4j + e, e < 4: few loads, of whole lines
+// (a wave that made the operands of its own 16 rows spent 8,000 clocks on loading them, 29 loads of 16 bytes a lane).
+// Loads and arithmetic are apart, so that other loads can go out between them.
+constexpr int QS = HD + 8;
+struct QNorm {   // of all rows
+    float4 norm[4], freq;
 };
-__device__ __forceinline__ void load_q(const Params &p, int t, int head, int g, QRow &r) {
-    const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 16 * g;
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        r.w[2 * c] = *(const u32x4 *)(src + 64 * c);
-        r.w[2 * c + 1] = *(const u32x4 *)(src + 64 * c + 8);
-    }
-    if (p.q_norm)
-#pragma unroll
-        for (int i = 0; i < 16; i++) r.norm[i] = *(const float4 *)(p.q_norm + 64 * (i >> 2) + 16 * g + 4 * (i & 3));
-    if (p.n_rot) {   // pairs 16 (g & 1) + 8 (g >> 1) + e
-        const int i0 = 16 * (g & 1) + 8 * (g >> 1);
-        r.freq[0] = *(const float4 *)(p.inv_freq + i0);
-        r.freq[1] = *(const float4 *)(p.inv_freq + i0 + 4);
-#pragma unroll
-        for (int i = 0; i < 3; i++) r.pos[i] = p.pos3[3 * (size_t)t + i];
-    }
-}
-__device__ __forceinline__ float other_half(float x) {   // lane ^ 32's value
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
-__device__ __forceinline__ void make_q(const Params &p, const QRow &r, int g, f16x8 (&q)[8], int32_t *flag) {
-    float x[4][16];
-    float ss = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[c][2 * i] = bf_lo(r.w[2 * c][i]);
-            x[c][2 * i + 1] = bf_hi(r.w[2 * c][i]);
-            x[c][8 + 2 * i] = bf_lo(r.w[2 * c + 1][i]);
-            x[c][9 + 2 * i] = bf_hi(r.w[2 * c + 1][i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) ss += x[c][i] * x[c][i];
-    }
-    if (p.q_norm) {
-        const float inv = rsqrtf(text::xrow_sum(ss) / (float)HD + p.eps);
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 w = r.norm[4 * c + i / 4];
-                x[c][i] *= inv * w.x;
-                x[c][i + 1] *= inv * w.y;
-                x[c][i + 2] *= inv * w.z;
-                x[c][i + 3] *= inv * w.w;
-            }
-    }
-    if (p.n_rot) {
-        // dims 16g + e of the first 64: pair (16g + e) % 32, whose other half lane ^ 32 holds; the two lanes share
-        // their 16 pairs' sin and cos, eight each
-        float sn[16], cn[16];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int axis = (16 * (g & 1) + 8 * (g >> 1) + e) % 3;
-            const float4 f4 = r.freq[e >> 2];
-            const float f = (e & 3) == 0 ? f4.x : (e & 3) == 1 ? f4.y : (e & 3) == 2 ? f4.z : f4.w;
-            rope_turns((float)(axis == 0 ? r.pos[0] : axis == 1 ? r.pos[1] : r.pos[2]) * f, &sn[e], &cn[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float s1 = other_half(sn[e]), c1 = other_half(cn[e]), s0 = sn[e], c0 = cn[e];
-            sn[e] = g < 2 ? s0 : s1;
-            sn[e + 8] = g < 2 ? s1 : s0;
-            cn[e] = g < 2 ? c0 : c1;
-            cn[e + 8] = g < 2 ? c1 : c0;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float o = other_half(x[0][e]);
-            x[0][e] = g < 2 ? x[0][e] * cn[e] - o * sn[e] : x[0][e] * cn[e] + o * sn[e];
-        }
-    }
-    // split16's saturation: the largest magnitude decides (NaN passes through the maximum and fails the compare)
-    float most = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2)
-            most = __builtin_elementwise_maximum(most, __builtin_elementwise_maximum(fabsf(x[c][i]), fabsf(x[c][i + 1])));
-    if (!(most <= p.f16_lim)) {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) saturate(x[c][i], p.f16_lim);
-        if (flag) __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const f16x2 h = __builtin_bit_cast(f16x2, pack_f16(x[c][i], x[c][i + 1]));
-            q[2 * c + (i >> 3)][i & 7] = h[0];
-            q[2 * c + (i >> 3)][(i & 7) + 1] = h[1];
-        }
-}
-
-// A sixteenth of a q row, for a workgroup whose waves share the making of their rows: lane j takes dims 64c + 4j + e,
-// e < 4, and the finished dims go to the row in LDS. The same arithmetic as QRow's.
 struct QPart {
     uint2 w[4];
-    float4 norm[4], freq;
     int pos[3];
 };
-__device__ __forceinline__ void load_part(const Params &p, int t, int head, int j, QPart &r) {
-    const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 4 * j;
+__device__ __forceinline__ void load_norm(const Params &p, int j, QNorm &n) {
     if (p.q_norm)
 #pragma unroll
-        for (int c = 0; c < 4; c++) r.norm[c] = *(const float4 *)(p.q_norm + 64 * c + 4 * j);
-    if (p.n_rot) {   // pairs 4 (j & 7) + e
-        r.freq = *(const float4 *)(p.inv_freq + 4 * (j & 7));
+        for (int c = 0; c < 4; c++) n.norm[c] = *(const float4 *)(p.q_norm + 64 * c + 4 * j);
+    if (p.n_rot) n.freq = *(const float4 *)(p.inv_freq + 4 * (j & 7));   // pairs 4 (j & 7) + e
+}
+__device__ __forceinline__ void load_part(const Params &p, int t, int head, int j, QPart &r) {
+    const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + 4 * j;
+    if (p.n_rot)
 #pragma unroll
         for (int i = 0; i < 3; i++) r.pos[i] = p.pos3[3 * (size_t)t + i];
-    }
 #pragma unroll
     for (int c = 0; c < 4; c++) r.w[c] = *(const uint2 *)(src + 64 * c);
 }
-__device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j, _Float16 *row, int32_t *flag) {
+__device__ __forceinline__ void make_part(const Params &p, const QNorm &n, const QPart &r, int j, _Float16 *row, int32_t *flag) {
     float x[4][4];
     float ss = 0.f;
 #pragma unroll
@@ -197,7 +96,7 @@ __device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j
         const float inv = rsqrtf(row16_sum(ss) / (float)HD + p.eps);
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            const float4 w = r.norm[c];
+            const float4 w = n.norm[c];
             x[c][0] *= inv * w.x;
             x[c][1] *= inv * w.y;
             x[c][2] *= inv * w.z;
@@ -205,7 +104,7 @@ __device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j
         }
     }
     if (p.n_rot) {
-        const float freq[4] = {r.freq.x, r.freq.y, r.freq.z, r.freq.w};
+        const float freq[4] = {n.freq.x, n.freq.y, n.freq.z, n.freq.w};
         const int ax = j & 7;   // pair 4 ax + e: axis (4 ax + e) % 3 = (ax + e) % 3
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -216,7 +115,8 @@ __device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j
             x[0][e] = j < 8 ? x[0][e] * cn - o * sn : x[0][e] * cn + o * sn;
         }
     }
-    float most = 0.f;   // split16's saturation, as in make_q
+    // split16's saturation: the largest magnitude decides (NaN passes through the maximum and fails the compare)
+    float most = 0.f;
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -233,33 +133,16 @@ __device__ __forceinline__ void make_part(const Params &p, const QPart &r, int j
     for (int c = 0; c < 4; c++) *(uint2 *)(row + 64 * c + 4 * j) = make_uint2(pack_f16(x[c][0], x[c][1]), pack_f16(x[c][2], x[c][3]));
 }
 
-// Sixteen finished outputs (dims d0 ..) of a row: times the sigmoid of their gates (loaded ahead), converted and stored.
-struct Gate16 {
-    u32x4 a, b;
-};
-__device__ __forceinline__ Gate16 load_gate(const Params &p, int t, int head, int d0) {
-    Gate16 w = {};
-    if (p.gate) {
-        const uint16_t *src = p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + d0;
-        w.a = *(const u32x4 *)src;
-        w.b = *(const u32x4 *)(src + 8);
-    }
-    return w;
+// Four finished outputs (dims d0 ..) of a row: times the sigmoid of their gates (loaded ahead), converted and stored.
+__device__ __forceinline__ uint2 load_gate(const Params &p, int t, int head, int d0) {
+    return p.gate ? *(const uint2 *)(p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + d0) : make_uint2(0, 0);
 }
-__device__ __forceinline__ void finish16(const Params &p, int t, int head, int d0, const Gate16 &w, float (&o)[16], int32_t *flag) {
-    if (p.gate) {
-        const u32x4 a = w.a, b = w.b;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            o[2 * i] *= sigmoidf(bf_lo(a[i]));
-            o[2 * i + 1] *= sigmoidf(bf_hi(a[i]));
-            o[8 + 2 * i] *= sigmoidf(bf_lo(b[i]));
-            o[9 + 2 * i] *= sigmoidf(bf_hi(b[i]));
-        }
-    }
-    const size_t idx = ((size_t)t * p.nh + head) * HD + d0;
-    store_out8(p.out, idx, o, p.out_type, p.f16_lim, flag);
-    store_out8(p.out, idx + 8, o + 8, p.out_type, p.f16_lim, flag);
+__device__ __forceinline__ f32x4 gated(f32x4 o, uint2 gate) {
+    return f32x4{o[0] * sigmoidf(bf_lo(gate.x)), o[1] * sigmoidf(bf_hi(gate.x)), o[2] * sigmoidf(bf_lo(gate.y)), o[3] * sigmoidf(bf_hi(gate.y))};
+}
+__device__ __forceinline__ void finish4(const Params &p, int t, int head, int d0, uint2 gate, f32x4 o, int32_t *flag) {
+    if (p.gate) o = gated(o, gate);
+    store_out4(p.out, ((size_t)t * p.nh + head) * HD + d0, o, p.out_type, p.f16_lim, flag);
 }
 
 // Partial results of a cut block: [split slot][kv head][row][256] unnormalised outputs, then
@@ -305,7 +188,9 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     // Each wave makes a quarter of the rows. Loads go out in the order of their uses, and none of them conditionally:
     // a wave without a page loads the item's last.
     const int part = lane & 15;
+    QNorm norm;
     QPart raw[MT];
+    load_norm(p, part, norm);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int fr = row0 + min(16 * m + 4 * wave + (lane >> 4), rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
@@ -330,12 +215,11 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     unsigned at = __builtin_amdgcn_readlane(ids, 0);
 #pragma unroll
     for (int c = 0; c < 4; c++) load(p.k_pages, at, c);
-    constexpr int QS = HD + 8;   // LDS row stride of the q rows
     _Float16 *const qs = (_Float16 *)&os[0][0][0];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int r = 16 * m + 4 * wave + (lane >> 4);
-        make_part(p, raw[m], part, qs + r * QS, p.ovf ? p.ovf + q0 : nullptr);
+        make_part(p, norm, raw[m], part, qs + r * QS, p.ovf ? p.ovf + q0 : nullptr);
     }
     landed();
     lds_barrier();
@@ -455,13 +339,15 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     };
     for (int i = 0; i + 1 < n_mine; i++) page(i, std::true_type{});
     if (n_mine > 0) page(n_mine - 1, std::false_type{});
-    Gate16 gate[MT];   // of the outputs that the thread will finish
+    uint2 gate[MT][4];   // of the outputs that the lane will finish: rows wave, wave + 4, ..., dims 4 lane ..
     if (slot < 0)
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int fr = row0 + min(16 * m + (tid >> 4), rows - 1), t = fr / p.group;
-            gate[m] = load_gate(p, q0 + t, kh * p.group + fr - t * p.group, 16 * (tid & 15));
-        }
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int fr = row0 + min(16 * m + 4 * i + wave, rows - 1), t = fr / p.group;
+                gate[m][i] = load_gate(p, q0 + t, kh * p.group + fr - t * p.group, 4 * lane);
+            }
     // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^5 P)
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -481,28 +367,25 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 #pragma unroll
         for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
         __syncthreads();
-        const int r = tid >> 4, d0 = 16 * (tid & 15), row = 16 * m + r;
-        if (row < rows) {
-            float x[16], l = 0.f;
-            float mrow = kNone;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 4 * i + wave, row = 16 * m + r;
+            if (row >= rows) break;
+            float mrow = kNone, l = 0.f;
 #pragma unroll
             for (int w = 0; w < kRowsWaves; w++) mrow = fmaxf(mrow, ml[w][row][0]);
 #pragma unroll
             for (int w = 0; w < kRowsWaves; w++) l += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - mrow);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = os[0][r][d0 + i] + os[1][r][d0 + i] + os[2][r][d0 + i] + os[3][r][d0 + i];
+            for (int w = 0; w < kRowsWaves; w++) x += *(const f32x4 *)&os[w][r][4 * lane];
             if (slot < 0) {
-                const int fr = row0 + row, t = fr / p.group, head = kh * p.group + fr - t * p.group;
-                const float inv = 1.f / l;
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] *= inv;
-                finish16(p, q0 + t, head, d0, gate[m], x, p.ovf ? p.ovf + q0 : nullptr);
+                const int fr = row0 + row, t = fr / p.group;
+                finish4(p, q0 + t, kh * p.group + fr - t * p.group, 4 * lane, gate[m][i], x * (1.f / l), p.ovf ? p.ovf + q0 : nullptr);
             } else {
                 const size_t pr = partial_row(p, slot, kh, row);
-                float *dst = p.partial + pr * HD + d0;
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) *(f32x4 *)(dst + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-                if ((tid & 15) == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
+                *(f32x4 *)(p.partial + pr * HD + 4 * lane) = x;
+                if (lane == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
             }
         }
         if (m + 1 < MT) __syncthreads();
@@ -575,21 +458,20 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
         t = fr / p.group;
         head = kh * p.group + fr - t * p.group;
     };
-    // the wave makes the operands of one of its group's two tiles and takes the other's through LDS
-    QRow raw;
-    {
-        int t, head;
-        row_at(half, t, head);
-        load_q(p, q0 + t, head, g, raw);
+    // lane j: page (i & ~63) + j of the run that is being loaded (ids), or being scored (scales); behind the last: the last
+    auto number = [&](int i0) { return (unsigned)table[pg0 + min(i0 + lane, n - 1)]; };
+    auto in_pool = [&](unsigned id) { return (id < (unsigned)p.n_pages ? id : 0u) * p.nkv + kh; };
+    unsigned ids = number(0);
+    // 32 q rows at a time, 16 lanes each; loads go out in the order of their uses, none conditionally
+    QNorm norm;
+    QPart raw[4];
+    load_norm(p, lane & 15, norm);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int fr = row0 + min(32 * k + (tid >> 4), rows - 1), t = fr / p.group;
+        load_part(p, q0 + t, kh * p.group + fr - t * p.group, lane & 15, raw[k]);
     }
-    // lane j: page (i & ~63) + j of the run that is being loaded (ids), or being scored (scales)
-    unsigned ids = 0;
-    auto look_up = [&](int i0) {
-        const int i = i0 + lane;
-        unsigned id = i < n ? (unsigned)table[pg0 + i] : 0u;
-        if (id >= (unsigned)p.n_pages) id = 0;
-        return id * p.nkv + kh;
-    };
+    __builtin_amdgcn_sched_barrier(0);
     const unsigned lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;
     const unsigned pofs = (wave >> 1) * 4096 + (wave & 1) * 512 + lofs;   // pieces 2 wave and 2 wave + 1 of a page
     u32x4 kr[2], vr[2];
@@ -603,28 +485,22 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
         lds_write<1024>(dst, codes_f16(r[2], r[3]));
     };
     const unsigned k_out = lds_at(sm.k[4 * wave]) + 16 * lane, v_out = lds_at(sm.v[4 * wave]) + 16 * lane;
-    ids = look_up(0);
+    ids = in_pool(ids);
     float kss = p.k_scale[ids], vss = p.v_scale[ids];
     unsigned id_next = __builtin_amdgcn_readlane(ids, n > 1 ? 1 : 0);   // of page i + 1
     load(kr, p.k_pages, __builtin_amdgcn_readlane(ids, 0));
     load(vr, p.v_pages, __builtin_amdgcn_readlane(ids, 0));
+    _Float16 *const qs = (_Float16 *)&sm;   // the rows lie where K, V and P will
+#pragma unroll
+    for (int k = 0; k < 4; k++) make_part(p, norm, raw[k], lane & 15, qs + (32 * k + (tid >> 4)) * QS, flag_row);
+    if (tid < 2) sm.flag[tid] = 0;
+    lds_barrier();
     f16x8 q[2][8];
-    {
-        f16x8 mine[8];
-        make_q(p, raw, g, mine, flag_row);
-        u32x4(*const ex)[64] = sm.k;   // exchanged in the 64 KB of the K and V slots
 #pragma unroll
-        for (int c = 0; c < 8; c++) ex[8 * wave + c][lane] = __builtin_bit_cast(u32x4, mine[c]);
-        if (tid < 2) sm.flag[tid] = 0;
-        lds_barrier();
+    for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-            const f16x8 other = __builtin_bit_cast(f16x8, ex[8 * (wave ^ 4) + c][lane]);
-            q[0][c] = half ? other : mine[c];
-            q[1][c] = half ? mine[c] : other;
-        }
-        lds_barrier();
-    }
+        for (int c = 0; c < 8; c++) q[m][c] = *(const f16x8 *)(qs + (32 * rg + 16 * m + q16) * QS + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+    lds_barrier();
     store(k_out, kr[0]);
     store(k_out + 2048, kr[1]);
     load(kr, p.k_pages, id_next);
@@ -662,7 +538,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
             }
         }
         if (i && (i & 63) == 0) {   // the scales of the next run
-            const unsigned id = look_up(i);
+            const unsigned id = in_pool(number(i));
             kss = p.k_scale[id];
             vss = p.v_scale[id];
             asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here and not at every page
@@ -783,47 +659,74 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
         };
         text::static_for<4>(v_part);
         const int ahead = min(i + 2, n - 1);
-        if (ahead == i + 2 && (ahead & 63) == 0) ids = look_up(ahead);
+        if (ahead == i + 2 && (ahead & 63) == 0) ids = in_pool(number(ahead));
         id_next = __builtin_amdgcn_readlane(ids, ahead & 63);
         load(kr, p.k_pages, id_next);
         if (tid == 0) sm.flag[(i + 1) & 1] = 0;
     }
-    Gate16 gate[2][2];
+    // The outputs go through LDS, 16 rows of the wave's 128 dims at a time, so that a store takes whole lines: lane dims
+    // 4 (lane & 31) .. of rows 2 k + (lane >> 5). (Stored as they lie in registers, 16 bytes of each of 64 rows and dim
+    // groups: 13,000 clocks of the 54,000 of a cut block of four pages; now 6,000 of 42,000.)
+    int t_own[2], head_own[2], unit_own[2];   // token, q head and output row of the lane's own rows
+    uint2 gate[2][8];
+    const int d0 = 128 * half + 4 * (lane & 31);
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        row_at(m, t_own[m], head_own[m]);
+        unit_own[m] = (q0 + t_own[m]) * p.nh + head_own[m];
+    }
+    auto of_row = [&](int own, int k) {   // what lane 2 k, or 2 k + 1 in the upper half, has of its row
+        const int a = __builtin_amdgcn_readlane(own, 2 * k), b = __builtin_amdgcn_readlane(own, 2 * k + 1);
+        return lane & 32 ? b : a;
+    };
     if (slot < 0)
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            int t, head;
-            row_at(m, t, head);
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) gate[m][c] = load_gate(p, q0 + t, head, 128 * half + 64 * c + 16 * g);
-        }
+            for (int k = 0; k < 8; k++) gate[m][k] = load_gate(p, q0 + of_row(t_own[m], k), of_row(head_own[m], k), d0);
 #pragma unroll
     for (int m = 0; m < 2; m++) {
         sum[m] = text::xrow_sum(sum[m]);
         if (g == 0) sm.sum[rg][half][16 * m + q16] = sum[m];
     }
     lds_barrier();
+    constexpr int OS = 128 + 4;   // LDS row stride
+    float *const os = (float *)&sm + wave * 16 * OS;
 #pragma unroll
     for (int m = 0; m < 2; m++) {
-        const int row = 32 * rg + 16 * m + q16;
-        if (row >= rows) continue;
-        int t, head;
-        row_at(m, t, head);
         const float l = sm.sum[rg][0][16 * m + q16] + sm.sum[rg][1][16 * m + q16];
         const float f = slot < 0 ? pow2(unit) / l : pow2(unit);
-        const size_t pr = slot < 0 ? 0 : partial_row(p, slot, kh, row);
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int d0 = 128 * half + 64 * c + 16 * g;
-            float x[16];
+        for (int d = 0; d < 8; d++) *(f32x4 *)(os + q16 * OS + 64 * (d >> 2) + 16 * g + 4 * (d & 3)) = o[m][d] * f;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own rows
+        const int row0_m = 32 * rg + 16 * m;
+        if (slot >= 0 && g == 0 && half == 0 && row0_m + q16 < rows)
+            *(float2 *)(partial_ml(p) + 2 * partial_row(p, slot, kh, row0_m + q16)) = make_float2(mx[m], l);
+        f32x4 x[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = o[m][4 * c + (e >> 2)][e & 3] * f;
-            if (slot < 0) finish16(p, q0 + t, head, d0, gate[m][c], x, flag_row);
-            else
+        for (int k = 0; k < 8; k++) x[k] = *(const f32x4 *)(os + (2 * k + (lane >> 5)) * OS + 4 * (lane & 31));
+        auto put = [&](auto store) {   // one loop of stores for each kind, not a choice at each store
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) *(f32x4 *)(p.partial + pr * HD + d0 + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+            for (int k = 0; k < 8; k++)
+                if (row0_m + 2 * k + (lane >> 5) < rows) store(k, x[k]);
+        };
+        auto finished = [&](auto type) {
+            put([&](int k, f32x4 v) {
+                store_out4(p.out, (size_t)of_row(unit_own[m], k) * HD + d0, v, decltype(type)::value, p.f16_lim, flag_row);
+            });
+        };
+        if (slot >= 0) {
+            float *const dst = p.partial + partial_row(p, slot, kh, row0_m + (lane >> 5)) * HD + d0;
+            put([&](int k, f32x4 v) { *(f32x4 *)(dst + 2 * k * HD) = v; });
+        } else {
+            if (p.gate)
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = gated(x[k], gate[m][k]);
+            if (p.out_type == CLEF_HIP_OUT_BF16) finished(std::integral_constant<int, CLEF_HIP_OUT_BF16>{});
+            else if (p.out_type == CLEF_HIP_OUT_F16) finished(std::integral_constant<int, CLEF_HIP_OUT_F16>{});
+            else finished(std::integral_constant<int, CLEF_HIP_OUT_F32>{});
         }
-        if (slot >= 0 && g == 0 && half == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mx[m], l);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -848,7 +751,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
         uint2 gate = {0, 0};
         if (u < units) {
             blk = ((const int4 *)(p.plan + p.l.blk))[b];
-            if (p.gate) gate = *(const uint2 *)(p.qkv + (size_t)t * p.row + (size_t)head * 2 * HD + HD + 4 * lane);
+            gate = load_gate(p, t, head, 4 * lane);
         }
         const int n = __builtin_amdgcn_readfirstlane(blk.y), row = fr - blk.z;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -898,14 +801,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
             }
         }
         if (n > 1 && sub == 0) {
-            o *= 1.f / l;
-            if (p.gate) {
-                o[0] *= sigmoidf(bf_lo(gate.x));
-                o[1] *= sigmoidf(bf_hi(gate.x));
-                o[2] *= sigmoidf(bf_lo(gate.y));
-                o[3] *= sigmoidf(bf_hi(gate.y));
-            }
-            store_out4(p.out, ((size_t)t * p.nh + head) * HD + 4 * lane, o, p.out_type, p.f16_lim, p.ovf ? p.ovf + t - tok.y : nullptr);
+            finish4(p, t, head, 4 * lane, gate, o * (1.f / l), p.ovf ? p.ovf + t - tok.y : nullptr);
         }
         if (W > 1) __syncthreads();
     }
