@@ -64,8 +64,9 @@ def _check_attention(out, model_len_before, new, cu, q, gate, cache, model, valu
 
 
 def _run(nh, nkv, passes, seed=0, n_rot=64, norm=True, gate=True, out_dtype="bf16", max_pages=80, n_pages=400, max_new="known",
-         extra=0, scale=1.0, ovf=False, theta=1e7):
-    """Runs passes (lists of new tokens per sequence) one after the other and checks each."""
+         extra=0, scale=1.0, ovf=False, theta=1e7, spare=2):
+    """Runs passes (lists of new tokens per sequence) one after the other and checks each; each pass has spare rows more
+    than its tokens need (with many, and of more than 64 rows a sequence and kv head, the form of large passes runs)."""
     n_seq = len(passes[0])
     cache = Kv8Cache(1, nkv, n_pages, n_seq, max_pages)
     model = ref.Cache(n_pages, n_seq, max_pages)
@@ -73,7 +74,7 @@ def _run(nh, nkv, passes, seed=0, n_rot=64, norm=True, gate=True, out_dtype="bf1
     cache.v[0].fill_(0xff)
     att = TextAttention(nh, nkv, HD, n_rot, rope_theta=theta)
     for i, new in enumerate(passes):
-        T = sum(max(n, 0) for n in new) + 2
+        T = sum(max(n, 0) for n in new) + spare
         _say(f"heads {nh}/{nkv} pass {i} new {new} T {T}")
         plan = Kv8Plan(cache, T, nh, max(new) if max_new == "known" else max_new)
         before = model.len.copy()
@@ -104,7 +105,7 @@ def _run(nh, nkv, passes, seed=0, n_rot=64, norm=True, gate=True, out_dtype="bf1
                 room = np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s.T[..., None]) * (1 + 2.0 ** -12) + 2.0 ** -19 * np.abs(x).max(-1, keepdims=True)
                 assert (np.abs(got - x) <= room).all(), f"codes of sequence {r}"
         _check_attention(out, before, new, cu, q, g, cache, model, values, HD ** -0.5, gate, out_dtype)
-        assert (out[T - 2:] == 7.0).all(), "rows behind the last sequence changed"
+        assert (out[T - spare:] == 7.0).all(), "rows behind the last sequence changed"
     return cache, model
 
 
@@ -114,30 +115,41 @@ def test_tokens_and_prompts(nh, nkv):
     _run(nh, nkv, [[70, 1, 128, 63, 0], [1, 1, 1, 1, 1], [1, 64, 0, 2, -1], [0, 5, 1, 66, 90]], seed=nh)
 
 
+@pytest.mark.parametrize("nh,nkv", [(24, 4), (16, 4), (8, 8), (16, 1), (5, 1), (40, 2)])
+def test_tokens_and_prompts_large(nh, nkv):
+    """The same in passes that have the rows of large ones."""
+    _run(nh, nkv, [[70, 1, 128, 63, 0], [1, 1, 1, 1, 1], [1, 64, 0, 2, -1], [0, 5, 1, 66, 90]], seed=nh, max_new=None, spare=8192 // nh + 1)
+
+
+@pytest.mark.parametrize("room", [2, 342])
 @pytest.mark.parametrize("max_new", [None, 1, 3, 200])
-def test_max_new_is_a_hint(max_new):
-    _run(24, 4, [[40, 3, 100], [1, 2, 3], [5, 1, 130]], max_new=max_new, seed=3)
+def test_max_new_is_a_hint(max_new, room):
+    _run(24, 4, [[40, 3, 100], [1, 2, 3], [5, 1, 130]], max_new=max_new, seed=3, spare=room)
 
 
+@pytest.mark.parametrize("max_new,room", [("known", 2), (None, 513)])
 @pytest.mark.parametrize("lens", [[1], [63], [64], [65], [300], [1, 2, 3, 4, 5, 6, 7, 8]])
-def test_lengths(lens):
-    _run(16, 4, [lens, [1] * len(lens)], seed=len(lens) + lens[0])
+def test_lengths(lens, max_new, room):
+    _run(16, 4, [lens, [1] * len(lens)], seed=len(lens) + lens[0], max_new=max_new, spare=room)
 
 
-def test_long_sequence_is_cut():
+@pytest.mark.parametrize("max_new,room", [("known", 2), (None, 1025)])
+def test_long_sequence_is_cut(max_new, room):
     """One sequence whose pages are split over many workgroups and joined."""
-    _run(8, 2, [[1300], [1], [2], [5]], seed=11)
+    _run(8, 2, [[1300], [1], [2], [5]], seed=11, max_new=max_new, spare=room)
 
 
+@pytest.mark.parametrize("max_new,room", [("known", 2), (None, 1025)])
 @pytest.mark.parametrize("out_dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("n_rot,norm,gate", [(64, True, True), (0, False, False), (64, False, True)])
-def test_variants(out_dtype, n_rot, norm, gate):
-    _run(8, 4, [[33, 100], [1, 1]], n_rot=n_rot, norm=norm, gate=gate, out_dtype=out_dtype, seed=5)
+def test_variants(out_dtype, n_rot, norm, gate, max_new, room):
+    _run(8, 4, [[33, 100], [1, 1]], n_rot=n_rot, norm=norm, gate=gate, out_dtype=out_dtype, seed=5, max_new=max_new, spare=room)
 
 
-def test_sharp_rows_and_row_stride():
+@pytest.mark.parametrize("max_new,room", [("known", 2), (None, 1025)])
+def test_sharp_rows_and_row_stride(max_new, room):
     """Keys that dominate their rows (large queries and keys, no norm), and rows wider than needed."""
-    _run(8, 4, [[90], [1], [7]], n_rot=0, norm=False, scale=4.0, extra=24, seed=8)
+    _run(8, 4, [[90], [1], [7]], n_rot=0, norm=False, scale=4.0, extra=24, seed=8, max_new=max_new, spare=room)
 
 
 @pytest.mark.parametrize("n_seq,new,group", [(70, 1, 2), (70, 3, 8), (40, 40, 4), (6, 1, 1)])
@@ -182,13 +194,13 @@ def test_items_of_many_pages(n_seq, new, group):
             assert (d <= off).all(), (r, t, float((d / off).max()))
 
 
-@pytest.mark.parametrize("new", [[1], [40]])
+@pytest.mark.parametrize("new,rows", [([1], 1), ([40], 40), ([40], 4097)])
 @pytest.mark.parametrize("where", ["first", "last"])
-def test_many_small_weights(new, where):
+def test_many_small_weights(new, rows, where):
     """One key outweighs each other one by 2^23, and together they make 0.4% of the output: weights far below the
     largest still count, whether the largest comes before or behind them."""
     nh, nkv, n = 2, 1, 32768
-    _say("small weights", new, where)
+    _say("small weights", new, rows, where)
     cache, model = Kv8Cache(1, nkv, 520, 1, 520), ref.Cache(520, 1, 520)
     att = TextAttention(nh, nkv, HD, 0)
     plan = Kv8Plan(cache, n, nh)
@@ -201,12 +213,12 @@ def test_many_small_weights(new, where):
     qkv[at, 2 * nh * HD + HD:] = 0
     att.forward_kv8(qkv, None, None, None, plan, cache, 0, stage="append")
     T = new[0]
-    plan = Kv8Plan(cache, T, nh, T)
+    plan = Kv8Plan(cache, rows, nh, T)
     plan.update(_int(new))
-    model.plan(new, T)
-    q = torch.zeros(T, att.row, dtype=torch.bfloat16, device="cuda")
+    model.plan(new, rows)
+    q = torch.zeros(rows, att.row, dtype=torch.bfloat16, device="cuda")
     q[:, 0] = q[:, 2 * HD] = 16.0                                     # scores 16 = 23.08 in log2, and 0
-    out = att.forward_kv8(q, None, None, None, plan, cache, 0, gate=False)
+    out = att.forward_kv8(q, None, None, None, plan, cache, 0, gate=False)[:T]
     torch.cuda.synchronize()
     rest = np.arange(T)[:, None] + n - 1                              # other keys of value 1 (the new ones' values are 0)
     w = np.exp(-16.0)
@@ -254,8 +266,8 @@ def test_codes_exact(magnitude):
             assert np.array_equal((got[page] * scale[page][:, None, None])[:, :m], val[:, :m]), (name, page)
 
 
-@pytest.mark.parametrize("last", [1, 30])
-def test_pages_of_very_different_magnitude(last):
+@pytest.mark.parametrize("last,room", [(1, 0), (30, 0), (30, 2049)])
+def test_pages_of_very_different_magnitude(last, room):
     """Pages whose keys and values differ by up to 2^75 in one sequence, in both orders: the outputs' units move with them."""
     nh, nkv, mags = 4, 2, [2.0 ** 13, 2.0 ** -60, 1.0, 2.0 ** -20, 2.0 ** 12, 2.0 ** -62, 2.0 ** -3]
     for order in (mags, mags[::-1]):
@@ -266,18 +278,18 @@ def test_pages_of_very_different_magnitude(last):
         att = TextAttention(nh, nkv, HD, 0)
         for i, n in enumerate([PAGE] * len(order) + [last]):
             before = model.len.copy()
-            plan = Kv8Plan(cache, n, nh, n)
+            plan = Kv8Plan(cache, n + room, nh, None if room else n)
             plan.update(_int([n]))
-            _, cu, _, _ = model.plan([n], n)
-            qkv, _, _ = _qkv(n, nh, nkv, 60 + i)
+            _, cu, _, _ = model.plan([n], n + room)
+            qkv, _, _ = _qkv(n + room, nh, nkv, 60 + i)
             if i < len(order):
                 x = qkv.float()
                 x[:, 2 * nh * HD:] *= order[i]
                 qkv = x.to(torch.bfloat16)
             out = att.forward_kv8(qkv, None, None, None, plan, cache, 0)
             torch.cuda.synchronize()
-            q, _, _, g = ref.rows(_np(qkv.float()), nh, nkv, 0, None, None, None)
-            _check_attention(out, before, [n], cu, q, g, cache, model, _cache_values(cache), HD ** -0.5, True)
+            q, _, _, g = ref.rows(_np(qkv[:n].float()), nh, nkv, 0, None, None, None)
+            _check_attention(out[:n], before, [n], cu, q, g, cache, model, _cache_values(cache), HD ** -0.5, True)
 
 
 def test_other_pages_and_rows_untouched():
@@ -303,31 +315,32 @@ def test_other_pages_and_rows_untouched():
         assert same[~mine].all() and not same[mine].all()
 
 
-def test_bad_values_saturate_and_flag():
+@pytest.mark.parametrize("rows", [90, 1025])
+def test_bad_values_saturate_and_flag(rows):
     """Infinities, NaN and values beyond the limit in queries, keys and values: finite outputs and one flag at the
     sequence's first row; other sequences' rows keep their results bit for bit."""
     nh, nkv, lens = 8, 2, [20, 30, 40]
     res = []
     for bad in (False, True):
-        _say("bad values", bad)
+        _say("bad values", bad, rows)
         cache = Kv8Cache(1, nkv, 8, 3, 4)
-        plan = Kv8Plan(cache, 90, nh)
+        plan = Kv8Plan(cache, rows, nh)
         plan.update(_int(lens))
-        qkv, _, _ = _qkv(90, nh, nkv, 4)
+        qkv, _, _ = _qkv(rows, nh, nkv, 4)
         if bad:
             qkv[25, 3] = float("nan")                          # a query of sequence 1
             qkv[30, 2 * nh * HD + 5] = float("inf")            # a key of it
             qkv[31, (2 * nh + nkv) * HD + 9] = -float("inf")   # a value of it
-        ovf = torch.zeros(90, dtype=torch.int32, device="cuda")
+        ovf = torch.zeros(rows, dtype=torch.int32, device="cuda")
         out = TextAttention(nh, nkv, HD, 0).forward_kv8(qkv, None, None, None, plan, cache, 0, ovf=ovf)
         torch.cuda.synchronize()
-        flags = np.zeros(90, np.int32)
+        flags = np.zeros(rows, np.int32)
         flags[20] = bad
         assert np.array_equal(_np(ovf), flags)
-        assert torch.isfinite(out.float()).all()
+        assert torch.isfinite(out[:90].float()).all()
         res.append(out)
-    rows = [i for i in range(90) if not 20 <= i < 50]
-    assert torch.equal(res[0][rows].view(torch.int16), res[1][rows].view(torch.int16))
+    others = [i for i in range(90) if not 20 <= i < 50]
+    assert torch.equal(res[0][others].view(torch.int16), res[1][others].view(torch.int16))
 
 
 def test_f16_output_saturates():
