@@ -745,14 +745,18 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
     __shared__ float os[kJoinWaves][HD], ml[kJoinWaves][2];
     const int32_t *h = p.plan;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int most = h[H_MOST], units = h[H_TOKENS] * p.nh;
-    if (!plan_fits(h, p.n_seq, p.T, p.group, p.l.bm) || most <= 1) return;
+    // a unit's wave or waves depend on the header: the token entries of both choices are asked for with it
+    const int2 *const toks = (const int2 *)(p.plan + p.l.tok);
+    const int2 tok1 = toks[min(((int)blockIdx.x * kJoinWaves + wave) / p.nh, p.T - 1)], tok4 = toks[min((int)blockIdx.x / p.nh, p.T - 1)];
+    int4 first = {tok1.x, tok1.y, tok4.x, tok4.y}, head_words = {h[H_MOST], h[H_TOKENS], 0, 0};
+    if (!plan_has(h, H_MOST, 1, p.n_seq, p.T, p.group, p.l.bm, first, head_words)) return;   // no block is cut
+    const int most = head_words.x, units = head_words.y * p.nh;
     const int W = most <= kJoinBatch / 2 ? 1 : kJoinWaves, sub = wave & (W - 1), per = kJoinWaves / W;
     const int rounds = (units + per * (int)gridDim.x - 1) / (per * (int)gridDim.x);
     for (int round = 0; round < rounds; round++) {
         const int u = (round * (int)gridDim.x + (int)blockIdx.x) * per + wave / W;
         const int t = min(u / p.nh, p.T - 1), head = u % p.nh, kh = head / p.group;
-        const int2 tok = ((const int2 *)(p.plan + p.l.tok))[t];
+        const int2 tok = round ? toks[t] : W == 1 ? make_int2(first.x, first.y) : make_int2(first.z, first.w);
         const int fr = tok.y * p.group + head - kh * p.group, b = tok.x + fr / p.l.bm;
         int4 blk = {0, 0, 0, 0};
         uint2 gate = {0, 0};
