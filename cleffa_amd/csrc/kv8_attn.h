@@ -171,11 +171,10 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     constexpr int BM = 16 * MT, OS = HD + 4;   // LDS row stride of the outputs
     __shared__ __attribute__((aligned(16))) float os[kRowsWaves][16][OS];   // holds the q rows before
     __shared__ float ml[kRowsWaves][BM][2];
-    const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
     int4 e0 = it[0], e1 = it[1];
-    if (!plan_has(h, H_ITEMS, item, p.n_seq, p.T, p.group, p.l.bm, e0, e1)) return;
+    if (!plan_has(p, H_ITEMS, item, e0, e1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q16 = lane & 15, g = lane >> 4;
     const int lofs = (16 * (q16 >> 2) + (q16 & 3)) * 64 + 16 * g;   // the lane's piece of tile 0
@@ -445,11 +444,10 @@ __device__ __forceinline__ void lds_wait2(u32x4 (&r)[4], u32x4 &a, u32x4 &b) {
 }
 __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p) {
     __shared__ __attribute__((aligned(16))) TileLds sm;
-    const int32_t *h = p.plan;
     const int item = blockIdx.x / p.nkv, kh = blockIdx.x - item * p.nkv;
     const int4 *it = (const int4 *)(p.plan + p.l.items) + 2 * item;
     int4 e0 = it[0], e1 = it[1];
-    if (!plan_has(h, H_ITEMS, item, p.n_seq, p.T, p.group, p.l.bm, e0, e1)) return;
+    if (!plan_has(p, H_ITEMS, item, e0, e1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave & 3, half = wave >> 2;   // rows 32 rg .. 32 rg + 31, half of the tokens or dims
     const int q16 = lane & 15, g = lane >> 4;
@@ -743,13 +741,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kJoinBatch = 8;
 __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
     __shared__ float os[kJoinWaves][HD], ml[kJoinWaves][2];
-    const int32_t *h = p.plan;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // a unit's wave or waves depend on the header: the token entries of both choices are asked for with it
     const int2 *const toks = (const int2 *)(p.plan + p.l.tok);
     const int2 tok1 = toks[min(((int)blockIdx.x * kJoinWaves + wave) / p.nh, p.T - 1)], tok4 = toks[min((int)blockIdx.x / p.nh, p.T - 1)];
-    int4 first = {tok1.x, tok1.y, tok4.x, tok4.y}, head_words = {h[H_MOST], h[H_TOKENS], 0, 0};
-    if (!plan_has(h, H_MOST, 1, p.n_seq, p.T, p.group, p.l.bm, first, head_words)) return;   // no block is cut
+    int4 first = {tok1.x, tok1.y, tok4.x, tok4.y}, head_words = {p.plan[H_MOST], p.plan[H_TOKENS], 0, 0};
+    if (!plan_has(p, H_MOST, 1, first, head_words)) return;   // no block is cut
     const int most = head_words.x, units = head_words.y * p.nh;
     const int W = most <= kJoinBatch / 2 ? 1 : kJoinWaves, sub = wave & (W - 1), per = kJoinWaves / W;
     const int rounds = (units + per * (int)gridDim.x - 1) / (per * (int)gridDim.x);

@@ -71,10 +71,9 @@ constexpr int kAppendThreads = 256;
 __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Params p) {
     __shared__ float red[4];
     const int kh = blockIdx.x % p.nkv, item = blockIdx.x / p.nkv, tid = threadIdx.x;
-    const int32_t *h = p.plan;
     int4 it = ((const int4 *)(p.plan + p.l.app))[item];   // the grid ends with the list's room
     int4 none = {0, 0, 0, 0};
-    if (!plan_has(h, H_APPEND, item, p.n_seq, p.T, p.group, p.l.bm, it, none)) return;
+    if (!plan_has(p, H_APPEND, item, it, none)) return;
     const int page = it.x, t0 = it.y, off = it.z & 0xff, n = it.z >> 8, flag = it.w;
     if ((unsigned)page >= (unsigned)p.n_pages) return;
     const size_t at = (size_t)page * p.nkv + kh;

@@ -20,7 +20,7 @@ constexpr int kMaxGroup = 128;                 // q heads per kv head
 constexpr int32_t kPlanMagic = 0x4b563850;     // 'KV8P'
 
 // Plan header words. A failed plan leaves counts of 0, so the kernels that follow do nothing.
-enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_ITEMS, H_BLOCKS, H_SPLIT, H_MOST, H_WORDS = 16 };
+enum { H_MAGIC, H_SEQ, H_ROWS, H_SHAPE, H_TABLE, H_TOKENS, H_APPEND, H_ITEMS, H_MOST, H_WORDS = 16 };
 
 // Where the parts of a plan buffer lie (in int32) and how many entries each can need:
 //  the first block of each sequence (of passes whose rows a second kernel writes);
@@ -35,7 +35,7 @@ enum { H_MAGIC, H_SEQ, H_ROWS, H_GROUP, H_BM, H_STATUS, H_TOKENS, H_APPEND, H_IT
 // A block of p pages makes max(1, floor(p / C + 1/2)) items, C at least W / budget, W the pages of all
 // blocks: items <= blocks + budget, and those of cut blocks (split slots; p >= 1.5 C) <= 4 W / (3 C) < 2 budget.
 struct Layout {
-    int bm, budget, least, max_app, max_blk, max_items, max_slots;
+    int bm, shape, budget, least, max_app, max_blk, max_items, max_slots;
     long seq_blk, app, tok, blk, items, ints;
     size_t ws_bytes;
 };
@@ -50,6 +50,7 @@ inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
     // 30.9 against 38.1, 512 tokens 16/16 on 8,000 91.5 against 90.7; most is lost behind one very long text (1,536 rows on
     // 30,000 tokens 248 against 219). Above: 64 x 96 rows on 4,000 183 against 168, 16 x 128 tokens 16/16 222 against 181.
     l.bm = rows <= 16 ? 16 : rows <= 64 || (long)T * nh <= 8192 ? 32 : 128;
+    l.shape = G | nkv << 8 | l.bm << 20;   // what the lists go by beside n_seq and T
     l.budget = ((l.bm == 16 ? 2 : 1) * n_cu + nkv - 1) / nkv;   // items of one round of workgroups, two or one to a CU
     l.least = 4;
     const long app = (long)T / PAGE + 2L * n_seq;
@@ -88,20 +89,19 @@ struct Params {
     Layout l;
 };
 
-// A plan is run only with the sizes it was made for.
-__device__ __forceinline__ bool plan_fits(int magic, int seq, int rows, int rows_group, int rows_bm, int n_seq, int T, int group, int bm) {
-    return ((magic ^ kPlanMagic) | (seq ^ n_seq) | (rows ^ T) | (rows_group ^ group) | (rows_bm ^ bm)) == 0;
-}
-__device__ __forceinline__ bool plan_fits(const int32_t *h, int n_seq, int T, int group, int bm) {
-    return plan_fits(h[H_MAGIC], h[H_SEQ], h[H_ROWS], h[H_GROUP], h[H_BM], n_seq, T, group, bm);
+// A plan is run only with the sizes it was made for: list entries, items and split slots stay within those sizes.
+// One wait for all five words (&& would load each after the one before).
+__device__ __forceinline__ bool plan_fits(int magic, int seq, int rows, int shape, int table, const Params &p) {
+    return ((magic ^ kPlanMagic) | (seq ^ p.n_seq) | (rows ^ p.T) | (shape ^ p.l.shape) | (table ^ p.max_pages)) == 0;
 }
 // Whether list entry i of h[count] is one of a plan that fits. Its words a, b come with the header's, not behind the
 // check of them (one trip to memory for two: one token 7.1 -> 6.8 us): named together, all are loaded before.
-__device__ __forceinline__ bool plan_has(const int32_t *h, int count, int i, int n_seq, int T, int group, int bm, int4 &a, int4 &b) {
-    int magic = h[H_MAGIC], seq = h[H_SEQ], rows = h[H_ROWS], rows_group = h[H_GROUP], rows_bm = h[H_BM], n = h[count];
+__device__ __forceinline__ bool plan_has(const Params &p, int count, int i, int4 &a, int4 &b) {
+    const int32_t *h = p.plan;
+    int magic = h[H_MAGIC], seq = h[H_SEQ], rows = h[H_ROWS], shape = h[H_SHAPE], table = h[H_TABLE], n = h[count];
     asm volatile("" : "+s"(a.x), "+s"(a.y), "+s"(a.z), "+s"(a.w), "+s"(b.x), "+s"(b.y), "+s"(b.z), "+s"(b.w),
-                      "+s"(magic), "+s"(seq), "+s"(rows), "+s"(rows_group), "+s"(rows_bm), "+s"(n));
-    return plan_fits(magic, seq, rows, rows_group, rows_bm, n_seq, T, group, bm) && i < n;
+                      "+s"(magic), "+s"(seq), "+s"(rows), "+s"(shape), "+s"(table), "+s"(n));
+    return plan_fits(magic, seq, rows, shape, table, p) && i < n;
 }
 
 }  // namespace kv8

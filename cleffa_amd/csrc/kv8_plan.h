@@ -226,7 +226,7 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
         rows = min(p.l.bm, q * p.group - row0);
         return (len[r] + (row0 + rows - 1) / p.group) / PAGE + 1;   // pages up to its last token's own key
     };
-    int n_items = 0, n_slots = 0;
+    int n_items = 0;
     if (good && n_blk) {
         int r = 0, row0 = 0, rows = 0;
         const int pages0 = tid < n_blk ? block(tid, r, row0, rows) : 0;   // of the thread's first block
@@ -303,7 +303,6 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
             }
         }
         n_items = at;
-        n_slots = at_slot;
     }
     __syncthreads();
     if (tid == 0) {
@@ -314,14 +313,11 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
         h[H_MAGIC] = kPlanMagic;
         h[H_SEQ] = n;
         h[H_ROWS] = p.T;
-        h[H_GROUP] = p.group;
-        h[H_BM] = p.l.bm;
-        h[H_STATUS] = status;
+        h[H_SHAPE] = p.l.shape;
+        h[H_TABLE] = p.max_pages;
         h[H_TOKENS] = good ? n_tok : 0;
         h[H_APPEND] = good ? n_app : 0;
         h[H_ITEMS] = n_items;
-        h[H_BLOCKS] = good ? n_blk : 0;
-        h[H_SPLIT] = n_slots;
         h[H_MOST] = most;   // items of the most cut block
     }
 }

@@ -680,11 +680,14 @@ def test_another_stream():
     assert torch.equal(out, want)
 
 
-def test_plan_of_another_shape_is_not_run():
-    """A plan buffer made for other sizes is left alone by the kernels: nothing is written."""
+@pytest.mark.parametrize("rows,heads,pages,max_new", [(31, 1, 10, None), (30, 2, 10, None), (30, 1, 11, None), (30, 1, 10, 4)])
+def test_plan_of_another_shape_is_not_run(rows, heads, pages, max_new):
+    """A plan buffer made for other sizes (rows; kv heads of the same group; table rows; another form's blocks) is left
+    alone by the kernels: nothing is written."""
     nh, nkv = 8, 2
+    _say("plan of", rows, heads, pages, max_new)
     cache, att = Kv8Cache(1, nkv, 20, 2, 10), TextAttention(nh, nkv)
-    plan, wrong = Kv8Plan(cache, 30, nh), Kv8Plan(cache, 31, nh)
+    plan, wrong = Kv8Plan(cache, 30, nh), Kv8Plan(Kv8Cache(1, nkv * heads, 20, 2, pages), rows, nh * heads, max_new)
     wrong.update(_int([20, 10]))
     plan.work[:16].copy_(wrong.work[:16])
     rows = _qkv(30, nh, nkv, 1)
