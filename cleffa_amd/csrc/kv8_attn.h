@@ -162,8 +162,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // four that K and V share: as a piece is used up, the one four later is loaded into its registers, so 16 KB a
 // wave are always in flight, and with 16 rows two workgroups fit a CU, one's prologue and joins behind the
 // other's stream. Page numbers and scales of a wave's next 64 pages are held one per lane. The four waves'
-// results join through LDS. One token of 16/4 heads behind 130,000: 48.4 us, 5.5 TB/s; of 64 sequences of 30 to 8,000
-// tokens (24/4): 49.6 us, 4.8 TB/s (a large copy: 4.9). Short ones are bound by the chain of loads: 6.7 us for one
+// results join through LDS. One token of 16/4 heads behind 130,000: 48.5 us, 5.5 TB/s; of 64 sequences of 30 to 8,000
+// tokens (24/4): 50 us, 4.7 TB/s (a large copy: 4.9). Short ones are bound by the chain of loads: 6.7 us for one
 // token on 4,091.
 constexpr int kRowsThreads = 256, kRowsWaves = 4;
 template <int MT>
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 // The maximum of a row is common to its two waves, and no page's own maximum is looked for while weights stay small: a
 // wave whose sums of eight weights pass what the slack allows says so in a flag; behind the barrier all waves then
 // take the pairs' new maxima and make that page's P again (the first page, and hardly ever after).
-// Bound by conversions and products together: 4 x 512 tokens of 16/4 heads on 2,048 take 96 us, 800 TFLOP/s (a large f16
+// Bound by conversions and products together: 4 x 512 tokens of 16/4 heads on 2,048 take 92 to 97 us, 800 to 840 TFLOP/s (a large f16
 // product: 1,209); a page takes 4,500 clocks of an item, of which the products alone are 2,050.
 constexpr int kTileThreads = 512;
 struct TileLds {
@@ -735,7 +735,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
 // Joins the items of cut blocks. A unit is a pass row's q head; one or four waves take its items in turn (by the
 // plan's most cut block: what a wave reads is in flight at once), a lane four dims, and the first of them adds
 // them up. The order is fixed, so results do not change from run to run. Bound by its chain of loads (header, token,
-// block, partial results): 4.6 us for one token's 24 heads in 16 pieces, 8.8 for 16 heads in 128; the last workgroup of
+// block, partial results): 4.2 us for one token's 24 heads in 16 pieces, 8.2 for 16 heads in 128; the last workgroup of
 // a block joining it instead took longer (64 sequences: 109 us for both against 52 + 7 with fences, 60.5 against 59.4
 // with write-through stores).
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kJoinBatch = 8;
