@@ -340,16 +340,20 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     };
     for (int i = 0; i + 1 < n_mine; i++) page(i, std::true_type{});
     if (n_mine > 0) page(n_mine - 1, std::false_type{});
-    uint2 gate[MT][4];   // of the outputs that the lane will finish: rows wave, wave + 4, ..., dims 4 lane ..
+    // the lane will finish dims 4 lane .. of rows wave, wave + 4, ...: their gates, and their places in the output
+    uint2 gate[MT][4];
+    int unit_row[MT][4];
     if (slot < 0)
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int fr = row0 + min(16 * m + 4 * i + wave, rows - 1), t = fr / p.group;
-                gate[m][i] = load_gate(p, q0 + t, kh * p.group + fr - t * p.group, 4 * lane);
+                const int fr = row0 + min(16 * m + 4 * i + wave, rows - 1), t = fr / p.group, head = kh * p.group + fr - t * p.group;
+                gate[m][i] = load_gate(p, q0 + t, head, 4 * lane);
+                unit_row[m][i] = (q0 + t) * p.nh + head;
             }
-    // join the waves: each scales its outputs to the common maximum and to units of 1 (sums are of 2^5 P)
+    // join the waves: each scales its outputs to the common maximum, to units of 1 (sums are of 2^5 P) and, if they
+    // are not partial results, by the sum of all
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         sum[m] = text::xrow_sum(sum[m]);
@@ -361,33 +365,33 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        float top = kNone;
+        const int own = 16 * m + q16;
+        float top = kNone, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][16 * m + q16][0]);
-        const float f = ldexpf(__builtin_amdgcn_exp2f(mx[m] - top), unit);
+        for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][own][0]);
+#pragma unroll
+        for (int w = 0; w < kRowsWaves; w++) l += ml[w][own][1] * __builtin_amdgcn_exp2f(ml[w][own][0] - top);
+        const float f = ldexpf(__builtin_amdgcn_exp2f(mx[m] - top), unit) * (slot < 0 ? 1.f / l : 1.f);
+        if (slot >= 0 && wave == 0 && g == 0 && own < rows) *(float2 *)(partial_ml(p) + 2 * partial_row(p, slot, kh, own)) = make_float2(top, l);
 #pragma unroll
         for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
         __syncthreads();
+        f32x4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = 4 * i + wave, row = 16 * m + r;
+            x[i] = *(const f32x4 *)&os[0][4 * i + wave][4 * lane];
+#pragma unroll
+            for (int w = 1; w < kRowsWaves; w++) x[i] += *(const f32x4 *)&os[w][4 * i + wave][4 * lane];
+        }
+        if (slot < 0 && p.gate)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = gated(x[i], gate[m][i]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 16 * m + 4 * i + wave;
             if (row >= rows) break;
-            float mrow = kNone, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kRowsWaves; w++) mrow = fmaxf(mrow, ml[w][row][0]);
-#pragma unroll
-            for (int w = 0; w < kRowsWaves; w++) l += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - mrow);
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < kRowsWaves; w++) x += *(const f32x4 *)&os[w][r][4 * lane];
-            if (slot < 0) {
-                const int fr = row0 + row, t = fr / p.group;
-                finish4(p, q0 + t, kh * p.group + fr - t * p.group, 4 * lane, gate[m][i], x * (1.f / l), p.ovf ? p.ovf + q0 : nullptr);
-            } else {
-                const size_t pr = partial_row(p, slot, kh, row);
-                *(f32x4 *)(p.partial + pr * HD + 4 * lane) = x;
-                if (lane == 0) *(float2 *)(partial_ml(p) + 2 * pr) = make_float2(mrow, l);
-            }
+            if (slot < 0) store_out4(p.out, (size_t)unit_row[m][i] * HD + 4 * lane, x[i], p.out_type, p.f16_lim, p.ovf ? p.ovf + q0 : nullptr);
+            else *(f32x4 *)(p.partial + partial_row(p, slot, kh, row) * HD + 4 * lane) = x[i];
         }
         if (m + 1 < MT) __syncthreads();
     }
