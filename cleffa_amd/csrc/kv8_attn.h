@@ -38,10 +38,16 @@ constexpr float kPUnit = 5.f, kSlack = 8.f;
 constexpr int kUnitSlack = 2;
 constexpr float kPMost = 8192.f;   // 2^(5 + 8): a weight as large as the slack allows, of a page in its own unit
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+// Maxima are of q . k with the K scale in it, a power of two, so they are exact images of the scores they came from; the
+// softmax scale times log2 e comes behind the difference from m. (A rounded product as m, and the weights from the exact
+// one, would part by half a step of m: 2^16 in a weight from scores of 2^28 on.)
+__device__ __forceinline__ float weight(float s, float k_scale, float m, float scale_log2, float unit) {
+    return __builtin_amdgcn_exp2f(fmaf(fmaf(s, k_scale, -m), scale_log2, unit));
+}
 // Moves m for a page whose largest score top passes it by more than the slack; returns the factor that sums under the old m take.
-__device__ __forceinline__ float new_max(float &m, float top, float slack) {
-    const float now = top > m + slack ? top : m;
-    const float f = __builtin_amdgcn_exp2f(m - now);
+__device__ __forceinline__ float new_max(float &m, float top, float slack, float scale_log2) {
+    const float now = (top - m) * scale_log2 > slack ? top : m;
+    const float f = __builtin_amdgcn_exp2f((m - now) * scale_log2);
     m = now;
     return f;
 }
@@ -146,7 +152,7 @@ __device__ __forceinline__ void finish4(const Params &p, int t, int head, int d0
 }
 
 // Partial results of a cut block: [split slot][kv head][row][256] unnormalised outputs, then
-// [split slot][kv head][row][2] running maximum (log2 units) and sum.
+// [split slot][kv head][row][2] running maximum (of q . k) and sum.
 __device__ __forceinline__ size_t partial_row(const Params &p, int slot, int kh, int row) {
     return ((size_t)slot * p.nkv + kh) * p.l.bm + row;
 }
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
     auto page = [&](int i, auto more_t) {
         constexpr bool MORE = decltype(more_t)::value;
         const int pg = pg0 + wave + kRowsWaves * i;
-        const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63));
         const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;   // the V scale is 2^ev
         f32x4 s[MT][4];
 #pragma unroll
@@ -287,14 +293,14 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) top = fmaxf(top, s[m][t][e]);
-            const float f = new_max(mx[m], text::xrow_max(top) * kf, kSlack);
+            const float f = new_max(mx[m], text::xrow_max(top) * ks, kSlack, p.scale_log2);
             float add = 0.f;
-            const float shift = kPUnit + (float)(ev - now_unit) - mx[m];
+            const float in_unit = kPUnit + (float)(ev - now_unit);
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[m][t][e], kf, shift));
+                    const float x = weight(s[m][t][e], ks, mx[m], p.scale_log2, in_unit);
                     add += x;
                     pb[m][t >> 1][4 * (t & 1) + e] = (_Float16)x;
                 }
@@ -370,8 +376,8 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 #pragma unroll
         for (int w = 0; w < kRowsWaves; w++) top = fmaxf(top, ml[w][own][0]);
 #pragma unroll
-        for (int w = 0; w < kRowsWaves; w++) l += ml[w][own][1] * __builtin_amdgcn_exp2f(ml[w][own][0] - top);
-        const float f = ldexpf(__builtin_amdgcn_exp2f(mx[m] - top), unit) * (slot < 0 ? 1.f / l : 1.f);
+        for (int w = 0; w < kRowsWaves; w++) l += ml[w][own][1] * __builtin_amdgcn_exp2f((ml[w][own][0] - top) * p.scale_log2);
+        const float f = ldexpf(__builtin_amdgcn_exp2f((mx[m] - top) * p.scale_log2), unit) * (slot < 0 ? 1.f / l : 1.f);
         if (slot >= 0 && wave == 0 && g == 0 && own < rows) *(float2 *)(partial_ml(p) + 2 * partial_row(p, slot, kh, own)) = make_float2(top, l);
 #pragma unroll
         for (int d = 0; d < 16; d++) *(f32x4 *)&os[wave][q16][64 * (d >> 2) + 16 * g + 4 * (d & 3)] = o[m][d] * f;
@@ -549,7 +555,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
             vss = p.v_scale[id];
             asm volatile("" : "+v"(kss), "+v"(vss));   // waited for here and not at every page
         }
-        const float kf = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63)) * p.scale_log2;
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), i & 63));
         const int ev = (int)(__builtin_amdgcn_readlane(__float_as_uint(vss), i & 63) >> 23) - 127;   // the V scale is 2^ev
         const int now_unit = abs(ev - unit) <= kUnitSlack ? unit : ev;
         const float in_unit = kPUnit + (float)(ev - now_unit), out_unit = pow2(now_unit - ev);
@@ -587,10 +593,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
         auto make_p = [&]() {
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                const float shift = in_unit - mx[m];
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], kf, shift));
+                for (int e = 0; e < 8; e++) x[e] = weight(s[m][e >> 2][e & 3], ks, mx[m], p.scale_log2, in_unit);
                 add[m] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
                 pb[m] = __builtin_bit_cast(f16x8, u32x4{pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7])});
                 sm.p[rg][half][m][lane] = __builtin_bit_cast(u32x4, pb[m]);
@@ -615,13 +620,13 @@ __global__ __launch_bounds__(kTileThreads, 2) void kv8_attn_tile_kernel(Params p
                 top[m] = s[m][0][0];
 #pragma unroll
                 for (int e = 1; e < 8; e++) top[m] = fmaxf(top[m], s[m][e >> 2][e & 3]);
-                top[m] = text::xrow_max(top[m]) * kf;
+                top[m] = text::xrow_max(top[m]) * ks;
                 if (g == 0) sm.top[rg][half][16 * m + q16] = top[m];
             }
             lds_barrier();
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                const float f = new_max(mx[m], fmaxf(sm.top[rg][0][16 * m + q16], sm.top[rg][1][16 * m + q16]), 0.f);
+                const float f = new_max(mx[m], fmaxf(sm.top[rg][0][16 * m + q16], sm.top[rg][1][16 * m + q16]), 0.f, p.scale_log2);
                 sum[m] *= f;
 #pragma unroll
                 for (int d = 0; d < 8; d++) o[m][d] *= f;
@@ -781,13 +786,13 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
                 float top = m;
 #pragma unroll
                 for (int j = 0; j < kJoinBatch; j++) top = fmaxf(top, e[j].x);
-                const float f = __builtin_amdgcn_exp2f(m - top);
+                const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
                 o *= f;
                 l *= f;
                 m = top;
 #pragma unroll
                 for (int j = 0; j < kJoinBatch; j++) {
-                    const float w = k0 + W * j < n ? __builtin_amdgcn_exp2f(e[j].x - top) : 0.f;
+                    const float w = k0 + W * j < n ? __builtin_amdgcn_exp2f((e[j].x - top) * p.scale_log2) : 0.f;
                     l += e[j].y * w;
                     o += x[j] * w;
                 }
@@ -802,11 +807,11 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Params p) {
             if (sub == 0) {
                 float top = m;
                 for (int w = 1; w < W; w++) top = fmaxf(top, ml[wave + w][0]);
-                const float f = __builtin_amdgcn_exp2f(m - top);
+                const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
                 o *= f;
                 l *= f;
                 for (int w = 1; w < W; w++) {
-                    const float g = __builtin_amdgcn_exp2f(ml[wave + w][0] - top);
+                    const float g = __builtin_amdgcn_exp2f((ml[wave + w][0] - top) * p.scale_log2);
                     l += ml[wave + w][1] * g;
                     o += *(const f32x4 *)&os[wave + w][4 * lane] * g;
                 }
