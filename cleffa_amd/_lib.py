@@ -110,7 +110,7 @@ class Kv8Args(ctypes.Structure):
         ("qkv", c_void_p), ("q_norm", c_void_p), ("k_norm", c_void_p), ("pos3", c_void_p), ("inv_freq", c_void_p),
         ("tables", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
         ("plan", c_void_p), ("gate", c_int), ("out", c_void_p), ("out_type", c_int), ("f16_lim", c_float),
-        ("ovf", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("ovf", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("plan_ints", c_size_t),
     ]
 
 

@@ -431,7 +431,7 @@ class TextAttention:
             to = _arg(out, "out", (T, self.nh * hd), odt, dev)
         a = _lib.Kv8Args(self.nh, self.nkv, hd, self.n_rot, self.eps, self.scale, T, row, cache.max_seqs, cache.max_pages, cache.n_pages,
                          plan.max_new, qkv, q_norm, k_norm, pos3, self.inv_freq.data_ptr(), *pools, plan.work.data_ptr(), int(gate), to,
-                         out_type, f16_lim, ovf, plan.workspace.data_ptr(), plan.workspace_bytes)
+                         out_type, f16_lim, ovf, plan.workspace.data_ptr(), plan.workspace_bytes, plan.work.numel())
         lib = _lib.load()
         if stage != "core":
             _launch(lib.clef_hip_kv8_append, a, dev, stream)

@@ -27,7 +27,7 @@ static __device__ __align__(256) unsigned char scratch[CLEF_HIP_VIS_SCRATCH_BYTE
 
 namespace {
 
-constexpr int kVersion = 5;
+constexpr int kVersion = 6;
 constexpr int32_t kSchedMagic = 0x53434844;   // header word of a schedule ('SCHD')
 constexpr int kSchedHeader = 8;                 // {magic, n_blk, nh, n_wg, nkv, fingerprint, 0, 0}
 // A 32-bit fingerprint of a block list: FNV-1a over words 0-6 of every entry (word 7 holds the

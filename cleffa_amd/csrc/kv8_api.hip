@@ -82,6 +82,8 @@ bool fill(const clef_hip_kv8_args *a, bool core, kv8::Params *q, char *err, size
         if (!a->workspace || !aligned16(a->workspace)) return fail(err, errlen, "workspace must be a 16-byte aligned device pointer");
         if (a->workspace_bytes < q->l.ws_bytes) return fail(err, errlen, "workspace of %zu bytes, %zu are needed", a->workspace_bytes, q->l.ws_bytes);
     }
+    // the kernels load their list entries, at offsets by these sizes, together with the plan's header
+    if (a->plan_ints < (size_t)q->l.ints) return fail(err, errlen, "plan of %zu int32, %ld are needed", a->plan_ints, q->l.ints);
     q->qkv = a->qkv; q->q_norm = a->q_norm; q->k_norm = a->k_norm; q->inv_freq = a->inv_freq; q->pos3 = a->pos3;
     q->tables = a->tables; q->plan = a->plan;
     q->k_pages = a->k_pages; q->v_pages = a->v_pages; q->k_scale = a->k_scale; q->v_scale = a->v_scale;

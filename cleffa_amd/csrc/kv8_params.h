@@ -95,7 +95,8 @@ __device__ __forceinline__ bool plan_fits(int magic, int seq, int rows, int shap
     return ((magic ^ kPlanMagic) | (seq ^ p.n_seq) | (rows ^ p.T) | (shape ^ p.l.shape) | (table ^ p.max_pages)) == 0;
 }
 // Whether list entry i of h[count] is one of a plan that fits. Its words a, b come with the header's, not behind the
-// check of them (one trip to memory for two: one token 7.1 -> 6.8 us): named together, all are loaded before.
+// check of them (one trip to memory for two: one token 7.1 -> 6.8 us): named together, all are loaded before. The host
+// has checked that the buffer is as long as this call's layout, so they lie within it whatever the header says.
 __device__ __forceinline__ bool plan_has(const Params &p, int count, int i, int4 &a, int4 &b) {
     const int32_t *h = p.plan;
     int magic = h[H_MAGIC], seq = h[H_SEQ], rows = h[H_ROWS], shape = h[H_SHAPE], table = h[H_TABLE], n = h[count];

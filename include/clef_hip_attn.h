@@ -450,7 +450,7 @@ typedef struct {
 bool clef_hip_kv8_plan(const clef_hip_kv8_plan_args *a, void *stream, char *err, size_t errlen);
 
 /* One full-attention layer of a planned pass. n_seq, T, nh, nkv and max_new are the plan's (a plan made for
- * others is not run: nothing is written). */
+ * others, in a buffer large enough for these, is not run: nothing is written). */
 typedef struct {
     int nh, nkv, hd, n_rot;   /* hd 256; n_rot 64 or 0 */
     float eps, scale;
@@ -472,6 +472,7 @@ typedef struct {
     int32_t *ovf;             /* [T] flags at each sequence's first pass row, or NULL */
     void *workspace;          /* attention only; calls that overlap need one each */
     size_t workspace_bytes;
+    size_t plan_ints;         /* int32 that plan holds: at least clef_hip_kv8_sizes' for this call's sizes (refused otherwise) */
 } clef_hip_kv8_args;
 /* The new tokens' keys (RMSNorm, rotary) and values into the pages that the plan names. Rows of a page
  * that hold no token of its sequence are left as they are. */
