@@ -17,6 +17,7 @@ BLOCK_Q = 128
 KV_ALIGN = 8
 BLOCK_INTS = 8
 KV8_PAGE, KV8_MAX_SEQ, KV8_MAX_ROWS = 64, 4096, 262143
+KV8_PLAN_STATUS, KV8_PLAN_FAILED = 9, 10
 
 # Every symbol include/clef_hip_attn.h declares.
 EXPORTS = (

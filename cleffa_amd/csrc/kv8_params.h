@@ -20,7 +20,8 @@ constexpr int kMaxGroup = 128;                 // q heads per kv head
 constexpr int32_t kPlanMagic = 0x4b563850;     // 'KV8P'
 
 // Plan header words. A failed plan leaves counts of 0, so the kernels that follow do nothing.
-enum { H_MAGIC, H_SEQ, H_ROWS, H_SHAPE, H_TABLE, H_TOKENS, H_APPEND, H_ITEMS, H_MOST, H_WORDS = 16 };
+enum { H_MAGIC, H_SEQ, H_ROWS, H_SHAPE, H_TABLE, H_TOKENS, H_APPEND, H_ITEMS, H_MOST,
+       H_STATUS = CLEF_HIP_KV8_PLAN_STATUS, H_FAILED = CLEF_HIP_KV8_PLAN_FAILED, H_WORDS = 16 };
 
 // Where the parts of a plan buffer lie (in int32) and how many entries each can need:
 //  the first block of each sequence (of passes whose rows a second kernel writes);

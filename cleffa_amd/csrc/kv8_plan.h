@@ -111,6 +111,7 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
     int *const cu_q = cu[0], *const cu_add = cu[1], *const cu_rel = cu[2], *const cu_app = cu[3], *const cu_blk = cu[4];
     const int tid = threadIdx.x, n = p.n_seq;
     const int n_free = p.state[0];
+    const int failed = p.work[H_MAGIC] == kPlanMagic ? p.work[H_FAILED] : 0;   // a buffer's first plan has none before it
     int status = (unsigned)n_free > (unsigned)p.n_pages ? CLEF_HIP_KV8_BAD_STATE : 0;
     int base[kPlanSums] = {0, 0, 0, 0, 0};
     if (tid == 0) bad = most = 0;   // the scans' barriers come before their first use
@@ -319,6 +320,8 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
         h[H_APPEND] = good ? n_app : 0;
         h[H_ITEMS] = n_items;
         h[H_MOST] = most;   // items of the most cut block
+        h[H_STATUS] = status;
+        h[H_FAILED] = failed | status;
     }
 }
 

@@ -14,6 +14,7 @@ A serving loop needs no host round trip between its passes:
         plan.update(new_lens)                       # state, tables, slots, positions: all on the device
         for l in range(n_layers):
             out = att.forward_kv8(qkv[l], q_norm, k_norm, plan.pos3, plan, cache, l)
+    assert not plan.failed()                        # where the loop waits anyway: no pass was left out
 """
 import ctypes
 
@@ -108,7 +109,7 @@ class Kv8Plan:
         self.work = torch.zeros(ints.value, dtype=torch.int32, device=dev)
         self.workspace = torch.empty(ws.value, dtype=torch.uint8, device=dev)
         self.workspace_bytes = ws.value
-        self.state = None   # the state that the last update wrote
+        self.state = None   # the state that the last update wrote (its word 1 is any other plan's too, see status())
 
     def update(self, new_lens, pos_off=None, state_out=None, stream=None):
         """Plans a pass: new_lens int32 [max_seqs] on the device (0: the sequence rests, negative: it has ended and
@@ -128,9 +129,16 @@ class Kv8Plan:
         return self
 
     def status(self):
-        """0, or what kept the last update from planning (waits for it). A pass that could not be planned changes
-        nothing: append and attention with it write nothing."""
-        return 0 if self.state is None else int(self.state[1])
+        """0, or what kept this plan's last update from planning (waits for it). A pass that could not be planned
+        changes nothing: append and attention with it write nothing."""
+        return int(self.work[_lib.KV8_PLAN_STATUS])
+
+    def failed(self):
+        """What kept any of this plan's updates since the last call of failed() from planning, or-ed (waits for
+        them): status() of a loop that looks only now and then, or is replayed from a graph."""
+        s = int(self.work[_lib.KV8_PLAN_FAILED])
+        self.work[_lib.KV8_PLAN_FAILED] = 0
+        return s
 
     def check(self):
         """Raises if the last update could not plan its pass."""

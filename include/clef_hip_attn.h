@@ -416,6 +416,9 @@ bool clef_hip_prefix_copy(const uint16_t *k_src, const uint16_t *vt_src, int src
 #define CLEF_HIP_KV8_ROWS 2       /* more new tokens than the pass has rows */
 #define CLEF_HIP_KV8_TOO_LONG 4   /* a sequence would pass max_pages pages */
 #define CLEF_HIP_KV8_BAD_STATE 8  /* lengths, counts or page numbers that cannot be */
+/* words of a plan buffer that a caller may look at (the rest is opaque) */
+#define CLEF_HIP_KV8_PLAN_STATUS 9   /* status of the last plan made in this buffer (state[1]: of the last made from that state) */
+#define CLEF_HIP_KV8_PLAN_FAILED 10  /* statuses of all plans made in it since the caller last set the word to 0, or-ed */
 
 /* The int32 of a plan buffer and the bytes of an attention workspace for passes of T rows over a table
  * of n_seq sequences. max_new: the most new tokens of a sequence in such a pass, or 0 if that is not
@@ -433,7 +436,8 @@ bool clef_hip_kv8_sizes(int n_seq, int T, int nh, int nkv, int max_new, size_t *
  *   slots [T]: page * 64 + token in page of each pass row, -1 behind the last sequence's rows;
  *   pos3 [T][3] (or NULL): text positions, the token's index in its sequence + pos_off[sequence]
  *   (pos_off NULL: 0) in all three; 0 behind the last sequence's rows;
- *   plan: the work lists of the append and attention kernels (opaque).
+ *   plan: the work lists of the append and attention kernels, and the two status words above. They are the buffer's
+ *   own: state[1] is overwritten by any other plan made from the same state, and by the next of a replayed loop.
  * All or nothing: where status (state_out[1]) is not 0, state_out is the state otherwise unchanged, no
  * page has changed hands, cu_q is 0, slots -1, and append and attention with this plan do nothing. */
 typedef struct {

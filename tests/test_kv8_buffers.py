@@ -45,3 +45,11 @@ def test_a_plan_one_short_is_refused(fn):
     assert not getattr(_lib.load(), fn)(ctypes.byref(a), None, err, 256) and b"are needed" in err.value
     a.plan_ints = 0
     assert not getattr(_lib.load(), fn)(ctypes.byref(a), None, err, 256) and b"are needed" in err.value
+
+
+def test_status_words_match_the_header():
+    import re
+    from pathlib import Path
+    text = (Path(__file__).resolve().parents[1] / "include" / "clef_hip_attn.h").read_text()
+    for name in ("STATUS", "FAILED"):
+        assert int(re.search(rf"#define CLEF_HIP_KV8_PLAN_{name} (\d+)", text).group(1)) == getattr(_lib, "KV8_PLAN_" + name)
