@@ -107,14 +107,14 @@ __global__ __launch_bounds__(kRowThreads) void kv8_plan_rows_kernel(PlanParams p
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
     constexpr int kPlanThreads = THREADS, kPlanWaves = THREADS / 64;
-    __shared__ int cu[kPlanSums][kMaxSeq + 1], len[kMaxSeq], held[kMaxSeq], fresh[kMaxFresh], waves[kChunks][kPlanWaves], bad, most;
+    __shared__ int cu[kPlanSums][kMaxSeq + 1], len[kMaxSeq], held[kMaxSeq], fresh[kMaxFresh], waves[kChunks][kPlanWaves], bad, bad_page, most;
     int *const cu_q = cu[0], *const cu_add = cu[1], *const cu_rel = cu[2], *const cu_app = cu[3], *const cu_blk = cu[4];
     const int tid = threadIdx.x, n = p.n_seq;
     const int n_free = p.state[0];
     const int failed = p.work[H_MAGIC] == kPlanMagic ? p.work[H_FAILED] : 0;   // a buffer's first plan has none before it
     int status = (unsigned)n_free > (unsigned)p.n_pages ? CLEF_HIP_KV8_BAD_STATE : 0;
     int base[kPlanSums] = {0, 0, 0, 0, 0};
-    if (tid == 0) bad = most = 0;   // the scans' barriers come before their first use
+    if (tid == 0) bad = bad_page = most = 0;   // the scans' barriers come before their first use
     for (int r0 = 0; r0 < n; r0 += kPlanThreads) {
         const int r = r0 + tid;
         int v[kPlanSums] = {0, 0, 0, 0, 0}, total[kPlanSums];
@@ -154,7 +154,8 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
     __syncthreads();
     status = bad;
     // The stack after the pages that come back are pushed: those lie above its old top. The pages that go out come
-    // off its top, into LDS; every page that changes hands is looked at before anything is written.
+    // off its top, into LDS; every page that changes hands is looked at before anything is written. Its finding has a
+    // word of its own: the one before may still be read, and all waves must take the same way past the barrier below.
     auto released = [&](int j) {
         const int r = find(cu_rel, n, j);
         return p.tables[(size_t)r * p.max_pages + j - cu_rel[r]];
@@ -167,9 +168,9 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
             odd |= (unsigned)page >= (unsigned)p.n_pages;
         }
         for (int j = tid; j < n_rel; j += kPlanThreads) odd |= (unsigned)released(j) >= (unsigned)p.n_pages;
-        if (odd) atomicOr(&bad, CLEF_HIP_KV8_BAD_STATE);
+        if (odd) atomicOr(&bad_page, CLEF_HIP_KV8_BAD_STATE);
         __syncthreads();
-        status = bad;
+        status = bad_page;
     }
     const bool good = status == 0;
     // the table's entry, also of pages that are only now written there
