@@ -90,5 +90,6 @@ def test_pages_of_different_magnitude(form, which, mags, whole):
     tight = np.median(off, -1) / np.median(np.abs(want), -1)
     assert tight.max() < 0.03, "the bound says too little"
     d = np.abs(_np(out)[:m].reshape(want.shape) - want)
-    _say(f"largest error {np.nanmax(d / off):.3f} of its bound, which is {tight.max():.4f} of the outputs")
+    with np.errstate(invalid="ignore"):   # a first token's value of 0
+        _say(f"largest error {np.nanmax(d / off):.3f} of its bound, which is {tight.max():.4f} of the outputs")
     assert (d <= off).all()
