@@ -407,7 +407,9 @@ bool clef_hip_prefix_copy(const uint16_t *k_src, const uint16_t *vt_src, int src
  *   state [2 + 2 n_seq] int32: {free pages on the stack, status of the last plan, then tokens and
  *   pages held of each sequence}. A caller may lower a sequence's tokens (a new request that shares only
  *   part of a cached text); its pages stay with it. Pages that several table rows share may be read, not
- *   appended to or released. */
+ *   appended to or released: a plan does not know whose they are, and would put them on the stack once for each. Before
+ *   a sequence that borrowed its first pages ends, the caller takes them out of its row: the later entries move
+ *   to the front, its pages go down by as many, its tokens to 0 (all on the device, as it lent them). */
 #define CLEF_HIP_KV8_PAGE 64
 #define CLEF_HIP_KV8_MAX_SEQ 4096     /* sequences of a table */
 #define CLEF_HIP_KV8_MAX_ROWS 262143  /* rows of a pass */
