@@ -111,7 +111,8 @@ __global__ __launch_bounds__(THREADS) void kv8_plan_kernel(PlanParams p) {
     int *const cu_q = cu[0], *const cu_add = cu[1], *const cu_rel = cu[2], *const cu_app = cu[3], *const cu_blk = cu[4];
     const int tid = threadIdx.x, n = p.n_seq;
     const int n_free = p.state[0];
-    const int failed = p.work[H_MAGIC] == kPlanMagic ? p.work[H_FAILED] : 0;   // a buffer's first plan has none before it
+    const int magic = p.work[H_MAGIC], kept = p.work[H_FAILED];
+    const int failed = kept & -(int)(magic == kPlanMagic);   // a buffer's first plan has none before it
     int status = (unsigned)n_free > (unsigned)p.n_pages ? CLEF_HIP_KV8_BAD_STATE : 0;
     int base[kPlanSums] = {0, 0, 0, 0, 0};
     if (tid == 0) bad = bad_page = most = 0;   // the scans' barriers come before their first use
