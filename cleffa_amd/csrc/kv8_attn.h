@@ -5,8 +5,8 @@
 // pages: one token of 24/4 heads is 6 rows of a 16-row matrix tile. Per 16-row tile and 64-token page
 //   S^T = K . Q^T     v_mfma_f32_16x16x32_f16: A = K codes as f16 (exact), B = Q (f16)
 //   O^T += V^T . P^T  v_mfma_f32_16x16x32_f16: A = V codes as f16 (exact), B = P (f16)
-// The page's K scale multiplies the f32 scores together with the softmax scale, its V scale is a unit of O or goes
-// into the exponent of P: neither costs an instruction per element. P in f16 rounds by 2^-11 of itself (bf16:
+// The page's K scale multiplies the f32 scores in the instruction that takes the maximum off, its V scale is a unit of O or
+// goes into the exponent of P: neither costs an instruction per element. P in f16 rounds by 2^-11 of itself (bf16:
 // 2^-8); against the row's largest it is held from 2^3 on, which keeps that down to P = 2^-17, with steps of
 // 2^-27 below. Units of 2^-64 to 2^8 leave O within 2^113 and 2^-100. Row r of A tile t (of four that make up 64
 // rows) is token / dim 16 (r / 4) + 4 t + r % 4: then a lane's 16 scores of a page are 16 consecutive tokens,
@@ -168,8 +168,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // four that K and V share: as a piece is used up, the one four later is loaded into its registers, so 16 KB a
 // wave are always in flight, and with 16 rows two workgroups fit a CU, one's prologue and joins behind the
 // other's stream. Page numbers and scales of a wave's next 64 pages are held one per lane. The four waves'
-// results join through LDS. One token of 16/4 heads behind 130,000: 48.5 us, 5.5 TB/s; of 64 sequences of 30 to 8,000
-// tokens (24/4): 50 us, 4.7 TB/s (a large copy: 4.9). Short ones are bound by the chain of loads: 6.7 us for one
+// results join through LDS. One token of 16/4 heads behind 130,000: 48.7 us, 5.5 TB/s; of 64 sequences of 30 to 8,000
+// tokens (24/4): 49.8 us, 4.7 TB/s (a large read: 6.4, a large copy: 4.9), where CUs have work for 0.64 of the time. Short ones are bound by the chain of loads: 6.7 us for one
 // token on 4,091.
 constexpr int kRowsThreads = 256, kRowsWaves = 4;
 template <int MT>
@@ -415,8 +415,11 @@ __global__ __launch_bounds__(kRowsThreads, MT == 1 ? 2 : 1) void kv8_attn_rows_k
 // The maximum of a row is common to its two waves, and no page's own maximum is looked for while weights stay small: a
 // wave whose sums of eight weights pass what the slack allows says so in a flag; behind the barrier all waves then
 // take the pairs' new maxima and make that page's P again (the first page, and hardly ever after).
-// Bound by conversions and products together: 4 x 512 tokens of 16/4 heads on 2,048 take 92 to 97 us, 800 to 840 TFLOP/s (a large f16
-// product: 1,209); a page takes 4,500 clocks of an item, of which the products alone are 2,050.
+// 4 x 512 tokens of 16/4 heads on 2,048 take 92 to 97 us, 800 to 840 TFLOP/s (a large f16 product: 1,209); a page takes 4,500
+// clocks of an item. No unit is full: of the time that a CU has work its matrix units are busy for 0.39 (2,050 clocks a page), other
+// vector instructions are issued for 0.27, LDS moves data for 0.35 (conflicts 0.003). What bounds it is the turn of the phases: with two
+// waves a SIMD and two barriers a page, all waves are in the same one, a wave stands at waits and barriers for 0.29 of
+// its time and behind the other's instructions for 0.38.
 constexpr int kTileThreads = 512;
 struct TileLds {
     u32x4 k[32][64], v[32][64];   // operand [2 (4 c + t) + h][lane]

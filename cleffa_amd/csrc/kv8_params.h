@@ -44,12 +44,13 @@ inline Layout layout(int n_seq, int T, int nh, int nkv, int max_new, int n_cu) {
     Layout l;
     const int G = nh / nkv;
     const long rows = (long)(max_new > 0 && max_new < T ? max_new : T) * G;
-    // Blocks of 16 rows for single tokens (64 sequences of 4,000 tokens, 6 rows: 99 us, with blocks of 128 167; 30 rows: 156,
-    // with blocks of 32 101). Of 32, rather than 128 that share the conversion of a page, for up to 64 rows a sequence (the same
-    // 64, 48 rows: 160 against 172) and for passes of up to 8,192 (row, head) pairs, whose blocks of 128 would leave
-    // CUs idle or each page to few of them: 270 rows 24/4 on 4,091 tokens 25.4 against 30.5, 8 x 192 rows on 2,000
-    // 30.9 against 38.1, 512 tokens 16/16 on 8,000 91.5 against 90.7; most is lost behind one very long text (1,536 rows on
-    // 30,000 tokens 248 against 219). Above: 64 x 96 rows on 4,000 183 against 168, 16 x 128 tokens 16/16 222 against 181.
+    // Blocks of 16 rows for single tokens (one of 24/4 heads on 4,091 9.7 us, with blocks of 32 13.2, of 128 22.5; 64 sequences of
+    // 4,000 tokens 99, 97, 159; at 30 rows of them 155, with blocks of 32 100). Of 32, rather than 128 that share the conversion
+    // of a page, for up to 64 rows a sequence (the same 64, 48 rows: 160 against 163) and for passes of up to 8,192
+    // (row, head) pairs, whose blocks of 128 would leave CUs idle or each page to few of them: 270 rows 24/4 on 4,091
+    // tokens 24.7 against 30.3, 8 x 192 rows on 2,000 30.5 against 37.5, 512 tokens 16/16 on 8,000 86.3 against 85.5; most is
+    // lost behind one very long text (1,536 rows on 30,000 tokens 251 against 211). Above: 64 x 96 rows on 4,000 175 against
+    // 164, 16 x 128 tokens 16/16 on 4,000 209 against 170.
     l.bm = rows <= 16 ? 16 : rows <= 64 || (long)T * nh <= 8192 ? 32 : 128;
     l.shape = G | nkv << 8 | l.bm << 20;   // what the lists go by beside n_seq and T
     l.budget = ((l.bm == 16 ? 2 : 1) * n_cu + nkv - 1) / nkv;   // items of one round of workgroups, two or one to a CU
