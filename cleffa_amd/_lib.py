@@ -18,6 +18,9 @@ KV_ALIGN = 8
 BLOCK_INTS = 8
 KV8_PAGE, KV8_MAX_SEQ, KV8_MAX_ROWS = 64, 4096, 262143
 KV8_PLAN_STATUS, KV8_PLAN_FAILED = 9, 10
+MX4_BLOCK, MX4_MAX = 32, 1 << 20
+ROTARY_SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
 
 # Every symbol include/clef_hip_attn.h declares.
 EXPORTS = (
@@ -35,6 +38,8 @@ EXPORTS = (
     "clef_hip_gguf_find_tensor", "clef_hip_gguf_get_u32", "clef_hip_gguf_get_f32", "clef_hip_gguf_attn_config",
     "clef_hip_gguf_attn_layer", "clef_hip_gguf_vis_layer",
     "clef_hip_kv8_sizes", "clef_hip_kv8_plan", "clef_hip_kv8_append", "clef_hip_kv8_attention", "clef_hip_kv8_read",
+    "clef_hip_mx4_sizes", "clef_hip_mx4_quantise", "clef_hip_mx4_values", "clef_hip_mx4_pack", "clef_hip_mx4_gemm",
+    "clef_hip_rotary_freqs", "clef_hip_rotary",
 )
 
 GGML_F32, GGML_F16, GGML_BF16 = 0, 1, 30
@@ -121,6 +126,32 @@ class Kv8ReadArgs(ctypes.Structure):
         ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
         ("tables", c_void_p), ("state", c_void_p), ("first_page", c_void_p), ("cu", c_void_p),
         ("k_plane", c_void_p), ("vt_plane", c_void_p),
+    ]
+
+
+class Mx4RowsArgs(ctypes.Structure):
+    _fields_ = [("rows", c_int), ("K", c_int), ("type", c_int), ("row", ctypes.c_long), ("x", c_void_p), ("codes", c_void_p), ("scales", c_void_p)]
+
+
+class Mx4GemmArgs(ctypes.Structure):
+    _fields_ = [
+        ("T", c_int), ("N", c_int), ("K", c_int), ("y_type", c_int),
+        ("w_codes", c_void_p), ("w_scales", c_void_p), ("x_codes", c_void_p), ("x_scales", c_void_p), ("x_bf16", c_void_p),
+        ("x_row", ctypes.c_long), ("y_row", ctypes.c_long), ("r_row", ctypes.c_long), ("y", c_void_p), ("residual", c_void_p),
+    ]
+
+
+class RotaryHeads(ctypes.Structure):
+    _fields_ = [
+        ("heads", c_int), ("x", c_void_p), ("out", c_void_p), ("x_row", ctypes.c_long), ("x_head", ctypes.c_long),
+        ("out_row", ctypes.c_long), ("out_head", ctypes.c_long), ("norm", c_void_p),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("T", c_int), ("hd", c_int), ("n_rot", c_int), ("layout", c_int), ("axes", c_int), ("type", c_int),
+        ("eps", c_float), ("magnitude", c_float), ("pos", c_void_p), ("freq", c_void_p), ("q", RotaryHeads), ("k", RotaryHeads),
     ]
 
 
@@ -211,6 +242,14 @@ def load():
     lib.clef_hip_kv8_sizes.restype = c_bool
     for name, args in (("plan", Kv8PlanArgs), ("append", Kv8Args), ("attention", Kv8Args), ("read", Kv8ReadArgs)):
         fn = getattr(lib, "clef_hip_kv8_" + name)
+        fn.argtypes = [POINTER(args), c_void_p, c_char_p, c_size_t]
+        fn.restype = c_bool
+    lib.clef_hip_mx4_sizes.argtypes = [c_int, c_int, POINTER(c_size_t), POINTER(c_size_t), c_char_p, c_size_t]
+    lib.clef_hip_mx4_pack.argtypes = [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_char_p, c_size_t]
+    lib.clef_hip_rotary_freqs.argtypes = [c_int, ctypes.c_double, c_int, *[ctypes.c_double] * 4, POINTER(ctypes.c_double), c_char_p, c_size_t]
+    lib.clef_hip_mx4_sizes.restype = lib.clef_hip_mx4_pack.restype = lib.clef_hip_rotary_freqs.restype = c_bool
+    for name, args in (("mx4_quantise", Mx4RowsArgs), ("mx4_values", Mx4RowsArgs), ("mx4_gemm", Mx4GemmArgs), ("rotary", RotaryArgs)):
+        fn = getattr(lib, "clef_hip_" + name)
         fn.argtypes = [POINTER(args), c_void_p, c_char_p, c_size_t]
         fn.restype = c_bool
     for name in ("clef_hip_attn_prep_kv", "clef_hip_attn_core", "clef_hip_attn_prefill"):

@@ -24,6 +24,7 @@ from ._lib import AttnArgs, VisArgs, OUT_BF16, OUT_F16, OUT_F32, BLOCK_INTS
 _OUT_TYPES = {"bf16": (OUT_BF16, torch.bfloat16), "f16": (OUT_F16, torch.float16),
               "f32": (OUT_F32, torch.float32)}
 _OUT_DTYPE = dict(_OUT_TYPES.values())
+_DTYPE_OUT = {t: o for o, t in _OUT_DTYPE.items()}
 
 
 def _i32p(a):
@@ -369,11 +370,19 @@ class TextAttention:
         """The QKV projection qkv = X . W^T (X [T][H] bf16, W [row][H] bf16, the attn_qkv weight as
         stored) through clef_hip_qkv_gemm. With prologue, its epilogue also writes the K / V^T
         planes (and rope_cs) as the "prep" stage would, so forward(stage="core") may follow on
-        the same planes and table. Returns qkv."""
+        the same planes and table. W may also be an mx4.Mx4Matrix, and X then one too: the product is
+        mx4_gemm's, and the "prep" stage runs behind it. Returns qkv."""
+        from .mx4 import Mx4Matrix, mx4_gemm
         dev = self.device
-        T, H = plan.T, X.shape[1] if X.dim() == 2 else -1
-        _check(X, "X", (T, H), torch.bfloat16, dev)
-        _check(W, "W", (self.row, H), torch.bfloat16, dev)
+        T = plan.T
+        four_bit = isinstance(W, Mx4Matrix)
+        if four_bit:
+            if W.rows != self.row or W.device != dev or (X.rows if isinstance(X, Mx4Matrix) else X.shape[0]) != T:
+                raise ValueError(f"X and W must have {T} and {self.row} rows, on {dev}")
+        else:
+            H = X.shape[1] if X.dim() == 2 else -1
+            _check(X, "X", (T, H), torch.bfloat16, dev)
+            _check(W, "W", (self.row, H), torch.bfloat16, dev)
         if qkv is None:
             qkv = torch.empty((T, self.row), dtype=torch.bfloat16, device=dev)
         _check(qkv, "qkv", (T, self.row), torch.bfloat16, dev)
@@ -389,6 +398,11 @@ class TextAttention:
             a = AttnArgs()
             a.nh, a.nkv, a.hd, a.n_rot, a.T, a.row = self.nh, self.nkv, self.hd, self.n_rot, T, self.row
             a.qkv, a.qkv_type = _ptr(qkv), _lib.QKV_BF16
+        if four_bit:
+            mx4_gemm(X, W, Y=qkv, stream=stream)
+            if prologue:
+                _launch(_lib.load().clef_hip_attn_prep_kv, a, dev, stream)
+            return qkv
         err = _err()
         _lib.check(_lib.load().clef_hip_qkv_gemm(H, X.data_ptr(), W.data_ptr(), ctypes.byref(a),
                                                  _ptr(plan.tok_kv) if prologue else None,

@@ -1,0 +1,97 @@
+// Y = X . W^T (+ residual) with W in microscaled 4 bits and X in the same or in bf16.
+#pragma once
+#include <utility>
+
+#include "mx4_params.h"
+
+namespace clef_hip {
+namespace mx4 {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+
+__device__ __forceinline__ i32x8 operand(u32x4 c) { return i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0}; }
+// 16 x 16 outputs, 128 deep: A = 16 rows of W (columns of Y), B = 16 rows of X. Lane l's accumulators are columns
+// 4 (l / 16) .. + 3 of row l % 16. The scales are the low bytes of sw and sx.
+__device__ __forceinline__ f32x4 mfma4(u32x4 w, u32x4 x, f32x4 acc, int sw, int sx) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(x), acc, 4, 4, 0, sw, 0, sx);
+}
+// Eight codes as bf16, exactly (but for magnitudes beyond bf16).
+__device__ __forceinline__ bf16x8 widen(unsigned c, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+
+// MT x NT tiles of 16 rows and 16 columns a workgroup, whose W waves share the K tiles and add their sums in LDS in a
+// fixed order. Operands come straight from memory. BF: X is bf16.
+template <bool BF, int MT, int NT, int W>
+__global__ __launch_bounds__(64 * W) void mx4_rows_kernel(GemmParams p) {
+    __shared__ f32x4 part[W > 1 ? W : 1][MT * NT][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int n_tiles = ceil_div(p.N, 16), t_tiles = ceil_div(p.T, 16);
+    const int nb = ceil_div(n_tiles, NT);
+    const int n0 = (blockIdx.x % nb) * NT, t0 = (blockIdx.x / nb) * MT;
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int k_lo = (int)((long)p.w.ktiles * wave / W), k_hi = (int)((long)p.w.ktiles * (wave + 1) / W);
+    for (int kt = k_lo; kt < k_hi; kt++) {
+        const int sh = 8 * (kt & 3);
+        u32x4 wc[NT];
+        int ws[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int nt = min(n0 + j, n_tiles - 1);
+            wc[j] = *(const u32x4 *)(p.w.tile(nt, kt) + 16 * lane);
+            ws[j] = *(const int *)(p.w.group(nt, kt >> 2) + 4 * lane) >> sh;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int tt = min(t0 + i, t_tiles - 1);
+            if constexpr (BF) {
+                const int t = min(16 * tt + l16, p.T - 1), k = KT * kt + 32 * g;
+                const uint16_t *x = p.xb + (size_t)t * p.x_row + k;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bf16x8 b = k < p.K ? *(const bf16x8 *)(x + 8 * j) : bf16x8{};
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(wc[n][j], __uint_as_float((unsigned)(ws[n] & 255) << 23)), b, acc[i][n], 0, 0, 0);
+                }
+            } else {
+                const u32x4 xc = *(const u32x4 *)(p.x.tile(tt, kt) + 16 * lane);
+                const int xs = *(const int *)(p.x.group(tt, kt >> 2) + 4 * lane) >> sh;
+#pragma unroll
+                for (int n = 0; n < NT; n++) acc[i][n] = mfma4(wc[n], xc, acc[i][n], ws[n], xs);
+            }
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) part[wave][i * NT + j][lane] = acc[i][j];
+        __syncthreads();
+        for (int u = wave; u < MT * NT; u += W) {
+            f32x4 s = part[0][u][lane];
+#pragma unroll
+            for (int w = 1; w < W; w++) s += part[w][u][lane];
+            const int t = 16 * (t0 + u / NT) + l16, c = 16 * (n0 + u % NT) + 4 * g;
+            if (t < p.T && c < p.N) store4(p, t, c, s[0], s[1], s[2], s[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int t = 16 * (t0 + i) + l16, c = 16 * (n0 + j) + 4 * g;
+                if (t < p.T && c < p.N) store4(p, t, c, acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+            }
+    }
+}
+
+}  // namespace mx4
+}  // namespace clef_hip

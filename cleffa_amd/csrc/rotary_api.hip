@@ -1,0 +1,150 @@
+// C ABI of the rotary operator: frequency tables, argument checks and launches. Documented in include/clef_hip_attn.h.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "clef_hip_attn.h"
+#include "rotary.h"
+
+using namespace clef_hip;
+
+namespace {
+
+bool fail(char *err, size_t errlen, const char *fmt, ...) {
+    if (err && errlen) {
+        int n = snprintf(err, errlen, "hip: ");
+        if (n < 0) n = 0;
+        if ((size_t)n < errlen) {
+            va_list ap;
+            va_start(ap, fmt);
+            vsnprintf(err + n, errlen - (size_t)n, fmt, ap);
+            va_end(ap);
+        }
+    }
+    return false;
+}
+
+bool group_ok(const char *what, const clef_hip_rotary_heads *g, int T, int hd, int size, char *err, size_t errlen) {
+    if (g->heads < 0 || g->heads > 4096) return fail(err, errlen, "rotary: %d %s heads", g->heads, what);
+    if (g->heads == 0 || T == 0) return true;
+    const uintptr_t a = (uintptr_t)(size - 1);
+    if (!g->x || !g->out || ((uintptr_t)g->x & a) || ((uintptr_t)g->out & a) || ((uintptr_t)g->norm & 3u))
+        return fail(err, errlen, "rotary: %s, its output and norm must be aligned device pointers", what);
+    if ((T > 1 && (g->x_row < 0 || g->out_row < 0)) || (g->heads > 1 && (g->x_head < 0 || g->out_head < 0)))
+        return fail(err, errlen, "rotary: negative %s strides", what);
+    // rows of heads, or heads of rows
+    const long row = T > 1 ? g->out_row : LONG_MAX, head = g->heads > 1 ? g->out_head : LONG_MAX;
+    const bool by_row = head >= hd && (T == 1 || row >= (g->heads - 1) * g->out_head + hd);
+    const bool by_head = row >= hd && (g->heads == 1 || head >= (T - 1) * g->out_row + hd);
+    if (!by_row && !by_head) return fail(err, errlen, "rotary: heads or rows of the %s output overlap", what);
+    if (g->x == g->out && ((T > 1 && g->x_row != g->out_row) || (g->heads > 1 && g->x_head != g->out_head)))
+        return fail(err, errlen, "rotary: %s in place needs the same strides", what);
+    return true;
+}
+
+// whether all of a group's runs of v values of `size` bytes start at multiples of their size
+bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size) {
+    if (g->heads == 0) return true;
+    const uintptr_t a = (uintptr_t)(v * size - 1);
+    if (((uintptr_t)g->x & a) || ((uintptr_t)g->out & a)) return false;
+    if (g->heads > 1 && (g->x_head % v || g->out_head % v)) return false;
+    return T <= 1 || (g->x_row % v == 0 && g->out_row % v == 0);
+}
+
+rotary::Group group(const clef_hip_rotary_heads *g) {
+    return rotary::Group{g->x, g->out, g->norm, g->x_row, g->x_head, g->out_row, g->out_head, g->heads};
+}
+
+template <int TYPE, int V, int L, int I>
+void launch(rotary::Params &p, hipStream_t s) {
+    constexpr int TOK = 1;
+    p.q_units = (p.q.heads + 64 / L - 1) / (64 / L);
+    p.units = p.q_units + (p.k.heads + 64 / L - 1) / (64 / L);
+    hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, TOK>), dim3((unsigned)((p.T + TOK - 1) / TOK)), dim3(rotary::kThreads), 0, s, p);
+}
+// L: the least power of two of lanes that holds a head in pairs of runs of V
+template <int TYPE, int V>
+void launch_runs(rotary::Params &p, hipStream_t s) {
+    const int pairs = (p.hd + 2 * V - 1) / (2 * V);
+    if (pairs <= 4) launch<TYPE, V, 4, 1>(p, s);
+    else if (pairs <= 8) launch<TYPE, V, 8, 1>(p, s);
+    else if (pairs <= 16) launch<TYPE, V, 16, 1>(p, s);
+    else if constexpr (V <= 4) {
+        if (pairs <= 32) launch<TYPE, V, 32, 1>(p, s);
+        else if constexpr (V <= 2) {
+            if (pairs <= 64) launch<TYPE, V, 64, 1>(p, s);
+            else launch<TYPE, V, 64, 2>(p, s);
+        }
+    }
+}
+template <int TYPE>
+void launch_type(rotary::Params &p, int v, hipStream_t s) {
+    if constexpr (TYPE != CLEF_HIP_OUT_F32) {
+        if (v == 8) return launch_runs<TYPE, 8>(p, s);
+    }
+    if (v == 4) launch_runs<TYPE, 4>(p, s);
+    else if (v == 2) launch_runs<TYPE, 2>(p, s);
+    else launch_runs<TYPE, 1>(p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+bool clef_hip_rotary_freqs(int n_rot, double theta, int scaling, double factor, double original, double low, double high, double *freq,
+                           char *err, size_t errlen) {
+    if (n_rot <= 0 || n_rot % 2 || n_rot > rotary::kMaxHd) return fail(err, errlen, "rotary: n_rot %d must be even, 2 to %d", n_rot, rotary::kMaxHd);
+    if (!(theta > 1.) || !isfinite(theta)) return fail(err, errlen, "rotary: bad theta");
+    if (scaling < CLEF_HIP_ROTARY_NONE || scaling > CLEF_HIP_ROTARY_PARTS) return fail(err, errlen, "rotary: bad scaling %d", scaling);
+    if (scaling != CLEF_HIP_ROTARY_NONE && (!(factor >= 1.) || !isfinite(factor))) return fail(err, errlen, "rotary: the scaling factor must be at least 1");
+    if (scaling == CLEF_HIP_ROTARY_BASE && n_rot == 2) return fail(err, errlen, "rotary: a changed base needs more than one pair");
+    if (scaling == CLEF_HIP_ROTARY_PARTS && (!(original > 0.) || !isfinite(original) || !(low >= 0.) || !(high > low) || !isfinite(high)))
+        return fail(err, errlen, "rotary: scaling by parts needs an original length and 0 <= low < high");
+    if (!freq) return fail(err, errlen, "rotary: missing freq");
+    const double tau = 6.283185307179586476925;
+    const double base = scaling == CLEF_HIP_ROTARY_BASE ? theta * pow(factor, (double)n_rot / (n_rot - 2)) : theta;
+    for (int j = 0; j < n_rot / 2; j++) {
+        double f = pow(base, -2. * j / n_rot);
+        if (scaling == CLEF_HIP_ROTARY_LINEAR) f /= factor;
+        if (scaling == CLEF_HIP_ROTARY_PARTS) {
+            const double keep = fmin(1., fmax(0., (original * f / tau - low) / (high - low)));
+            f = keep * f + (1. - keep) * f / factor;
+        }
+        freq[j] = f / tau;
+    }
+    return true;
+}
+
+bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, size_t errlen) {
+    if (!a) return fail(err, errlen, "null rotary arguments");
+    if (a->T < 0) return fail(err, errlen, "rotary: %d rows", a->T);
+    if (a->hd <= 0 || a->hd > rotary::kMaxHd || a->hd % 2) return fail(err, errlen, "rotary: head dim %d must be even, 2 to %d", a->hd, rotary::kMaxHd);
+    if (a->n_rot <= 0 || a->n_rot % 2 || a->n_rot > a->hd) return fail(err, errlen, "rotary: n_rot %d must be even, 2 to the head dim", a->n_rot);
+    if (a->layout != CLEF_HIP_ROTARY_HALF && a->layout != CLEF_HIP_ROTARY_INTERLEAVED) return fail(err, errlen, "rotary: bad layout %d", a->layout);
+    if (a->axes < 1 || a->axes > 4) return fail(err, errlen, "rotary: %d position axes, 1 to 4 are supported", a->axes);
+    if (a->type < CLEF_HIP_OUT_BF16 || a->type > CLEF_HIP_OUT_F32) return fail(err, errlen, "rotary: bad type %d", a->type);
+    if (!(a->eps >= 0.f) || !isfinite(a->magnitude)) return fail(err, errlen, "rotary: bad eps or magnitude");
+    const int size = a->type == CLEF_HIP_OUT_F32 ? 4 : 2;
+    if (!group_ok("q", &a->q, a->T, a->hd, size, err, errlen) || !group_ok("k", &a->k, a->T, a->hd, size, err, errlen)) return false;
+    if (a->T == 0 || a->q.heads + a->k.heads == 0) return true;
+    if (!a->pos || !a->freq || ((uintptr_t)a->pos & 3u) || ((uintptr_t)a->freq & 7u)) return fail(err, errlen, "rotary: pos and freq must be aligned device pointers");
+    rotary::Params p;
+    p.q = group(&a->q); p.k = group(&a->k); p.pos = a->pos; p.freq = a->freq;
+    p.T = a->T; p.hd = a->hd; p.n_rot = a->n_rot; p.half = a->layout == CLEF_HIP_ROTARY_HALF; p.axes = a->axes;
+    p.eps = a->eps; p.magnitude = a->magnitude;
+    // the longest runs that heads divide into and that pointers and strides allow
+    int v = 16 / size;
+    while (v > 1 && (a->hd % v || (p.half && (a->n_rot / 2) % v) || !runs_ok(&a->q, a->T, v, size) || !runs_ok(&a->k, a->T, v, size))) v /= 2;
+    const hipStream_t s = (hipStream_t)stream;
+    if (a->type == CLEF_HIP_OUT_BF16) launch_type<CLEF_HIP_OUT_BF16>(p, v, s);
+    else if (a->type == CLEF_HIP_OUT_F16) launch_type<CLEF_HIP_OUT_F16>(p, v, s);
+    else launch_type<CLEF_HIP_OUT_F32>(p, v, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(err, errlen, "rotary launch failed: %s", hipGetErrorString(e));
+    return true;
+}
+
+}  // extern "C"

@@ -1,0 +1,104 @@
+"""Rotary positions of q and k heads, RMSNorm ahead of them where the model has one, as an operator of its own: the
+prologues inside the attention turn 64 dims in the half layout; this one turns any even part of the head, in both
+layouts, with frequencies scaled for long texts, in the rows of a projection or out of them.
+
+    rotary = Rotary(n_rot=128, theta=1e7, layout="interleaved", scaling={"kind": "parts", "factor": 8, "original": 16384})
+    q, k = rotary.heads(qkv, nh, nkv, hd)             # views of the projection's rows
+    rotary.apply(q, k, pos, q_norm, k_norm, q_out=q, k_out=k)
+    out = TextAttention(nh, nkv, n_rot=0).forward(qkv, None, None, pos3, plan)
+
+Formulas: include/clef_hip_attn.h.
+"""
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+from .attention import _DTYPE_OUT, _arg, _device, _launch, _err, init_device
+
+
+class Rotary:
+    """Frequencies and layout of a model's rotary positions. layout "half" (dims j and j + n_rot / 2 turn together) or
+    "interleaved" (2j and 2j + 1). axes: int32 positions a row; pair j goes by position j % axes. scaling: None, or
+    a dict of "kind" ("linear", "base" or "parts"), "factor" and for "parts" "original" (the length that the model was
+    trained for), "low" and "high" (1 and 32: pairs that turn less over it are stretched, that turn more are kept). magnitude
+    multiplies all turned dims (None: 0.1 ln factor + 1 for "parts", else 1). freqs: radians a position of each pair,
+    float64 [n_rot / 2], in place of the formula."""
+
+    def __init__(self, n_rot, theta=1e7, layout="half", axes=1, scaling=None, magnitude=None, freqs=None, eps=1e-6, device="cuda"):
+        if layout not in _lib.ROTARY_LAYOUTS:
+            raise ValueError(f"layout {layout!r}: half or interleaved")
+        if not 1 <= axes <= 4:
+            raise ValueError(f"{axes} position axes: 1 to 4 are supported")
+        s = {"kind": None, "factor": 1.0, "original": 0.0, "low": 1.0, "high": 32.0}
+        unknown = set(scaling or {}) - set(s)
+        s.update(scaling or {})
+        if unknown or s["kind"] not in _lib.ROTARY_SCALINGS or (scaling and s["kind"] is None):
+            raise ValueError(f"scaling {scaling!r}: kind linear, base or parts, factor, original, low, high")
+        table, err = np.zeros(max(n_rot // 2, 1)), _err()
+        _lib.check(_lib.load().clef_hip_rotary_freqs(n_rot, theta, _lib.ROTARY_SCALINGS[s["kind"]], s["factor"], s["original"], s["low"], s["high"],
+                                                     table.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), err, len(err)), err)
+        if freqs is not None:
+            freqs = np.asarray(freqs, dtype=np.float64)
+            if scaling is not None or freqs.shape != table.shape or not np.isfinite(freqs).all():
+                raise ValueError(f"freqs takes the place of a scaling: {n_rot // 2} finite values")
+            table = freqs / (2 * math.pi)
+        if magnitude is None:
+            magnitude = 0.1 * math.log(s["factor"]) + 1 if s["kind"] == "parts" else 1.0
+        if not math.isfinite(magnitude):
+            raise ValueError(f"magnitude {magnitude}")
+        self.n_rot, self.layout, self.axes, self.eps, self.magnitude = int(n_rot), layout, int(axes), eps, float(magnitude)
+        self.device = _device(device)
+        if self.device.type == "cuda":
+            init_device(self.device)
+        self.freq = torch.from_numpy(table).to(self.device)     # turns a position
+
+    @staticmethod
+    def heads(qkv, nh, nkv, hd, gated=True):
+        """The q and k heads [T][heads][hd] of projection rows, [query | gate] of each q head where the model gates, then
+        the k heads, then the v heads, as views."""
+        wide = 2 if gated else 1
+        if qkv.dim() != 2 or qkv.shape[1] < (wide * nh + 2 * nkv) * hd:
+            raise ValueError(f"rows {tuple(qkv.shape)} do not hold {nh} / {nkv} heads of {hd}")
+        q = qkv[:, :wide * nh * hd].unflatten(1, (nh, wide * hd))[:, :, :hd]
+        return q, qkv[:, wide * nh * hd:(wide * nh + nkv) * hd].unflatten(1, (nkv, hd))
+
+    def _heads(self, x, out, norm, name, T, hd, dtype):
+        if x is None:
+            if out is not None or norm is not None:
+                raise ValueError(f"{name}: an output or norm without heads")
+            return _lib.RotaryHeads(0, None, None, 0, 0, 0, 0, None)
+        for t, what in ((x, name), (out, name + "_out")):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{what} must be a torch tensor")
+            if t.dim() != 3 or t.shape[0] != T or t.shape[2] != hd or t.shape[1] != x.shape[1]:
+                raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {(T, x.shape[1], hd)}")
+            if t.dtype is not dtype:
+                raise TypeError(f"{what} has dtype {t.dtype}, expected {dtype}")
+            if t.device != self.device:
+                raise ValueError(f"{what} is on {t.device}, expected {self.device}")
+            if t.stride(2) != 1 and t.numel():
+                raise ValueError(f"the dims of a head of {what} must be contiguous")
+        norm = None if norm is None else _arg(norm, name + "_norm", (hd,), torch.float32, self.device)
+        return _lib.RotaryHeads(x.shape[1], x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1), norm)
+
+    def apply(self, q, k, pos, q_norm=None, k_norm=None, q_out=None, k_out=None, stream=None):
+        """q [T][nh][hd] and k [T][nkv][hd] (or None), bf16, f16 or f32, turned by pos (int32 [T] or [T][axes]), each after its
+        RMSNorm where a weight [hd] f32 is given. Rows and heads may lie apart (views of a projection's rows). q_out and
+        k_out: new tensors where they are None; q and k themselves for a rotation in place. Returns (q_out, k_out)."""
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPE_OUT:
+            raise TypeError("q must be a bf16, f16 or f32 tensor [T][heads][hd]")
+        T, _, hd = q.shape
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None and k is not None else k_out
+        if not isinstance(pos, torch.Tensor) or pos.dtype is not torch.int32 or pos.device != self.device or not pos.is_contiguous():
+            raise ValueError("pos must be contiguous int32 on the operator's device")
+        if tuple(pos.shape) not in (((T,), (T, 1)) if self.axes == 1 else ((T, self.axes),)):
+            raise ValueError(f"pos has shape {tuple(pos.shape)}, expected {(T, self.axes)}")
+        a = _lib.RotaryArgs(T, hd, self.n_rot, _lib.ROTARY_LAYOUTS[self.layout], self.axes, _DTYPE_OUT[q.dtype], self.eps, self.magnitude,
+                            pos.data_ptr(), self.freq.data_ptr(), self._heads(q, q_out, q_norm, "q", T, hd, q.dtype),
+                            self._heads(k, k_out, k_norm, "k", T, hd, q.dtype))
+        _launch(_lib.load().clef_hip_rotary, a, self.device, stream)
+        return q_out, k_out

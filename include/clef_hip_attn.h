@@ -500,6 +500,90 @@ typedef struct {
 } clef_hip_kv8_read_args;
 bool clef_hip_kv8_read(const clef_hip_kv8_read_args *a, void *stream, char *err, size_t errlen);
 
+/* ---- Microscaled 4-bit matrices, for the projections either side of the path. No reference counterpart: the reference's
+ * projections run on 16-bit weights (clef_metal.m:463-499). OCP microscaling format: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives) with one e8m0 scale 2^(s - 127) for each CLEF_HIP_MX4_BLOCK values along a row; s = 255: the
+ * block is NaN. A matrix [rows][K] lies in memory as two buffers in the order of the matrix instructions:
+ *   codes  [ceil(rows / 16)][ceil(K / 128)][4][16][16] bytes: row tile, K tile, block of 32 in the tile, row in the tile, 32
+ *          codes (the first in the lower four bits of a byte);
+ *   scales [ceil(rows / 16)][ceil(K / 512)][4][16][4] bytes: row tile, K group, block in the K tile, row, K tile in the group.
+ * Codes and scales beyond K are 0; rows of the last row tile beyond the matrix are neither written nor used. The first n
+ * rows of a matrix (n a multiple of 16, or all) are a matrix of n rows in the same buffers. Buffers are 16-byte aligned. */
+#define CLEF_HIP_MX4_BLOCK 32
+#define CLEF_HIP_MX4_MAX 1048576   /* rows, and values of a row */
+/* The bytes of both buffers; K a multiple of 32. Either output may be NULL. */
+bool clef_hip_mx4_sizes(int rows, int K, size_t *code_bytes, size_t *scale_bytes, char *err, size_t errlen);
+
+/* quantise: x [rows][row] into codes and scales. A block's scale is 2^e, e the least integer from -127 on with max|x| <
+ * 7 * 2^e (so that the largest rounds to at most 6), at most 125; a value becomes the nearest code, ties to the one with an even fraction.
+ * A block with an infinity or a NaN becomes NaN. values: the reverse, exact in bf16 and f32 (the same fields; x is
+ * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity). */
+typedef struct {
+    int rows, K, type;        /* type: CLEF_HIP_OUT_* of x */
+    long row;                 /* row stride of x in elements, a multiple of 8 */
+    void *x;
+    uint8_t *codes, *scales;
+} clef_hip_mx4_rows_args;
+bool clef_hip_mx4_quantise(const clef_hip_mx4_rows_args *a, void *stream, char *err, size_t errlen);
+bool clef_hip_mx4_values(const clef_hip_mx4_rows_args *a, void *stream, char *err, size_t errlen);
+/* Codes and scales as files store them, flat_codes [rows][K / 2] (16-byte aligned) and flat_scales [rows][K / 32], into a
+ * matrix's buffers, or (to_flat) back. All on the device. */
+bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scales, uint8_t *codes, uint8_t *scales, int to_flat,
+                       void *stream, char *err, size_t errlen);
+
+/* Y[T][N] = X[T][K] . W[N][K]^T (+ residual), W in 4 bits, X in 4 bits (x_codes, x_scales) or in bf16 (x_bf16, its rows x_row
+ * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly, and summed
+ * in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
+ * be Y itself. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W. The sums' order
+ * depends on the sizes alone: results do not change from run to run. No workspace. */
+typedef struct {
+    int T, N, K, y_type;
+    const uint8_t *w_codes, *w_scales;   /* [N][K] */
+    const uint8_t *x_codes, *x_scales;   /* [T][K], or both NULL */
+    const uint16_t *x_bf16;              /* [T][x_row] bf16, x_row a multiple of 8, or NULL */
+    long x_row, y_row, r_row;
+    void *y;
+    const float *residual;
+} clef_hip_mx4_gemm_args;
+bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err, size_t errlen);
+
+/* ---- Rotary positions of q and k heads as an operator of its own, RMSNorm ahead of it where the model has one: for layouts,
+ * rotated parts and frequency scalings other than those of the prologues above (which then run with n_rot 0 and no norms),
+ * and for rows whose product has no prologue in its epilogue.
+ *
+ * Pair j < n_rot / 2 of a head, dims (j, j + n_rot / 2) in the half layout (the prologues') or (2j, 2j + 1) in the interleaved one,
+ * turns by a = pos[t][j % axes] * f_j: (x, y) -> magnitude * (x cos a - y sin a, y cos a + x sin a). Dims from n_rot on are
+ * normalised alone. Angles are reduced in f64, so that far positions keep theirs; norm and rotation run in f32, rounded once.
+ * Negated positions turn back.
+ *
+ * clef_hip_rotary_freqs (host only): freq[j] = f_j / 2 pi, turns a position, in f64. f_j = theta^(-2j / n_rot); scaled for texts
+ * `factor` times as long: LINEAR f_j / factor; BASE theta * factor^(n_rot / (n_rot - 2)) for theta; PARTS keep f_j + (1 - keep) f_j /
+ * factor, keep = (r - low) / (high - low) within 0 and 1, r = original * f_j / 2 pi the turns over the original length. */
+#define CLEF_HIP_ROTARY_NONE 0
+#define CLEF_HIP_ROTARY_LINEAR 1
+#define CLEF_HIP_ROTARY_BASE 2
+#define CLEF_HIP_ROTARY_PARTS 3
+#define CLEF_HIP_ROTARY_HALF 0
+#define CLEF_HIP_ROTARY_INTERLEAVED 1
+bool clef_hip_rotary_freqs(int n_rot, double theta, int scaling, double factor, double original, double low, double high, double *freq,
+                           char *err, size_t errlen);
+typedef struct {
+    int heads;                /* 0: none */
+    const void *x;            /* head h of row t starts at x + t * x_row + h * x_head elements */
+    void *out;                /* may be x with the same strides; without a norm only the turned dims are then touched */
+    long x_row, x_head, out_row, out_head;
+    const float *norm;        /* [hd] f32, as given (already 1 + w), or NULL */
+} clef_hip_rotary_heads;
+typedef struct {
+    int T, hd, n_rot;         /* hd and n_rot even, n_rot <= hd <= 256 */
+    int layout, axes, type;   /* CLEF_HIP_ROTARY_HALF or _INTERLEAVED; 1 to 4; CLEF_HIP_OUT_* of all heads */
+    float eps, magnitude;
+    const int32_t *pos;       /* [T][axes] */
+    const double *freq;       /* [n_rot / 2], device */
+    clef_hip_rotary_heads q, k;
+} clef_hip_rotary_args;
+bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, size_t errlen);
+
 /* Host-only producers of the path's inputs. */
 
 /* M-RoPE positions pos3 [T][3] of one record (clef_record.c:938-962, clef_record_positions).
