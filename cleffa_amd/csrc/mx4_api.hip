@@ -8,6 +8,8 @@
 #include "mx4_gemm.h"
 #include "mx4_params.h"
 #include "mx4_quant.h"
+#include "mx4_tile.h"
+#include "mx4_wide.h"
 
 using namespace clef_hip;
 
@@ -60,6 +62,19 @@ void launch_rows(const mx4::GemmParams &p, hipStream_t s) {
     const unsigned grid = (unsigned)((long)mx4::ceil_div(mx4::ceil_div(p.N, 16), NT) * mx4::ceil_div(mx4::ceil_div(p.T, 16), MT));
     if (p.xb) hipLaunchKernelGGL((mx4::mx4_rows_kernel<true, MT, NT, W>), dim3(grid), dim3(64 * W), 0, s, p);
     else hipLaunchKernelGGL((mx4::mx4_rows_kernel<false, MT, NT, W>), dim3(grid), dim3(64 * W), 0, s, p);
+}
+
+template <typename C>
+dim3 tile_grid(const mx4::GemmParams &p) {
+    return dim3((unsigned)(8 * mx4::ceil_div(mx4::ceil_div(p.N, C::BN), 8) * mx4::ceil_div(p.T, C::BM)));
+}
+template <typename C>
+void launch_tile(const mx4::GemmParams &p, hipStream_t s) {
+    hipLaunchKernelGGL(mx4::mx4_tile_kernel<C>, tile_grid<C>(p), dim3(C::THREADS), 0, s, p);
+}
+template <typename C>
+void launch_wide(const mx4::GemmParams &p, hipStream_t s) {
+    hipLaunchKernelGGL(mx4::mx4_wide_kernel<C>, tile_grid<C>(p), dim3(C::THREADS), 0, s, p);
 }
 
 }  // namespace
@@ -140,11 +155,14 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     p.x = matrix(a->x_codes, a->x_scales, a->T, a->K);
     p.xb = a->x_bf16; p.x_row = a->x_row; p.y = a->y; p.y_row = a->y_row; p.residual = a->residual; p.r_row = a->r_row;
     p.T = a->T; p.N = a->N; p.K = a->K; p.y_bf16 = a->y_type == CLEF_HIP_GEMM_Y_BF16;
-    p.vec = aligned16(a->y) && a->y_row % 4 == 0 && (!a->residual || (aligned16(a->residual) && a->r_row % 4 == 0));
+    p.vec = aligned16(a->y) && a->y_row % (p.y_bf16 ? 8 : 4) == 0 && (!a->residual || (aligned16(a->residual) && a->r_row % 4 == 0));
     const hipStream_t s = (hipStream_t)stream;
     if (a->T <= 16) launch_rows<1, 1, 8>(p, s);
     else if (a->T <= 32) launch_rows<2, 2, 8>(p, s);
-    else launch_rows<4, 4, 4>(p, s);
+    else if (p.T < 256) launch_rows<4, 4, 4>(p, s);
+    else if (p.xb) launch_wide<mx4::WideCfg<128, 256, 64, 128, 3, 1>>(p, s);
+    else if ((long)mx4::ceil_div(p.T, 256) * mx4::ceil_div(p.N, 128) < 400) launch_tile<mx4::TileCfg<128, 128, 64, 64, 4, 2>>(p, s);
+    else launch_tile<mx4::TileCfg<256, 128, 128, 64, 3, 2>>(p, s);
     return launch_ok("mx4_gemm", err, errlen);
 }
 

@@ -61,23 +61,24 @@ struct GemmParams {
     int vec;                  // y (and the residual) allow stores of four columns at a time
 };
 
-// Four consecutive columns of a row, n of them inside the matrix: residual, rounding, store.
-__device__ __forceinline__ void store4(const GemmParams &p, int t, int c, float v0, float v1, float v2, float v3) {
-    float v[4] = {v0, v1, v2, v3};
-    const int n = p.N - c;
-    if (p.vec && n >= 4) {
-        if (p.y_bf16) {
-            *(u32x2 *)((uint16_t *)p.y + (size_t)t * p.y_row + c) = u32x2{pack_bf16(v0, v1), pack_bf16(v2, v3)};
-            return;
-        }
-        float4 o = {v0, v1, v2, v3};
-        if (p.residual) {
-            const float4 r = *(const float4 *)(p.residual + (size_t)t * p.r_row + c);
-            o = {v0 + r.x, v1 + r.y, v2 + r.z, v3 + r.w};
-        }
-        *(float4 *)((float *)p.y + (size_t)t * p.y_row + c) = o;
+// Four consecutive columns of a row, all inside the matrix, at addresses that allow it: residual, rounding, store.
+__device__ __forceinline__ void store4_whole(const GemmParams &p, int t, int c, float v0, float v1, float v2, float v3) {
+    if (p.y_bf16) {
+        *(u32x2 *)((uint16_t *)p.y + (size_t)t * p.y_row + c) = u32x2{pack_bf16(v0, v1), pack_bf16(v2, v3)};
         return;
     }
+    float4 o = {v0, v1, v2, v3};
+    if (p.residual) {
+        const float4 r = *(const float4 *)(p.residual + (size_t)t * p.r_row + c);
+        o = {v0 + r.x, v1 + r.y, v2 + r.z, v3 + r.w};
+    }
+    *(float4 *)((float *)p.y + (size_t)t * p.y_row + c) = o;
+}
+// Anywhere, c inside the matrix.
+__device__ __forceinline__ void store4(const GemmParams &p, int t, int c, float v0, float v1, float v2, float v3) {
+    const int n = p.N - c;
+    if (p.vec && n >= 4) return store4_whole(p, t, c, v0, v1, v2, v3);
+    const float v[4] = {v0, v1, v2, v3};
     for (int i = 0; i < 4 && i < n; i++) {
         if (p.y_bf16) ((uint16_t *)p.y)[(size_t)t * p.y_row + c + i] = f2bf(v[i]);
         else ((float *)p.y)[(size_t)t * p.y_row + c + i] = v[i] + (p.residual ? p.residual[(size_t)t * p.r_row + c + i] : 0.f);
