@@ -58,12 +58,17 @@ rotary::Group group(const clef_hip_rotary_heads *g) {
     return rotary::Group{g->x, g->out, g->norm, g->x_row, g->x_head, g->out_row, g->out_head, g->heads};
 }
 
+template <int TYPE, int V, int L, int I, bool HALF>
+void launch_tokens(const rotary::Params &p, hipStream_t s) {
+    if (p.T <= 512) hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, 1, HALF>), dim3((unsigned)p.T), dim3(rotary::kThreads), 0, s, p);
+    else hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, 4, HALF>), dim3((unsigned)((p.T + 3) / 4)), dim3(rotary::kThreads), 0, s, p);
+}
 template <int TYPE, int V, int L, int I>
 void launch(rotary::Params &p, hipStream_t s) {
-    constexpr int TOK = 1;
     p.q_units = (p.q.heads + 64 / L - 1) / (64 / L);
     p.units = p.q_units + (p.k.heads + 64 / L - 1) / (64 / L);
-    hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, TOK>), dim3((unsigned)((p.T + TOK - 1) / TOK)), dim3(rotary::kThreads), 0, s, p);
+    if (p.half) launch_tokens<TYPE, V, L, I, true>(p, s);
+    else launch_tokens<TYPE, V, L, I, false>(p, s);
 }
 // L: the least power of two of lanes that holds a head in pairs of runs of V
 template <int TYPE, int V>
