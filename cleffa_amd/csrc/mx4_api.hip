@@ -8,6 +8,7 @@
 #include "mx4_gemm.h"
 #include "mx4_params.h"
 #include "mx4_quant.h"
+#include "mx4_rows16.h"
 #include "mx4_tile.h"
 #include "mx4_wide.h"
 
@@ -37,6 +38,9 @@ bool launch_ok(const char *what, char *err, size_t errlen) {
     return true;
 }
 
+// The compute units of the chips this library is built for (gfx950): forms are chosen for them.
+constexpr int kCus = 256;
+
 // rows * K / 512 workgroups and rows * K / 8192 of them: both below 2^31
 bool shape_ok(const char *what, int rows, int K, char *err, size_t errlen) {
     if (rows < 0 || rows > CLEF_HIP_MX4_MAX) return fail(err, errlen, "%s: %d rows, 0 to %d are supported", what, rows, CLEF_HIP_MX4_MAX);
@@ -57,16 +61,45 @@ mx4::Matrix matrix(const uint8_t *codes, const uint8_t *scales, int rows, int K)
     return mx4::Matrix{codes, scales, rows, mx4::ceil_div(K, mx4::KT), mx4::ceil_div(K, mx4::KG)};
 }
 
+// The forms of the product. Where a form's workgroups make no more than one for each CU, its K loop is the time, and the smallest
+// tile wins; else the rounds of workgroups count. Measured in us (three weights in turn, K 6,144 at N 5,120, 5,120 at 14,336):
+//   4 bits, rows forms MT x NT row and column tiles of 16: N 5,120, 16 rows: 1x2 5.1, 2x2 6.0, 1x4 6.3; 32 rows: 2x2 6.2, 1x2 6.7; 64 rows: 2x4 7.0,
+//     1x2 9.0; 128 rows: 4x4 9.7, tiles 64 x 128 10.7; 256 rows: tiles 64 x 128 11.1, 4x4 17.9. N 14,336, 16 rows: 1x4 8.5, 1x1 9.1; 96 rows: tiles
+//     64 x 128 10.7, 4x4 17.9.
+//   bf16 rows: N 5,120, 16 rows: 1x2 7.1, 1x4 9.1; 48 rows: 1x4 9.5, 1x2 11.4; 64 rows: 2x4 12.3, 1x4 14.0; 128 rows: 2x4 of four waves (two workgroups a
+//     CU) 20, of eight 24; tiles of 64 x 256 33 up to 256 rows. N 14,336, 96 rows: 28 and 31, 128 rows 34 and 31.
+template <int MT, int NT>
+long rows_blocks(const mx4::GemmParams &p) {
+    return (long)mx4::ceil_div(mx4::ceil_div(p.N, 16), NT) * mx4::ceil_div(mx4::ceil_div(p.T, 16), MT);
+}
+template <int MT, int NT, int W, int D>
+bool launch_rows(const mx4::GemmParams &p, hipStream_t s) {
+    const long blocks = rows_blocks<MT, NT>(p);
+    if (blocks > kCus) return false;
+    hipLaunchKernelGGL((mx4::mx4_rows_kernel<MT, NT, W, D>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
+    return true;
+}
 template <int MT, int NT, int W>
-void launch_rows(const mx4::GemmParams &p, hipStream_t s) {
-    const unsigned grid = (unsigned)((long)mx4::ceil_div(mx4::ceil_div(p.N, 16), NT) * mx4::ceil_div(mx4::ceil_div(p.T, 16), MT));
-    if (p.xb) hipLaunchKernelGGL((mx4::mx4_rows_kernel<true, MT, NT, W>), dim3(grid), dim3(64 * W), 0, s, p);
-    else hipLaunchKernelGGL((mx4::mx4_rows_kernel<false, MT, NT, W>), dim3(grid), dim3(64 * W), 0, s, p);
+bool launch_rows16(const mx4::GemmParams &p, hipStream_t s) {
+    const long blocks = rows_blocks<MT, NT>(p);
+    if (blocks > (W == 8 ? kCus : 2 * kCus)) return false;
+    if (MT == 1 && p.T <= 4) hipLaunchKernelGGL((mx4::mx4_rows16_kernel<1, NT, W, 1>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
+    else hipLaunchKernelGGL((mx4::mx4_rows16_kernel<MT, NT, W, 4 * MT>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
+    return true;
 }
 
 template <typename C>
+long tiles(const mx4::GemmParams &p) {
+    return (long)mx4::ceil_div(p.N, C::BN) * mx4::ceil_div(p.T, C::BM);
+}
+template <typename C>
 dim3 tile_grid(const mx4::GemmParams &p) {
     return dim3((unsigned)(8 * mx4::ceil_div(mx4::ceil_div(p.N, C::BN), 8) * mx4::ceil_div(p.T, C::BM)));
+}
+// The time of n tiles, two a CU at a time, of which a round takes `full` and one of no more than a CU each `half`.
+float rounds(long n, float half, float full) {
+    const long r = n % (2 * kCus);
+    return (float)(n / (2 * kCus)) * full + (r == 0 ? 0.f : r <= kCus ? half : full);
 }
 template <typename C>
 void launch_tile(const mx4::GemmParams &p, hipStream_t s) {
@@ -75,6 +108,33 @@ void launch_tile(const mx4::GemmParams &p, hipStream_t s) {
 template <typename C>
 void launch_wide(const mx4::GemmParams &p, hipStream_t s) {
     hipLaunchKernelGGL(mx4::mx4_wide_kernel<C>, tile_grid<C>(p), dim3(C::THREADS), 0, s, p);
+}
+
+void launch4(const mx4::GemmParams &p, hipStream_t s) {
+    using Small = mx4::TileCfg<64, 128, 64, 32, 4, 2>;
+    using Middle = mx4::TileCfg<128, 128, 64, 64, 4, 2>;
+    using Large = mx4::TileCfg<256, 128, 128, 64, 3, 2>;
+    if (launch_rows<1, 1, 8, 3>(p, s) || launch_rows<1, 2, 8, 3>(p, s) || launch_rows<2, 2, 8, 2>(p, s) || launch_rows<2, 4, 8, 2>(p, s) ||
+        launch_rows<4, 4, 8, 2>(p, s))
+        return;
+    // rounds of 40 K tiles, us: 256 rows x 14,336 small 16.7, middle 13.7, large 18.6; 512 rows 31.8, 24.7, 23.3; 4,096 rows large 152, middle 174;
+    // 1,160 x 5,120 x 6,144 27.7, 26.6, 26.1, with a residual 32.9, 29.8, 29.5
+    const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 22.f, 41.f);
+    if (small <= middle && small <= large) launch_tile<Small>(p, s);
+    else if (middle <= large) launch_tile<Middle>(p, s);
+    else launch_tile<Large>(p, s);
+}
+
+void launch16(const mx4::GemmParams &p, hipStream_t s) {
+    using Small = mx4::WideCfg<64, 256, 64, 64, 2, 2>;      // two workgroups a CU
+    using Large = mx4::WideCfg<128, 256, 64, 128, 2, 1>;    // one
+    if (launch_rows16<1, 1, 8>(p, s) || launch_rows16<1, 2, 8>(p, s) || launch_rows16<1, 4, 8>(p, s) || launch_rows16<2, 4, 8>(p, s) || launch_rows16<2, 4, 4>(p, s))
+        return;
+    // rounds of 40 K tiles, us: 256 rows x 14,336 small 33, large 48; 512 rows 61, 57; 4,096 rows 451, 432
+    const long n = tiles<Large>(p);
+    const float small = rounds(tiles<Small>(p), 31.f, 64.f), large = 58.f * (float)((n + kCus - 1) / kCus);
+    if (small <= large) launch_wide<Small>(p, s);
+    else launch_wide<Large>(p, s);
 }
 
 }  // namespace
@@ -156,13 +216,8 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     p.xb = a->x_bf16; p.x_row = a->x_row; p.y = a->y; p.y_row = a->y_row; p.residual = a->residual; p.r_row = a->r_row;
     p.T = a->T; p.N = a->N; p.K = a->K; p.y_bf16 = a->y_type == CLEF_HIP_GEMM_Y_BF16;
     p.vec = aligned16(a->y) && a->y_row % (p.y_bf16 ? 8 : 4) == 0 && (!a->residual || (aligned16(a->residual) && a->r_row % 4 == 0));
-    const hipStream_t s = (hipStream_t)stream;
-    if (a->T <= 16) launch_rows<1, 1, 8>(p, s);
-    else if (a->T <= 32) launch_rows<2, 2, 8>(p, s);
-    else if (p.T < 256) launch_rows<4, 4, 4>(p, s);
-    else if (p.xb) launch_wide<mx4::WideCfg<128, 256, 64, 128, 3, 1>>(p, s);
-    else if ((long)mx4::ceil_div(p.T, 256) * mx4::ceil_div(p.N, 128) < 400) launch_tile<mx4::TileCfg<128, 128, 64, 64, 4, 2>>(p, s);
-    else launch_tile<mx4::TileCfg<256, 128, 128, 64, 3, 2>>(p, s);
+    if (p.xb) launch16(p, (hipStream_t)stream);
+    else launch4(p, (hipStream_t)stream);
     return launch_ok("mx4_gemm", err, errlen);
 }
 

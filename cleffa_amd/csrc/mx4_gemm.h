@@ -23,74 +23,77 @@ __device__ __forceinline__ bf16x8 widen(unsigned c, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
-// MT x NT tiles of 16 rows and 16 columns a workgroup, whose W waves share the K tiles and add their sums in LDS in a
-// fixed order. Operands come straight from memory. BF: X is bf16.
-template <bool BF, int MT, int NT, int W>
+// The sums of a workgroup's W waves, each of MT x NT tiles of 16 x 16, added in order through LDS and stored.
+template <int MT, int NT, int W>
+__device__ __forceinline__ void join_waves(const GemmParams &p, const f32x4 (&acc)[MT][NT], f32x4 (*part)[MT * NT][64], int t0, int n0) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) part[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int u = wave; u < MT * NT; u += W) {
+        f32x4 s = part[0][u][lane];
+#pragma unroll
+        for (int w = 1; w < W; w++) s += part[w][u][lane];
+        const int t = 16 * (t0 + u / NT) + (lane & 15), c = 16 * (n0 + u % NT) + 4 * (lane >> 4);
+        if (t < p.T && c < p.N) store4(p, t, c, s[0], s[1], s[2], s[3]);
+    }
+}
+
+// Few 4-bit rows: MT x NT tiles of 16 rows and 16 columns a workgroup, whose W waves share the K tiles and add their sums in LDS in a
+// fixed order. Operands come straight from memory, D K tiles ahead.
+template <int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(GemmParams p) {
-    __shared__ f32x4 part[W > 1 ? W : 1][MT * NT][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int n_tiles = ceil_div(p.N, 16), t_tiles = ceil_div(p.T, 16);
-    const int nb = ceil_div(n_tiles, NT);
+    __shared__ f32x4 part[W][MT * NT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int n_tiles = ceil_div(p.N, 16), t_tiles = ceil_div(p.T, 16), nb = ceil_div(n_tiles, NT);
     const int n0 = (blockIdx.x % nb) * NT, t0 = (blockIdx.x / nb) * MT;
+    const int k_lo = p.w.ktiles * wave / W, k_hi = p.w.ktiles * (wave + 1) / W;
+    struct Ops {
+        u32x4 w[NT], x[MT];
+        int ws[NT], xs[MT];
+    };
+    auto load = [&](Ops &o, int kt) __attribute__((always_inline)) {
+        kt = min(kt, k_hi - 1);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int nt = min(n0 + j, n_tiles - 1);
+            o.w[j] = *(const u32x4 *)(p.w.tile(nt, kt) + 16 * lane);
+            o.ws[j] = *(const int *)(p.w.group(nt, kt >> 2) + 4 * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int tt = min(t0 + i, t_tiles - 1);
+            o.x[i] = *(const u32x4 *)(p.x.tile(tt, kt) + 16 * lane);
+            o.xs[i] = *(const int *)(p.x.group(tt, kt >> 2) + 4 * lane);
+        }
+    };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int k_lo = (int)((long)p.w.ktiles * wave / W), k_hi = (int)((long)p.w.ktiles * (wave + 1) / W);
-    for (int kt = k_lo; kt < k_hi; kt++) {
-        const int sh = 8 * (kt & 3);
-        u32x4 wc[NT];
-        int ws[NT];
+    if (k_lo < k_hi) {
+        Ops ops[D];
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int nt = min(n0 + j, n_tiles - 1);
-            wc[j] = *(const u32x4 *)(p.w.tile(nt, kt) + 16 * lane);
-            ws[j] = *(const int *)(p.w.group(nt, kt >> 2) + 4 * lane) >> sh;
-        }
+        for (int d = 0; d < D; d++) load(ops[d], k_lo + d);
+        for (int kt = k_lo; kt < k_hi; kt += D) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const int tt = min(t0 + i, t_tiles - 1);
-            if constexpr (BF) {
-                const int t = min(16 * tt + l16, p.T - 1), k = KT * kt + 32 * g;
-                const uint16_t *x = p.xb + (size_t)t * p.x_row + k;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bf16x8 b = k < p.K ? *(const bf16x8 *)(x + 8 * j) : bf16x8{};
+            for (int d = 0; d < D; d++) {
+                const int sh = 8 * (kt + d & 3);
+                if (kt + d < k_hi) {
 #pragma unroll
                     for (int n = 0; n < NT; n++)
-                        acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(wc[n][j], __uint_as_float((unsigned)(ws[n] & 255) << 23)), b, acc[i][n], 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+                            acc[i][n] = mfma4(ops[d].w[n], ops[d].x[i], acc[i][n], (unsigned)ops[d].ws[n] >> sh, (unsigned)ops[d].xs[i] >> sh);
                 }
-            } else {
-                const u32x4 xc = *(const u32x4 *)(p.x.tile(tt, kt) + 16 * lane);
-                const int xs = *(const int *)(p.x.group(tt, kt >> 2) + 4 * lane) >> sh;
-#pragma unroll
-                for (int n = 0; n < NT; n++) acc[i][n] = mfma4(wc[n], xc, acc[i][n], ws[n], xs);
+                load(ops[d], kt + d + D);
             }
         }
     }
-    if constexpr (W > 1) {
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) part[wave][i * NT + j][lane] = acc[i][j];
-        __syncthreads();
-        for (int u = wave; u < MT * NT; u += W) {
-            f32x4 s = part[0][u][lane];
-#pragma unroll
-            for (int w = 1; w < W; w++) s += part[w][u][lane];
-            const int t = 16 * (t0 + u / NT) + l16, c = 16 * (n0 + u % NT) + 4 * g;
-            if (t < p.T && c < p.N) store4(p, t, c, s[0], s[1], s[2], s[3]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const int t = 16 * (t0 + i) + l16, c = 16 * (n0 + j) + 4 * g;
-                if (t < p.T && c < p.N) store4(p, t, c, acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-            }
-    }
+    join_waves<MT, NT, W>(p, acc, part, t0, n0);
 }
 
 }  // namespace mx4

@@ -45,8 +45,9 @@ __device__ __forceinline__ void for_each(F &&f) {
 // Waits for all LDS reads in one statement that names what they fill, codes and scales, so that no copy or use of it comes before.
 template <int F>
 __device__ __forceinline__ void lds_wait(u32x4 (&r)[F]) {
-    static_assert(F == 4 || F == 6 || F == 8, "operands of a wave's tile");
-    if constexpr (F == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3])::"memory");
+    static_assert(F == 3 || F == 4 || F == 6 || F == 8, "operands of a wave's tile");
+    if constexpr (F == 3) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2])::"memory");
+    else if constexpr (F == 4) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3])::"memory");
     else if constexpr (F == 6)
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(r[4]), "+v"(r[5])::"memory");
     else
@@ -54,7 +55,10 @@ __device__ __forceinline__ void lds_wait(u32x4 (&r)[F]) {
 }
 template <int F>
 __device__ __forceinline__ void lds_wait(u32x4 (&r)[F], unsigned (&s)[2][F]) {
-    if constexpr (F == 4)
+    if constexpr (F == 3)
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[1][0]), "+v"(s[1][1]),
+                     "+v"(s[1][2])::"memory");
+    else if constexpr (F == 4)
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[0][3]),
                      "+v"(s[1][0]), "+v"(s[1][1]), "+v"(s[1][2]), "+v"(s[1][3])::"memory");
     else if constexpr (F == 6)
@@ -95,20 +99,26 @@ __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&a
             continue;
         }
         constexpr int LANES = WN / 4, ROWS_I = 64 / LANES;
-        const int c = c0 + 4 * (lane % LANES);
+        const int c = c0 + 4 * (lane % LANES), t = t0 + lane / LANES;
         const uint8_t *from = mine + lane / LANES * OUT_ROW + 16 * (lane % LANES);
         if (p.vec && t0 + 32 <= p.T && c0 + WN <= p.N) {
+            f32x4 v[32 / ROWS_I];
+            if (p.residual) {       // all loads together
 #pragma unroll
-            for (int r = 0; r < 32; r += ROWS_I) {
-                const f32x4 v = *(const f32x4 *)(from + r * OUT_ROW);
-                store4_whole(p, t0 + r + lane / LANES, c, v[0], v[1], v[2], v[3]);
+                for (int r = 0; r < 32 / ROWS_I; r++) v[r] = *(const f32x4 *)(p.residual + (size_t)(t + r * ROWS_I) * p.r_row + c);
+#pragma unroll
+                for (int r = 0; r < 32 / ROWS_I; r++) v[r] += *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 32 / ROWS_I; r++) v[r] = *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
             }
+#pragma unroll
+            for (int r = 0; r < 32 / ROWS_I; r++) *(f32x4 *)((float *)p.y + (size_t)(t + r * ROWS_I) * p.y_row + c) = v[r];
         } else {
 #pragma unroll 1
             for (int r = 0; r < 32; r += ROWS_I) {
                 const f32x4 v = *(const f32x4 *)(from + r * OUT_ROW);
-                const int t = t0 + r + lane / LANES;
-                if (t < p.T && c < p.N) store4(p, t, c, v[0], v[1], v[2], v[3]);
+                if (t + r < p.T && c < p.N) store4(p, t + r, c, v[0], v[1], v[2], v[3]);
             }
         }
     }

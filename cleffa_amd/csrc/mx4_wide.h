@@ -136,46 +136,46 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES / 4 * C::PER_CU) void mx4_wide
             o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
         }
     };
-    // The products of a step; between them the next step's W is widened (POS_NEXT: its K tile's place in its group), and fills go out.
-    auto products = [&](auto STEP, auto POS_NEXT, auto STEP_NEXT, int fill_kt, unsigned fill_stage, auto F0, auto F1) CLEF_INLINE {
-        constexpr int st = decltype(STEP)::value, f0 = decltype(F0)::value, nf = decltype(F1)::value - f0;
-        for_each<P>([&](auto Q) CLEF_INLINE {
-            constexpr int q = decltype(Q)::value, i = q % MT, j = q / MT;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, wide[st & 1][j]), __builtin_bit_cast(bf16x8, x[st & 3][i]),
-                                                              acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            widen2(POS_NEXT, STEP_NEXT, j, i);
-#pragma unroll
-            for (int f = f0 + q * nf / P; f < f0 + (q + 1) * nf / P; f++) fill_one(fill_kt, fill_stage, f);
-            __builtin_amdgcn_sched_barrier(0);
-        });
-    };
     constexpr std::integral_constant<int, 0> i0;
     constexpr std::integral_constant<int, 1> i1;
     unsigned stage = 0;
     auto after = [&](unsigned st) CLEF_INLINE { return st == (STAGES - 1) * C::STAGE_BYTES ? 0u : st + C::STAGE_BYTES; };
     // K tile kt at POS of its group. X of a step is read two steps before, so that after the sixth step nothing more is read of this K
-    // tile, and its buffer takes kt + STAGES: a part with the last two steps, the rest with the next tile's first six.
+    // tile, and its buffer takes kt + STAGES, with the last two steps, at once: spread over the next tile's steps the last of it came late, and
+    // a K tile of a 64 x 128 tile took 0.75 us, not 0.5.
     auto k_tile = [&](int kt, auto POS) CLEF_INLINE {
         constexpr int pos = decltype(POS)::value, next = (pos + 1) & 3;
-        const unsigned before = stage == 0 ? (STAGES - 1) * C::STAGE_BYTES : stage - C::STAGE_BYTES, here = stage;
+        const unsigned here = stage;
         for_each<8>([&](auto STEP) CLEF_INLINE {
             constexpr int st = decltype(STEP)::value;
             constexpr std::integral_constant<int, (st + 1) & 7> st_next;
             constexpr std::integral_constant<int, st == 7 ? next : pos> pos_next;
-            if constexpr (st == 6) {
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((STAGES - 2) * FILLS + (next >= 2 && next < STAGES ? S_FILLS : 0)) : "memory");
-                if constexpr (next == 1) fill_scales((kt >> 2) + 1);
-                stage = after(stage);
-                if constexpr (next == 0) read_scales();
-                read_w(i0, stage);
-            }
-            if constexpr (st == 1) read_w(i1, stage);
-            read_x(std::integral_constant<int, (st + 2) & 7>{}, stage);
-            __builtin_amdgcn_sched_barrier(0);
-            constexpr int a0 = st >= 6 ? (st - 6) * FILLS / 8 : (st + 2) * FILLS / 8, a1 = st >= 6 ? (st - 5) * FILLS / 8 : (st + 3) * FILLS / 8;
-            products(STEP, pos_next, st_next, st >= 6 ? kt + STAGES : kt + STAGES - 1, st >= 6 ? here : before,
-                     std::integral_constant<int, a0>{}, std::integral_constant<int, a1>{});
+            // between the products the next step's W is widened, X and codes are read, fills go out; the barriers keep them there
+            for_each<P>([&](auto Q) CLEF_INLINE {
+                constexpr int q = decltype(Q)::value, i = q % MT, j = q / MT, first = st == 6 ? P / 4 : 0;
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, wide[st & 1][j]), __builtin_bit_cast(bf16x8, x[st & 3][i]), acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (q == first) {
+                    if constexpr (st == 6) {
+                        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((STAGES - 2) * FILLS + (next >= 2 && next < STAGES ? S_FILLS : 0)) : "memory");
+                        if constexpr (next == 1) fill_scales((kt >> 2) + 1);
+                        stage = after(stage);
+                    }
+                    read_x(std::integral_constant<int, (st + 2) & 7>{}, stage);
+                }
+                if constexpr (q == first + 1) {
+                    if constexpr (st == 6) read_w(i0, stage);
+                    if constexpr (st == 6 && next == 0) read_scales();
+                    if constexpr (st == 1) read_w(i1, stage);
+                }
+                widen2(pos_next, st_next, j, i);
+                constexpr int at = (st - 6) * P + q - P / 4 - 1, n = 2 * P - P / 4 - 1;    // of the products behind the barrier
+                if constexpr (st >= 6 && at >= 0) {
+#pragma unroll
+                    for (int f = at * FILLS / n; f < (at + 1) * FILLS / n; f++) fill_one(kt + STAGES, here, f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
             if constexpr (st == 6 && next == 0) {
                 lds_wait(x[(st + 2) & 3], w[0], s_next);
 #pragma unroll
@@ -186,10 +186,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES / 4 * C::PER_CU) void mx4_wide
         });
     };
     fill_scales(0);
-    for (int q = 0; q < STAGES - 1; q++)
+    for (int q = 0; q < STAGES; q++)
 #pragma unroll
         for (int f = 0; f < FILLS; f++) fill_one(q, q * C::STAGE_BYTES, f);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((STAGES - 2) * FILLS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((STAGES - 1) * FILLS) : "memory");
     read_w(i0, 0);
     read_scales();
     read_x(i0, 0);
@@ -203,8 +203,6 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES / 4 * C::PER_CU) void mx4_wide
         widen2(i0, i0, j, 1);
     }
     lds_wait(x[1], w[0]);
-#pragma unroll
-    for (int f = 0; f < 2 * FILLS / 8; f++) fill_one(STAGES - 1, (STAGES - 1) * C::STAGE_BYTES, f);
     int kt = 0;
     for (; kt + 4 <= ktiles; kt += 4) for_each<4>([&](auto POS) CLEF_INLINE { k_tile(kt + decltype(POS)::value, POS); });
     for_each<3>([&](auto POS) CLEF_INLINE {
