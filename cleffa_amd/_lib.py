@@ -141,17 +141,16 @@ class Mx4GemmArgs(ctypes.Structure):
     ]
 
 
-class RotaryHeads(ctypes.Structure):
-    _fields_ = [
-        ("heads", c_int), ("x", c_void_p), ("out", c_void_p), ("x_row", ctypes.c_long), ("x_head", ctypes.c_long),
-        ("out_row", ctypes.c_long), ("out_head", ctypes.c_long), ("norm", c_void_p),
-    ]
+_HEADS = (("heads", c_int), ("x", c_void_p), ("out", c_void_p), ("x_row", ctypes.c_long), ("x_head", ctypes.c_long),
+          ("out_row", ctypes.c_long), ("out_head", ctypes.c_long), ("norm", c_void_p))
 
 
 class RotaryArgs(ctypes.Structure):
+    # the members of q and k by name, so that one call fills all of them
     _fields_ = [
         ("T", c_int), ("hd", c_int), ("n_rot", c_int), ("layout", c_int), ("axes", c_int), ("type", c_int),
-        ("eps", c_float), ("magnitude", c_float), ("pos", c_void_p), ("freq", c_void_p), ("q", RotaryHeads), ("k", RotaryHeads),
+        ("eps", c_float), ("magnitude", c_float), ("pos", c_void_p), ("freq", c_void_p),
+        *((f"{g}.{name}", t) for g in "qk" for name, t in _HEADS),
     ]
 
 

@@ -19,7 +19,13 @@ _Y_TYPES = {torch.bfloat16: Y_BF16, torch.float32: Y_F32}
 
 
 def _rows_arg(t, name, shape, dtype, device, step=1):
-    """Address and row stride of a matrix whose rows may lie apart (by multiples of ``step`` elements)."""
+    """Address and row stride of a matrix whose rows may lie apart (by multiples of ``step`` elements). One test for the
+    ordinary case; the faults are told apart only where it fails."""
+    if t.__class__ is torch.Tensor and t.dtype is dtype and t.shape == shape and t.device == device:
+        row, one = t.stride()
+        p = t.data_ptr()
+        if one == 1 and row >= shape[1] and not row % step and (step == 1 or not p & 15):
+            return p, row
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if t.shape != shape:
@@ -49,24 +55,24 @@ class Mx4Matrix:
         self.rows, self.K, self.device = int(rows), int(K), _device(device)
         if self.device.type == "cuda":
             init_device(self.device)
-        self.codes = torch.empty(n_codes.value, dtype=torch.uint8, device=self.device) if codes is None else codes
-        self.scales = torch.empty(n_scales.value, dtype=torch.uint8, device=self.device) if scales is None else scales
-        self._shapes = (n_codes.value,), (n_scales.value,)
-        self._args()
+        self._codes = torch.empty(n_codes.value, dtype=torch.uint8, device=self.device) if codes is None else codes
+        self._scales = torch.empty(n_scales.value, dtype=torch.uint8, device=self.device) if scales is None else scales
+        # the buffers are the matrix's for good: their addresses are checked and taken once
+        self._ptrs = (_arg(self._codes, "codes", (n_codes.value,), torch.uint8, self.device),
+                      _arg(self._scales, "scales", (n_scales.value,), torch.uint8, self.device))
 
-    def _args(self):
-        return (_arg(self.codes, "codes", self._shapes[0], torch.uint8, self.device),
-                _arg(self.scales, "scales", self._shapes[1], torch.uint8, self.device))
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
 
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self._codes.numel() + self._scales.numel()
 
     def first(self, rows):
         """The first rows (a multiple of 16, or all) as a matrix in the same buffers."""
         if not 0 <= rows <= self.rows or (rows % 16 and rows != self.rows):
             raise ValueError(f"the first {rows} of {self.rows} rows: a multiple of 16, or all")
         tiles = -(-rows // 16)
-        return Mx4Matrix(rows, self.K, self.device, self.codes[:tiles * -(-self.K // 128) * 1024], self.scales[:tiles * -(-self.K // 512) * 256])
+        return Mx4Matrix(rows, self.K, self.device, self._codes[:tiles * -(-self.K // 128) * 1024], self._scales[:tiles * -(-self.K // 512) * 256])
 
     @classmethod
     def quantised(cls, x, stream=None):
@@ -97,7 +103,7 @@ class Mx4Matrix:
         flat = _arg(codes, "codes", codes.shape, torch.uint8, self.device)
         if scales.dtype is not torch.uint8 or scales.device != self.device or not scales.is_contiguous():
             raise ValueError("scales must be contiguous uint8 on the codes' device")
-        own, rows, K = self._args(), self.rows, self.K
+        own, rows, K = self._ptrs, self.rows, self.K
         lib = _lib.load()
         _launch(lambda a, s, err, n: lib.clef_hip_mx4_pack(rows, K, flat, scales.data_ptr(), *own, to_flat, s, err, n), ctypes.c_int(0), self.device, stream)
         return self
@@ -107,7 +113,7 @@ class Mx4Matrix:
         if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPE_OUT:
             raise TypeError(f"x must be a bf16, f16 or f32 tensor, not {getattr(x, 'dtype', type(x))}")
         px, row = _rows_arg(x, "x", (self.rows, self.K), x.dtype, self.device, 8)
-        _launch(_lib.load().clef_hip_mx4_quantise, _lib.Mx4RowsArgs(self.rows, self.K, _DTYPE_OUT[x.dtype], row, px, *self._args()), self.device, stream)
+        _launch(_lib.load().clef_hip_mx4_quantise, _lib.Mx4RowsArgs(self.rows, self.K, _DTYPE_OUT[x.dtype], row, px, *self._ptrs), self.device, stream)
         return self
 
     def values(self, out=None, out_dtype="bf16", stream=None):
@@ -119,7 +125,7 @@ class Mx4Matrix:
         if not isinstance(out, torch.Tensor) or out.dtype not in _Y_TYPES:
             raise TypeError("out must be a bf16 or f32 tensor")
         px, row = _rows_arg(out, "out", (self.rows, self.K), out.dtype, self.device, 8)
-        _launch(_lib.load().clef_hip_mx4_values, _lib.Mx4RowsArgs(self.rows, self.K, _DTYPE_OUT[out.dtype], row, px, *self._args()), self.device, stream)
+        _launch(_lib.load().clef_hip_mx4_values, _lib.Mx4RowsArgs(self.rows, self.K, _DTYPE_OUT[out.dtype], row, px, *self._ptrs), self.device, stream)
         return out
 
 
@@ -133,7 +139,7 @@ def mx4_gemm(X, W, Y=None, out="bf16", residual=None, stream=None):
     if isinstance(X, Mx4Matrix):
         if X.device != dev:
             raise ValueError(f"X is on {X.device}, W on {dev}")
-        T, xk, xb, x_row, xc = X.rows, X.K, None, 0, X._args()
+        T, xk, xb, x_row, xc = X.rows, X.K, None, 0, X._ptrs
     else:
         if not isinstance(X, torch.Tensor) or X.dim() != 2:
             raise TypeError("X must be an Mx4Matrix or a matrix in bf16")
@@ -152,6 +158,6 @@ def mx4_gemm(X, W, Y=None, out="bf16", residual=None, stream=None):
     if T == 0:
         return Y
     pr, r_row = (None, 0) if residual is None else _rows_arg(residual, "residual", (T, N), torch.float32, dev)
-    a = _lib.Mx4GemmArgs(T, N, K, _Y_TYPES[Y.dtype], *W._args(), *xc, xb, x_row, y_row, r_row, py, pr)
+    a = _lib.Mx4GemmArgs(T, N, K, _Y_TYPES[Y.dtype], *W._ptrs, *xc, xb, x_row, y_row, r_row, py, pr)
     _launch(_lib.load().clef_hip_mx4_gemm, a, dev, stream)
     return Y

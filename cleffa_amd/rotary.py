@@ -50,6 +50,7 @@ class Rotary:
         if not math.isfinite(magnitude):
             raise ValueError(f"magnitude {magnitude}")
         self.n_rot, self.layout, self.axes, self.eps, self.magnitude = int(n_rot), layout, int(axes), eps, float(magnitude)
+        self._layout = _lib.ROTARY_LAYOUTS[layout]
         self.device = _device(device)
         if self.device.type == "cuda":
             init_device(self.device)
@@ -65,24 +66,33 @@ class Rotary:
         q = qkv[:, :wide * nh * hd].unflatten(1, (nh, wide * hd))[:, :, :hd]
         return q, qkv[:, wide * nh * hd:(wide * nh + nkv) * hd].unflatten(1, (nkv, hd))
 
+    def _view(self, t, name, shape, dtype):
+        """Address, row and head stride of heads. One test for the ordinary case; the faults are told apart only where it fails."""
+        if t.__class__ is torch.Tensor and t.dtype is dtype and t.shape == shape and t.device == self.device:
+            row, head, one = t.stride()
+            if one == 1:
+                return t.data_ptr(), row, head
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor")
+        if t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dtype is not dtype:
+            raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, expected {self.device}")
+        if t.numel():
+            raise ValueError(f"the dims of a head of {name} must be contiguous")
+        return t.data_ptr(), 0, 0
+
     def _heads(self, x, out, norm, name, T, hd, dtype):
         if x is None:
             if out is not None or norm is not None:
                 raise ValueError(f"{name}: an output or norm without heads")
-            return _lib.RotaryHeads(0, None, None, 0, 0, 0, 0, None)
-        for t, what in ((x, name), (out, name + "_out")):
-            if not isinstance(t, torch.Tensor):
-                raise TypeError(f"{what} must be a torch tensor")
-            if t.dim() != 3 or t.shape[0] != T or t.shape[2] != hd or t.shape[1] != x.shape[1]:
-                raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {(T, x.shape[1], hd)}")
-            if t.dtype is not dtype:
-                raise TypeError(f"{what} has dtype {t.dtype}, expected {dtype}")
-            if t.device != self.device:
-                raise ValueError(f"{what} is on {t.device}, expected {self.device}")
-            if t.stride(2) != 1 and t.numel():
-                raise ValueError(f"the dims of a head of {what} must be contiguous")
-        norm = None if norm is None else _arg(norm, name + "_norm", (hd,), torch.float32, self.device)
-        return _lib.RotaryHeads(x.shape[1], x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1), norm)
+            return 0, None, None, 0, 0, 0, 0, None
+        shape = (T, x.shape[1] if isinstance(x, torch.Tensor) and x.dim() == 3 else -1, hd)
+        px, row, head = self._view(x, name, shape, dtype)
+        po, out_row, out_head = (px, row, head) if out is x else self._view(out, name + "_out", shape, dtype)
+        return shape[1], px, po, row, head, out_row, out_head, None if norm is None else _arg(norm, name + "_norm", (hd,), torch.float32, self.device)
 
     def apply(self, q, k, pos, q_norm=None, k_norm=None, q_out=None, k_out=None, stream=None):
         """q [T][nh][hd] and k [T][nkv][hd] (or None), bf16, f16 or f32, turned by pos (int32 [T] or [T][axes]), each after its
@@ -91,14 +101,16 @@ class Rotary:
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPE_OUT:
             raise TypeError("q must be a bf16, f16 or f32 tensor [T][heads][hd]")
         T, _, hd = q.shape
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None and k is not None else k_out
+        dtype = q.dtype
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if k_out is None and k is not None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         if not isinstance(pos, torch.Tensor) or pos.dtype is not torch.int32 or pos.device != self.device or not pos.is_contiguous():
             raise ValueError("pos must be contiguous int32 on the operator's device")
-        if tuple(pos.shape) not in (((T,), (T, 1)) if self.axes == 1 else ((T, self.axes),)):
+        if pos.shape != (T, self.axes) and (self.axes > 1 or pos.shape != (T,)):
             raise ValueError(f"pos has shape {tuple(pos.shape)}, expected {(T, self.axes)}")
-        a = _lib.RotaryArgs(T, hd, self.n_rot, _lib.ROTARY_LAYOUTS[self.layout], self.axes, _DTYPE_OUT[q.dtype], self.eps, self.magnitude,
-                            pos.data_ptr(), self.freq.data_ptr(), self._heads(q, q_out, q_norm, "q", T, hd, q.dtype),
-                            self._heads(k, k_out, k_norm, "k", T, hd, q.dtype))
+        a = _lib.RotaryArgs(T, hd, self.n_rot, self._layout, self.axes, _DTYPE_OUT[dtype], self.eps, self.magnitude, pos.data_ptr(), self.freq.data_ptr(),
+                            *self._heads(q, q_out, q_norm, "q", T, hd, dtype), *self._heads(k, k_out, k_norm, "k", T, hd, dtype))
         _launch(_lib.load().clef_hip_rotary, a, self.device, stream)
         return q_out, k_out

@@ -23,7 +23,7 @@ def _err():
 
 
 @pytest.mark.parametrize("name,cls", [("clef_hip_mx4_rows_args", _lib.Mx4RowsArgs), ("clef_hip_mx4_gemm_args", _lib.Mx4GemmArgs),
-                                      ("clef_hip_rotary_heads", _lib.RotaryHeads), ("clef_hip_rotary_args", _lib.RotaryArgs)])
+                                      ("clef_hip_rotary_args", _lib.RotaryArgs)])
 def test_struct_layouts(name, cls, tmp_path):
     """The ctypes mirrors have the C compiler's offsets and sizes."""
     src = "#include <stdio.h>\n#include <stddef.h>\n#include \"clef_hip_attn.h\"\nint main(void) {\n"
@@ -107,19 +107,16 @@ def test_no_rows_are_no_work():
     assert lib.clef_hip_mx4_quantise(ctypes.byref(_lib.Mx4RowsArgs(0, 32, 0, 32, None, None, None)), None, err, 256)
     assert lib.clef_hip_mx4_values(ctypes.byref(_lib.Mx4RowsArgs(0, 32, 0, 32, None, None, None)), None, err, 256)
     assert lib.clef_hip_mx4_pack(0, 32, None, None, None, None, 0, None, err, 256)
-    none = _lib.RotaryHeads(0, None, None, 0, 0, 0, 0, None)
-    assert lib.clef_hip_rotary(ctypes.byref(_lib.RotaryArgs(0, 64, 64, 0, 1, 0, 1e-6, 1.0, None, None, none, none)), None, err, 256)
-    assert lib.clef_hip_rotary(ctypes.byref(_lib.RotaryArgs(4, 64, 64, 0, 1, 0, 1e-6, 1.0, None, None, none, none)), None, err, 256)
+    none = (0, None, None, 0, 0, 0, 0, None) * 2
+    assert lib.clef_hip_rotary(ctypes.byref(_lib.RotaryArgs(0, 64, 64, 0, 1, 0, 1e-6, 1.0, None, None, *none)), None, err, 256)
+    assert lib.clef_hip_rotary(ctypes.byref(_lib.RotaryArgs(4, 64, 64, 0, 1, 0, 1e-6, 1.0, None, None, *none)), None, err, 256)
 
 
 def _rotary_args(**over):
     heads = dict(heads=4, x=FAKE, out=FAKE, x_row=512, x_head=128, out_row=512, out_head=128, norm=None)
-    a = _lib.RotaryArgs(3, 128, 64, 0, 1, 0, 1e-6, 1.0, FAKE, FAKE, _lib.RotaryHeads(*heads.values()), _lib.RotaryHeads(*heads.values()))
+    a = _lib.RotaryArgs(3, 128, 64, 0, 1, 0, 1e-6, 1.0, FAKE, FAKE, *heads.values(), *heads.values())
     for k, v in over.items():
-        if k in heads:
-            setattr(a.q, k, v)
-        else:
-            setattr(a, k, v)
+        setattr(a, "q." + k if k in heads else k, v)
     return a
 
 
