@@ -222,7 +222,6 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     p.x = matrix(a->x_codes, a->x_scales, a->T, a->K);
     p.xb = a->x_bf16; p.x_row = a->x_row; p.y = a->y; p.y_row = a->y_row; p.residual = a->residual; p.r_row = a->r_row;
     p.T = a->T; p.N = a->N; p.K = a->K; p.y_bf16 = a->y_type == CLEF_HIP_GEMM_Y_BF16;
-    p.vec = aligned16(a->y) && a->y_row % (p.y_bf16 ? 8 : 4) == 0 && (!a->residual || (aligned16(a->residual) && a->r_row % 4 == 0));
     if (p.xb) launch16(p, (hipStream_t)stream);
     else launch4(p, (hipStream_t)stream);
     return launch_ok("mx4_gemm", err, errlen);

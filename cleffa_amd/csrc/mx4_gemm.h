@@ -7,7 +7,6 @@
 namespace clef_hip {
 namespace mx4 {
 
-typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 __device__ __forceinline__ i32x8 operand(u32x4 c) { return i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0}; }
@@ -37,7 +36,7 @@ __device__ __forceinline__ void join_waves(const GemmParams &p, const f32x4 (&ac
 #pragma unroll
         for (int w = 1; w < W; w++) s += part[w][u][lane];
         const int t = 16 * (t0 + u / NT) + (lane & 15), c = 16 * (n0 + u % NT) + 4 * (lane >> 4);
-        if (t < p.T && c < p.N) store4(p, t, c, s[0], s[1], s[2], s[3]);
+        if (t < p.T && c < p.N) store4(p, t, c, s);
     }
 }
 

@@ -58,30 +58,31 @@ struct GemmParams {
     void *y;
     const float *residual;
     int T, N, K, y_bf16;
-    int vec;                  // y (and the residual) allow stores of four columns at a time
 };
 
-// Four consecutive columns of a row, all inside the matrix, at addresses that allow it: residual, rounding, store.
-__device__ __forceinline__ void store4_whole(const GemmParams &p, int t, int c, float v0, float v1, float v2, float v3) {
+// Vectors at any element's address: the memory takes them, and odd row strides keep their wide stores.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// Up to four consecutive columns of a row, c inside the matrix: residual, rounding, store.
+__device__ __forceinline__ void store4(const GemmParams &p, int t, int c, f32x4 v) {
+    const int n = p.N - c;
     if (p.y_bf16) {
-        *(u32x2 *)((uint16_t *)p.y + (size_t)t * p.y_row + c) = u32x2{pack_bf16(v0, v1), pack_bf16(v2, v3)};
+        uint16_t *y = (uint16_t *)p.y + (size_t)t * p.y_row + c;
+        if (n >= 4) *(u32x2_any *)y = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        else
+            for (int i = 0; i < n; i++) y[i] = f2bf(i == 0 ? v[0] : i == 1 ? v[1] : v[2]);
         return;
     }
-    float4 o = {v0, v1, v2, v3};
-    if (p.residual) {
-        const float4 r = *(const float4 *)(p.residual + (size_t)t * p.r_row + c);
-        o = {v0 + r.x, v1 + r.y, v2 + r.z, v3 + r.w};
-    }
-    *(float4 *)((float *)p.y + (size_t)t * p.y_row + c) = o;
-}
-// Anywhere, c inside the matrix.
-__device__ __forceinline__ void store4(const GemmParams &p, int t, int c, float v0, float v1, float v2, float v3) {
-    const int n = p.N - c;
-    if (p.vec && n >= 4) return store4_whole(p, t, c, v0, v1, v2, v3);
-    const float v[4] = {v0, v1, v2, v3};
-    for (int i = 0; i < 4 && i < n; i++) {
-        if (p.y_bf16) ((uint16_t *)p.y)[(size_t)t * p.y_row + c + i] = f2bf(v[i]);
-        else ((float *)p.y)[(size_t)t * p.y_row + c + i] = v[i] + (p.residual ? p.residual[(size_t)t * p.r_row + c + i] : 0.f);
+    float *y = (float *)p.y + (size_t)t * p.y_row + c;
+    const float *r = p.residual ? p.residual + (size_t)t * p.r_row + c : nullptr;
+    if (n >= 4) {
+        if (r) v += *(const f32x4_any *)r;
+        *(f32x4_any *)y = v;
+    } else {
+        for (int i = 0; i < n; i++) y[i] = (i == 0 ? v[0] : i == 1 ? v[1] : v[2]) + (r ? r[i] : 0.f);
     }
 }
 

@@ -87,39 +87,47 @@ __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&a
             for (int e = 0; e < 4; e++)
                 *(f32x4 *)(mine + (lane & 31) * OUT_ROW + (32 * j + 8 * e + 4 * (lane >> 5)) * 4) =
                     f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-        if (p.vec && p.y_bf16 && t0 + 32 <= p.T && c0 + WN <= p.N) {
+        // V columns a lane, 16 bytes of Y; the columns before N that are fewer come after, one by one
+        if (p.y_bf16) {
             constexpr int LANES = WN / 8, ROWS_I = 64 / LANES;    // lanes of a row, rows of an instruction
+            const int c = c0 + 8 * (lane % LANES), t = t0 + lane / LANES;
             const uint8_t *from = mine + lane / LANES * OUT_ROW + 32 * (lane % LANES);
-            uint16_t *to = (uint16_t *)p.y + (size_t)(t0 + lane / LANES) * p.y_row + c0 + 8 * (lane % LANES);
+            uint16_t *to = (uint16_t *)p.y + (size_t)t * p.y_row + c;
+            const int rows = c + 8 <= p.N ? p.T - t : 0;
 #pragma unroll
             for (int r = 0; r < 32; r += ROWS_I) {
                 const f32x4 a = *(const f32x4 *)(from + r * OUT_ROW), b = *(const f32x4 *)(from + r * OUT_ROW + 16);
-                *(u32x4 *)(to + (size_t)r * p.y_row) = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
+                if (r < rows)
+                    *(u32x4_any *)(to + (size_t)r * p.y_row) = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
+            }
+            if (c0 + WN > p.N && p.N % 8) {
+#pragma unroll 1
+                for (int r = 0; r < 32; r += ROWS_I)
+                    for (int k = 0; k < 8; k += 4)
+                        if (t + r < p.T && c + 8 > p.N && c + k < p.N) store4(p, t + r, c + k, *(const f32x4 *)(from + r * OUT_ROW + 4 * k));
             }
             continue;
         }
         constexpr int LANES = WN / 4, ROWS_I = 64 / LANES;
         const int c = c0 + 4 * (lane % LANES), t = t0 + lane / LANES;
         const uint8_t *from = mine + lane / LANES * OUT_ROW + 16 * (lane % LANES);
-        if (p.vec && t0 + 32 <= p.T && c0 + WN <= p.N) {
-            f32x4 v[32 / ROWS_I];
-            if (p.residual) {       // all loads together
+        const int rows = c + 4 <= p.N ? p.T - t : 0;
+        f32x4 v[32 / ROWS_I];
 #pragma unroll
-                for (int r = 0; r < 32 / ROWS_I; r++) v[r] = *(const f32x4 *)(p.residual + (size_t)(t + r * ROWS_I) * p.r_row + c);
+        for (int r = 0; r < 32 / ROWS_I; r++) {
+            f32x4 z{0.f, 0.f, 0.f, 0.f};
+            if (p.residual && r * ROWS_I < rows) z = *(const f32x4_any *)(p.residual + (size_t)(t + r * ROWS_I) * p.r_row + c);   // all loads together
+            v[r] = z;
+        }
 #pragma unroll
-                for (int r = 0; r < 32 / ROWS_I; r++) v[r] += *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 32 / ROWS_I; r++) v[r] = *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
-            }
-#pragma unroll
-            for (int r = 0; r < 32 / ROWS_I; r++) *(f32x4 *)((float *)p.y + (size_t)(t + r * ROWS_I) * p.y_row + c) = v[r];
-        } else {
+        for (int r = 0; r < 32 / ROWS_I; r++) {
+            v[r] += *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
+            if (r * ROWS_I < rows) *(f32x4_any *)((float *)p.y + (size_t)(t + r * ROWS_I) * p.y_row + c) = v[r];
+        }
+        if (c0 + WN > p.N && p.N % 4) {
 #pragma unroll 1
-            for (int r = 0; r < 32; r += ROWS_I) {
-                const f32x4 v = *(const f32x4 *)(from + r * OUT_ROW);
-                if (t + r < p.T && c < p.N) store4(p, t + r, c, v[0], v[1], v[2], v[3]);
-            }
+            for (int r = 0; r < 32; r += ROWS_I)
+                if (t + r < p.T && c + 4 > p.N && c < p.N) store4(p, t + r, c, *(const f32x4 *)(from + r * OUT_ROW));
         }
     }
 }
