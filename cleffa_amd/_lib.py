@@ -18,7 +18,7 @@ KV_ALIGN = 8
 BLOCK_INTS = 8
 KV8_PAGE, KV8_MAX_SEQ, KV8_MAX_ROWS = 64, 4096, 262143
 KV8_PLAN_STATUS, KV8_PLAN_FAILED = 9, 10
-MX4_BLOCK, MX4_MAX = 32, 1 << 20
+MX4_BLOCK, MX4_MAX, ROTARY_ROWS = 32, 1 << 20, 1 << 25
 ROTARY_SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
 

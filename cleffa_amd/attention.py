@@ -382,6 +382,8 @@ class TextAttention:
             if W.rows != self.row or W.device != dev or (X.rows if isinstance(X, Mx4Matrix) else X.shape[0]) != T:
                 raise ValueError(f"X and W must have {T} and {self.row} rows, on {dev}")
         else:
+            if isinstance(X, Mx4Matrix):
+                raise TypeError("X in 4 bits needs W in 4 bits")
             H = X.shape[1] if X.dim() == 2 else -1
             _check(X, "X", (T, H), torch.bfloat16, dev)
             _check(W, "W", (self.row, H), torch.bfloat16, dev)

@@ -41,12 +41,12 @@ bool launch_ok(const char *what, char *err, size_t errlen) {
 // The compute units of the chips this library is built for (gfx950): forms are chosen for them.
 constexpr int kCus = 256;
 
-// rows * K / 512 workgroups and rows * K / 8192 of them: both below 2^31
+// A launch holds fewer than 2^32 threads: of rows / 16 x K / 512 workgroups of 256, fewer than 2^24.
 bool shape_ok(const char *what, int rows, int K, char *err, size_t errlen) {
     if (rows < 0 || rows > CLEF_HIP_MX4_MAX) return fail(err, errlen, "%s: %d rows, 0 to %d are supported", what, rows, CLEF_HIP_MX4_MAX);
     if (K <= 0 || K > CLEF_HIP_MX4_MAX || K % mx4::BLOCK)
         return fail(err, errlen, "%s: rows of %d values, multiples of %d up to %d are supported", what, K, mx4::BLOCK, CLEF_HIP_MX4_MAX);
-    if ((long)mx4::ceil_div(rows, mx4::ROWS) * mx4::ceil_div(K, mx4::KG) > (1L << 26))
+    if ((long)mx4::ceil_div(rows, mx4::ROWS) * mx4::ceil_div(K, mx4::KG) >= (1L << 24))
         return fail(err, errlen, "%s: %d x %d values are too many", what, rows, K);
     return true;
 }
@@ -55,6 +55,16 @@ bool matrix_ok(const char *what, const uint8_t *codes, const uint8_t *scales, ch
     if (!codes || !scales || !aligned16(codes) || !aligned16(scales))
         return fail(err, errlen, "%s codes and scales must be 16-byte aligned device pointers", what);
     return true;
+}
+
+// Whether the residual is Y itself, or none of its values one of Y's: the other side of it, or other columns of rows of the same length.
+bool apart(const clef_hip_mx4_gemm_args *a) {
+    const uintptr_t y = (uintptr_t)a->y, r = (uintptr_t)a->residual;
+    if (y == r) return a->T == 1 || a->y_row == a->r_row;
+    const uintptr_t y_end = y + 4 * ((size_t)(a->T - 1) * a->y_row + a->N), r_end = r + 4 * ((size_t)(a->T - 1) * a->r_row + a->N);
+    if (r >= y_end || y >= r_end) return true;
+    const long d = ((long)(r - y) / 4 % a->y_row + a->y_row) % a->y_row;
+    return a->T > 1 && a->y_row == a->r_row && (r - y) % 4 == 0 && d >= a->N && d <= a->y_row - a->N;
 }
 
 mx4::Matrix matrix(const uint8_t *codes, const uint8_t *scales, int rows, int K) {
@@ -91,8 +101,13 @@ template <int MT, int NT, int W>
 bool launch_rows16(const mx4::GemmParams &p, hipStream_t s) {
     const long blocks = rows_blocks<MT, NT>(p);
     if (blocks > (W == 8 ? kCus : 2 * kCus)) return false;
-    if (MT == 1 && p.T <= 4) hipLaunchKernelGGL((mx4::mx4_rows16_kernel<1, NT, W, 1>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
-    else hipLaunchKernelGGL((mx4::mx4_rows16_kernel<MT, NT, W, 4 * MT>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
+    if constexpr (MT == 1) {
+        if (p.T <= 4) {
+            hipLaunchKernelGGL((mx4::mx4_rows16_kernel<1, NT, W, 1>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
+            return true;
+        }
+    }
+    hipLaunchKernelGGL((mx4::mx4_rows16_kernel<MT, NT, W, 4 * MT>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
     return true;
 }
 
@@ -122,13 +137,16 @@ void launch4(const mx4::GemmParams &p, hipStream_t s) {
     using Small = mx4::TileCfg<64, 128, 64, 32, 4, 2>;
     using Middle = mx4::TileCfg<128, 128, 64, 64, 4, 2>;
     using Large = mx4::TileCfg<256, 128, 128, 64, 3, 2>;
+    using Square = mx4::TileCfg<256, 256, 128, 64, 4, 1>;    // eight waves, one workgroup a CU
     if (launch_rows<1, 1, 8, 3>(p, s) || launch_rows<1, 2, 8, 3>(p, s) || launch_rows<2, 2, 8, 2>(p, s) || launch_rows<2, 4, 8, 2>(p, s) ||
         launch_rows<4, 4, 8, 2>(p, s))
         return;
-    // rounds of 40 K tiles, us: 256 rows x 14,336 small 16.7, middle 13.7, large 18.6; 512 rows 31.8, 24.7, 23.3; 4,096 rows large 152, middle 174;
-    // 1,160 x 5,120 x 6,144 27.7, 26.6, 26.1, with a residual 32.9, 29.8, 29.5
+    // rounds of 40 K tiles, us: 256 rows x 14,336 small 16.7, middle 13.7, large 18.6, square 26; 512 rows 31.8, 24.7, 23.3; 4,096 rows 227, 173, 150, 144;
+    // 1,160 x 5,120 x 6,144 27.7, 26.6, 26.1, 32, with a residual 32.9, 29.8, 29.5; 2,048 rows 44, 39, 39, 37.5
     const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 22.f, 41.f);
-    if (small <= middle && small <= large) launch_tile<Small>(p, s);
+    const float square = 36.f * (float)((tiles<Square>(p) + kCus - 1) / kCus);
+    if (square < large && square < middle && square < small) launch_tile<Square>(p, s);
+    else if (small <= middle && small <= large) launch_tile<Small>(p, s);
     else if (middle <= large) launch_tile<Middle>(p, s);
     else launch_tile<Large>(p, s);
 }
@@ -217,6 +235,7 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
         return fail(err, errlen, "4-bit product: X must be 16-byte aligned, its row %ld >= %d and a multiple of 8", a->x_row, a->K);
     if (!a->y || ((uintptr_t)a->y & (a->y_type == CLEF_HIP_GEMM_Y_BF16 ? 1u : 3u)) || ((uintptr_t)a->residual & 3u))
         return fail(err, errlen, "4-bit product: Y and the residual must be aligned device pointers");
+    if (a->residual && !apart(a)) return fail(err, errlen, "4-bit product: the residual may be Y itself, but not overlap it otherwise");
     mx4::GemmParams p;
     p.w = matrix(a->w_codes, a->w_scales, a->N, a->K);
     p.x = matrix(a->x_codes, a->x_scales, a->T, a->K);

@@ -6,6 +6,12 @@
 // Scales of four K tiles go to LDS together and from there into a register for each operand, of which the instruction
 // takes a byte. So the loop takes four K tiles at a time, one straight line of code: over branches the compiler would move the
 // products behind the waits.
+//
+// Bound by the matrix units and LDS together. A K tile of 256 x 256 is 1,024 clocks of a CU's products; its waves' operands are 96 KB
+// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 144 us, 4.2 PFLOP/s: the products
+// alone, on such data, ran at 6.3 in a loop without any loads, the chip at 1.8 of its 2.4 GHz for its power. Tiles of 256 x 128, two
+// workgroups a CU: 150 us; 128 x 128: 173; four waves of 128 x 128, which read a third less of LDS but have nothing that runs while
+// they wait: 149.
 #pragma once
 #include <utility>
 
@@ -55,20 +61,17 @@ __device__ __forceinline__ void lds_wait(u32x4 (&r)[F]) {
 }
 template <int F>
 __device__ __forceinline__ void lds_wait(u32x4 (&r)[F], unsigned (&s)[2][F]) {
+    static_assert(F == 3 || F == 4 || F == 6, "operands of a wave's tile");
     if constexpr (F == 3)
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[1][0]), "+v"(s[1][1]),
                      "+v"(s[1][2])::"memory");
     else if constexpr (F == 4)
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[0][3]),
                      "+v"(s[1][0]), "+v"(s[1][1]), "+v"(s[1][2]), "+v"(s[1][3])::"memory");
-    else if constexpr (F == 6)
+    else
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(r[4]), "+v"(r[5]), "+v"(s[0][0]), "+v"(s[0][1]),
                      "+v"(s[0][2]), "+v"(s[0][3]), "+v"(s[0][4]), "+v"(s[0][5]), "+v"(s[1][0]), "+v"(s[1][1]), "+v"(s[1][2]), "+v"(s[1][3]),
                      "+v"(s[1][4]), "+v"(s[1][5])::"memory");
-    else
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3]), "+v"(r[4]), "+v"(r[5]), "+v"(r[6]), "+v"(r[7]), "+v"(s[0][0]),
-                     "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[0][3]), "+v"(s[0][4]), "+v"(s[0][5]), "+v"(s[0][6]), "+v"(s[0][7]), "+v"(s[1][0]),
-                     "+v"(s[1][1]), "+v"(s[1][2]), "+v"(s[1][3]), "+v"(s[1][4]), "+v"(s[1][5]), "+v"(s[1][6]), "+v"(s[1][7])::"memory");
 }
 
 // A wave's outputs, rows t0 .. and columns c0 ..: lane l's accumulators of a 32 x 32 part are columns 8 (e / 4) + 4 (l / 32) + e % 4 of row
@@ -231,10 +234,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES / 4 * C::PER_CU) void mx4_tile
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(r[j]), operand(r[NT + i]), acc[i][j], 4, 4, pos, (int)s[h][j], pos, (int)s[h][NT + i]);
     };
     // Products FROM .. of a half, reads of the next half's operands between them, so that the matrix unit has work while
-    // reads are issued and in flight; and fills F0 .. F1, which issue as fast as addresses are taken, 16 clocks each for all of
-    // the CU's waves.
+    // reads are issued and in flight (behind the first half of the products: there is time left for them to arrive); and fills F0 .. F1,
+    // which issue as fast as addresses are taken, 16 clocks each for all of the CU's waves.
     auto step = [&](auto POS, u32x4 (&now)[FR], auto H, auto FROM, u32x4 (&next)[FR], unsigned stage, auto H_NEXT, int fill_kt, unsigned fill_stage, auto F0, auto F1) CLEF_INLINE {
-        constexpr int from = decltype(FROM)::value, n = P - from, per = (FR + n - 1) / n, f0 = decltype(F0)::value, nf = decltype(F1)::value - f0;
+        constexpr int from = decltype(FROM)::value, n = P - from, early = n > 1 ? n / 2 : 1, per = (FR + early - 1) / early, f0 = decltype(F0)::value, nf = decltype(F1)::value - f0;
         for_each<n>([&](auto Q) CLEF_INLINE {
             constexpr int q = decltype(Q)::value;
             product(now, POS, H, std::integral_constant<int, q + from>{});

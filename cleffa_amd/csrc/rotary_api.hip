@@ -125,7 +125,7 @@ bool clef_hip_rotary_freqs(int n_rot, double theta, int scaling, double factor, 
 
 bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, size_t errlen) {
     if (!a) return fail(err, errlen, "null rotary arguments");
-    if (a->T < 0) return fail(err, errlen, "rotary: %d rows", a->T);
+    if (a->T < 0 || a->T > CLEF_HIP_ROTARY_ROWS) return fail(err, errlen, "rotary: %d rows, 0 to %d are supported", a->T, CLEF_HIP_ROTARY_ROWS);
     if (a->hd <= 0 || a->hd > rotary::kMaxHd || a->hd % 2) return fail(err, errlen, "rotary: head dim %d must be even, 2 to %d", a->hd, rotary::kMaxHd);
     if (a->n_rot <= 0 || a->n_rot % 2 || a->n_rot > a->hd) return fail(err, errlen, "rotary: n_rot %d must be even, 2 to the head dim", a->n_rot);
     if (a->layout != CLEF_HIP_ROTARY_HALF && a->layout != CLEF_HIP_ROTARY_INTERLEAVED) return fail(err, errlen, "rotary: bad layout %d", a->layout);

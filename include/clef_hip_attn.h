@@ -534,7 +534,7 @@ bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scale
 /* Y[T][N] = X[T][K] . W[N][K]^T (+ residual), W in 4 bits, X in 4 bits (x_codes, x_scales) or in bf16 (x_bf16, its rows x_row
  * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly, and summed
  * in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
- * be Y itself. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W. The sums' order
+ * be Y itself (the same rows), but not overlap it otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W. The sums' order
  * depends on the sizes alone: results do not change from run to run. No workspace. */
 typedef struct {
     int T, N, K, y_type;
@@ -565,12 +565,14 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
 #define CLEF_HIP_ROTARY_PARTS 3
 #define CLEF_HIP_ROTARY_HALF 0
 #define CLEF_HIP_ROTARY_INTERLEAVED 1
+#define CLEF_HIP_ROTARY_ROWS 33554432   /* of a call */
 bool clef_hip_rotary_freqs(int n_rot, double theta, int scaling, double factor, double original, double low, double high, double *freq,
                            char *err, size_t errlen);
 typedef struct {
     int heads;                /* 0: none */
     const void *x;            /* head h of row t starts at x + t * x_row + h * x_head elements */
-    void *out;                /* may be x with the same strides; without a norm only the turned dims are then touched */
+    void *out;                /* may be x with the same strides; without a norm only the turned dims are then touched. Else no
+                                 output overlaps an input, or the other output */
     long x_row, x_head, out_row, out_head;
     const float *norm;        /* [hd] f32, as given (already 1 + w), or NULL */
 } clef_hip_rotary_heads;

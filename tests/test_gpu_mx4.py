@@ -170,7 +170,7 @@ SHAPES = [(1, 1, 32), (1, 16, 128), (1, 100, 5120), (1, 517, 96), (2, 640, 544),
           (33, 64, 640), (45, 1024, 1024), (64, 130, 416), (65, 200, 3200), (127, 255, 544), (128, 384, 256), (200, 96, 1120), (257, 513, 768),
           (300, 1000, 672), (520, 777, 2080), (1025, 515, 1536),
           # the larger tiles of both forms, K of one tile to three groups, and between
-          (520, 2105, 32), (257, 4099, 544), (1025, 2050, 288), (1025, 2047, 1120), (1025, 4100, 416), (700, 6150, 1056), (2000, 6390, 160), (130, 14300, 672), (2048, 6400, 512)]
+          (520, 2105, 32), (257, 4099, 544), (1025, 2050, 288), (1025, 2047, 1120), (1025, 4100, 416), (700, 6150, 1056), (2000, 6390, 160), (130, 14300, 672), (2048, 6400, 512), (1900, 6301, 1696)]
 
 
 @pytest.mark.parametrize("T,N,K", SHAPES)

@@ -5,12 +5,13 @@ import math
 import re
 import subprocess
 from pathlib import Path
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
 import torch
 
-from cleffa_amd import Mx4Matrix, Rotary, _lib, mx4_gemm
+from cleffa_amd import Mx4Matrix, Rotary, TextAttention, _lib, mx4_gemm
 from tests import mx4_ref
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "clef_hip_attn.h"
@@ -40,7 +41,7 @@ def test_struct_layouts(name, cls, tmp_path):
 
 def test_constants_match_the_header():
     text = HEADER.read_text()
-    for name, value in (("MX4_BLOCK", _lib.MX4_BLOCK), ("MX4_MAX", _lib.MX4_MAX), ("ROTARY_LINEAR", _lib.ROTARY_SCALINGS["linear"]),
+    for name, value in (("MX4_BLOCK", _lib.MX4_BLOCK), ("MX4_MAX", _lib.MX4_MAX), ("ROTARY_ROWS", _lib.ROTARY_ROWS), ("ROTARY_LINEAR", _lib.ROTARY_SCALINGS["linear"]),
                         ("ROTARY_BASE", _lib.ROTARY_SCALINGS["base"]), ("ROTARY_PARTS", _lib.ROTARY_SCALINGS["parts"]),
                         ("ROTARY_HALF", _lib.ROTARY_LAYOUTS["half"]), ("ROTARY_INTERLEAVED", _lib.ROTARY_LAYOUTS["interleaved"])):
         assert int(re.search(rf"#define CLEF_HIP_{name} (\d+)", text).group(1)) == value
@@ -101,6 +102,19 @@ def test_product_refusals(over, msg):
     _refused(_lib.load().clef_hip_mx4_gemm, None, "null")
 
 
+@pytest.mark.parametrize("at,r_row,y_row,ok", [
+    (0, 200, 200, True), (0, 204, 200, False), (400, 200, 200, True), (404, 200, 200, False), (396, 200, 200, False), (-400, 200, 200, True), (-396, 200, 200, False),
+    (4 * 200 * 7 + 400, 200, 200, True), (4 * 200 * 7 + 396, 200, 200, False), (4 * 200 * 7 + 396, 100, 200, False), (4 * 200 * 7 + 400, 100, 200, True), (-4 * 800, 100, 200, True),
+    (-4 * 799, 100, 200, False), (1000, 200, 200, False), (1200, 200, 200, True), (1200, 200, 201, False),
+])
+def test_residual_overlap(at, r_row, y_row, ok):
+    """The residual is Y, lies apart from it, or between its rows; a call that passes fails at the next check, X's."""
+    a = _lib.Mx4GemmArgs(8, 100, 64, 0, FAKE, FAKE, FAKE, FAKE, None, 0, y_row, r_row, 1 << 20, (1 << 20) + at)
+    if ok:
+        a.x_codes = ODD
+    _refused(_lib.load().clef_hip_mx4_gemm, a, "X codes" if ok else "overlap")
+
+
 def test_no_rows_are_no_work():
     lib, err = _lib.load(), _err()
     assert lib.clef_hip_mx4_gemm(ctypes.byref(_lib.Mx4GemmArgs(0, 8, 32, 0, None, None, None, None, FAKE, 32, 8, 0, None, None)), None, err, 256)
@@ -125,7 +139,7 @@ def _rotary_args(**over):
     (dict(n_rot=63), "n_rot"), (dict(layout=2), "layout"), (dict(axes=0), "axes"), (dict(axes=5), "axes"), (dict(type=3), "type"), (dict(eps=-1.0), "eps"),
     (dict(magnitude=math.inf), "magnitude"), (dict(pos=None), "pos"), (dict(freq=None), "freq"), (dict(heads=-1), "heads"), (dict(x=None), "aligned"),
     (dict(out=ODD), "aligned"), (dict(type=2, x=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(norm=ODD), "aligned"), (dict(out_head=64, x_head=64), "overlap"),
-    (dict(out_row=256, x_row=256), "overlap"), (dict(x_row=-512), "negative"), (dict(x_row=1024), "same strides"), (dict(x_head=256), "same strides"),
+    (dict(T=_lib.ROTARY_ROWS + 1), "rows"), (dict(out_row=256, x_row=256), "overlap"), (dict(x_row=-512), "negative"), (dict(x_row=1024), "same strides"), (dict(x_head=256), "same strides"),
 ])
 def test_rotary_refusals(over, msg):
     _refused(_lib.load().clef_hip_rotary, _rotary_args(**over), msg)
@@ -172,6 +186,12 @@ def test_python_refusals():
                  lambda: r.apply(q, None, pos, q_norm=torch.ones(32)), lambda: r.apply(q[0], None, pos), lambda: r.apply(q.transpose(1, 2), None, pos)):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+def test_project_refuses_mixed_operands():
+    att = SimpleNamespace(device=torch.device("cpu"), row=2048)
+    with pytest.raises(TypeError, match="4 bits"):
+        TextAttention.project(att, Mx4Matrix(8, 64, device="cpu"), torch.zeros(att.row, 64, dtype=torch.bfloat16), SimpleNamespace(T=8))
 
 
 def test_reference_grid():
