@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace clef_hip {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -30,5 +32,25 @@ __device__ __forceinline__ uint16_t f2bf(float a) {
     __bf16 v = (__bf16)a;
     return __builtin_bit_cast(uint16_t, v);
 }
+
+// Stores of rows that a wave writes in order: past the caches where rows begin at whole lines of 128 bytes, so that the caches
+// keep what is read. (Parts of lines would each go to memory by themselves.) The statements keep the compiler from making one of
+// the two ways, and that the ordinary one.
+template <typename F>
+__device__ __forceinline__ void with_past(bool past, F &&f) {
+    if (past) {
+        asm volatile("; past the caches");
+        f(std::true_type{});
+        asm volatile("");
+    } else {
+        f(std::false_type{});
+    }
+}
+template <typename PAST, typename V, typename T>
+__device__ __forceinline__ void store_past(PAST, V *to, T v) {
+    if constexpr (PAST::value) __builtin_nontemporal_store((V)v, to);
+    else *to = v;
+}
+inline bool whole_lines(const void *base, long row_bytes) { return (((uintptr_t)base | (uintptr_t)row_bytes) & 127u) == 0; }
 
 }  // namespace clef_hip

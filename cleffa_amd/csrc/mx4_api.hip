@@ -71,12 +71,9 @@ mx4::Matrix matrix(const uint8_t *codes, const uint8_t *scales, int rows, int K)
     return mx4::Matrix{codes, scales, rows, mx4::ceil_div(K, mx4::KT), mx4::ceil_div(K, mx4::KG)};
 }
 
-// Two row tiles a workgroup where that leaves enough of them (4,096 x 6,144: 18.1 us with one, 17.5).
 template <int TYPE>
 void launch_quantise(const mx4::QuantParams &p, hipStream_t s) {
-    const long rt = mx4::ceil_div(p.rows, mx4::ROWS);
-    if (rt * p.kgroups < 8L * kCus) hipLaunchKernelGGL((mx4::mx4_quantise_kernel<TYPE, 1>), dim3((unsigned)(rt * p.kgroups)), dim3(mx4::kQuantThreads), 0, s, p);
-    else hipLaunchKernelGGL((mx4::mx4_quantise_kernel<TYPE, 2>), dim3((unsigned)((rt + 1) / 2 * p.kgroups)), dim3(mx4::kQuantThreads), 0, s, p);
+    hipLaunchKernelGGL(mx4::mx4_quantise_kernel<TYPE>, dim3((unsigned)(mx4::ceil_div(p.rows, mx4::ROWS) * p.kgroups)), dim3(mx4::kQuantThreads), 0, s, p);
 }
 
 // The forms of the product. Where a form's workgroups make no more than one for each CU, its K loop is the time, and the smallest
@@ -183,7 +180,7 @@ bool clef_hip_mx4_quantise(const clef_hip_mx4_rows_args *a, void *stream, char *
     if (a->rows == 0) return true;
     if (!matrix_ok("quantise:", a->codes, a->scales, err, errlen)) return false;
     if (!a->x || !aligned16(a->x)) return fail(err, errlen, "quantise: x must be a 16-byte aligned device pointer");
-    mx4::QuantParams p{a->x, nullptr, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row};
+    mx4::QuantParams p{a->x, nullptr, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row, false};
     if (a->type == CLEF_HIP_OUT_BF16) launch_quantise<mx4::X_BF16>(p, (hipStream_t)stream);
     else if (a->type == CLEF_HIP_OUT_F16) launch_quantise<mx4::X_F16>(p, (hipStream_t)stream);
     else launch_quantise<mx4::X_F32>(p, (hipStream_t)stream);
@@ -198,7 +195,8 @@ bool clef_hip_mx4_values(const clef_hip_mx4_rows_args *a, void *stream, char *er
     if (a->rows == 0) return true;
     if (!matrix_ok("values:", a->codes, a->scales, err, errlen)) return false;
     if (!a->x || !aligned16(a->x)) return fail(err, errlen, "values: x must be a 16-byte aligned device pointer");
-    mx4::QuantParams p{nullptr, a->x, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row};
+    mx4::QuantParams p{nullptr, a->x, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row,
+                       whole_lines(a->x, a->row * (a->type == CLEF_HIP_OUT_F32 ? 4 : 2))};
     const dim3 grid((unsigned)((long)mx4::ceil_div(a->rows, mx4::ROWS) * p.kgroups)), block(mx4::kQuantThreads);
     if (a->type == CLEF_HIP_OUT_BF16) hipLaunchKernelGGL(mx4::mx4_values_kernel<false>, grid, block, 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL(mx4::mx4_values_kernel<true>, grid, block, 0, (hipStream_t)stream, p);
@@ -241,6 +239,7 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     p.x = matrix(a->x_codes, a->x_scales, a->T, a->K);
     p.xb = a->x_bf16; p.x_row = a->x_row; p.y = a->y; p.y_row = a->y_row; p.residual = a->residual; p.r_row = a->r_row;
     p.T = a->T; p.N = a->N; p.K = a->K; p.y_bf16 = a->y_type == CLEF_HIP_GEMM_Y_BF16;
+    p.past = whole_lines(a->y, a->y_row * (p.y_bf16 ? 2 : 4));
     if (p.xb) launch16(p, (hipStream_t)stream);
     else launch4(p, (hipStream_t)stream);
     return launch_ok("mx4_gemm", err, errlen);

@@ -43,6 +43,7 @@ struct QuantParams {
     uint8_t *codes, *scales;
     int rows, K, ktiles, kgroups;
     long row;                 // elements between rows of x or y
+    bool past;                // of y: store_past
 };
 
 struct PackParams {
@@ -58,6 +59,7 @@ struct GemmParams {
     void *y;
     const float *residual;
     int T, N, K, y_bf16;
+    bool past;                // of y: store_past
 };
 
 // Vectors at any element's address: the memory takes them, and odd row strides keep their wide stores.

@@ -67,81 +67,86 @@ __device__ __forceinline__ unsigned quad_max(unsigned m) {
 
 // A workgroup makes 16 rows x 512 columns, each of its four waves a tile of 16 x 128: four loads of 4 rows x 256 bytes, a
 // block's 32 values in four neighbouring lanes. Codes go through LDS, so that a tile's 1 KB is stored in a row.
-// Bound by memory: 4,096 x 6,144 f16 values 17.5 us, 3.6 TB/s of what it reads and writes (a large copy: 4.9).
+// Bound by memory: 4,096 x 6,144 f16 values 11.0 us one call behind the other, 5.8 TB/s of what it reads and writes; reading alone takes
+// 8.0. Two row tiles a workgroup, for more loads in flight, took 11.5.
 constexpr int kQuantThreads = 256;
-// RT: row tiles of a workgroup, whose loads go out together
-template <int TYPE, int RT>
+template <int TYPE>
 __global__ __launch_bounds__(kQuantThreads) void mx4_quantise_kernel(QuantParams p) {
-    __shared__ __attribute__((aligned(16))) uint8_t sc[RT][GROUP_BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t cd[RT][4 * TILE_BYTES];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int rt0 = blockIdx.x / p.kgroups * RT, kg = blockIdx.x % p.kgroups, kt = 4 * kg + wave;
-    const int c = lane & 15, g = c >> 2;
-    const int k = kt * KT + 8 * c;
-    Values<TYPE> x[RT][4];
-#pragma unroll
-    for (int n = 0; n < RT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = ROWS * (rt0 + n) + 4 * i + (lane >> 4);
-            Values<TYPE> zero{}, in = zero;
-            if (t < p.rows && k < p.K) in = load8<TYPE>(p.x, (size_t)t * p.row + k);
-            x[n][i] = in;
-        }
-#pragma unroll
-    for (int n = 0; n < RT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = 4 * i + (lane >> 4);
-            float v[8];
-            values8<TYPE>(x[n][i], v);
-            unsigned m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-            const int s = scale_byte(quad_max(m));
-            *(unsigned *)(cd[n] + wave * TILE_BYTES + 16 * (ROWS * g + r) + 4 * (c & 3)) = s == kNanScale ? 0u : to_codes(v, scale_value(s));
-            if ((c & 3) == 0) sc[n][4 * (ROWS * g + r) + wave] = (uint8_t)s;
-        }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < RT; n++) {
-        if (ROWS * (rt0 + n) + (lane & 15) >= p.rows) return;       // lane l now has row l % 16
-        const size_t rt = rt0 + n;
-        if (kt < p.ktiles) *(u32x4 *)(p.codes + (rt * p.ktiles + kt) * TILE_BYTES + 16 * lane) = *(const u32x4 *)(cd[n] + wave * TILE_BYTES + 16 * lane);
-        if (wave == 0) *(unsigned *)(p.scales + (rt * p.kgroups + kg) * GROUP_BYTES + 4 * lane) = *(const unsigned *)(sc[n] + 4 * lane);
-    }
-}
-
-// The values that codes stand for; the same split.
-template <bool F32>
-__global__ __launch_bounds__(kQuantThreads) void mx4_values_kernel(QuantParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t sc[GROUP_BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t cd[4 * TILE_BYTES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int rt = blockIdx.x / p.kgroups, kg = blockIdx.x % p.kgroups, kt = 4 * kg + wave;
     const int c = lane & 15, g = c >> 2;
     const int k = kt * KT + 8 * c;
-    if (k >= p.K) return;
+    Values<TYPE> x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int r = 4 * i + (lane >> 4), t = ROWS * rt + r;
-        if (t >= p.rows) continue;
-        const unsigned w = *(const unsigned *)(p.codes + ((size_t)rt * p.ktiles + kt) * TILE_BYTES + 16 * (ROWS * g + r) + 4 * (c & 3));
-        const float s = scale_value(p.scales[((size_t)rt * p.kgroups + kg) * GROUP_BYTES + 4 * (ROWS * g + r) + wave]);
-        if constexpr (F32) {
-            typedef __attribute__((ext_vector_type(2))) float f32x2;
-            const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-            const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-            float *y = (float *)p.y + (size_t)t * p.row + k;
-            *(float4 *)y = float4{a[0], a[1], b[0], b[1]};
-            *(float4 *)(y + 4) = float4{d[0], d[1], e[0], e[1]};
-        } else {
-            u32x4 o;
-            o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-            o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-            o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-            o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
-            *(u32x4 *)((uint16_t *)p.y + (size_t)t * p.row + k) = o;
-        }
+        const int t = ROWS * rt + 4 * i + (lane >> 4);
+        Values<TYPE> zero{}, in = zero;
+        if (t < p.rows && k < p.K) in = load8<TYPE>(p.x, (size_t)t * p.row + k);
+        x[i] = in;
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = 4 * i + (lane >> 4);
+        float v[8];
+        values8<TYPE>(x[i], v);
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        const int s = scale_byte(quad_max(m));
+        *(unsigned *)(cd + wave * TILE_BYTES + 16 * (ROWS * g + r) + 4 * (c & 3)) = s == kNanScale ? 0u : to_codes(v, scale_value(s));
+        if ((c & 3) == 0) sc[4 * (ROWS * g + r) + wave] = (uint8_t)s;
+    }
+    __syncthreads();
+    if (ROWS * rt + (lane & 15) >= p.rows) return;       // lane l now has row l % 16
+    if (kt < p.ktiles) *(u32x4 *)(p.codes + ((size_t)rt * p.ktiles + kt) * TILE_BYTES + 16 * lane) = *(const u32x4 *)(cd + wave * TILE_BYTES + 16 * lane);
+    if (wave == 0) *(unsigned *)(p.scales + ((size_t)rt * p.kgroups + kg) * GROUP_BYTES + 4 * lane) = *(const unsigned *)(sc + 4 * lane);
+}
+
+// The values that codes stand for; the same split. Bound by memory: four times as many bytes out as in, stored past the caches, which
+// keep what was there (4,096 x 6,144 to bf16 and the quantisation ahead of it 26.6 us with ordinary stores, 21.5 with these).
+template <bool F32>
+__global__ __launch_bounds__(kQuantThreads) void mx4_values_kernel(QuantParams p) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int rt = blockIdx.x / p.kgroups, kg = blockIdx.x % p.kgroups, kt = 4 * kg + wave;
+    // a lane's values of a row: eight of bf16, or two runs of four of f32, 64 apart, so that 16 lanes store whole lines (4,096 x 5,152 17 us; with
+    // eight in a row, half of each line a store, 31)
+    constexpr int RUNS = F32 ? 2 : 1, V = F32 ? 4 : 8;
+    const int c = lane & 15, r0 = lane >> 4;
+    unsigned w[4][RUNS];
+    float s[4][RUNS];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < RUNS; j++) {
+            const int r = 4 * i + r0, k = 64 * j + V * c, place = ROWS * (k / BLOCK) + r;     // in the K tile
+            const bool in = ROWS * rt + r < p.rows && KT * kt + k < p.K;
+            const uint8_t *codes = p.codes + ((size_t)rt * p.ktiles + kt) * TILE_BYTES + 16 * place + k % BLOCK / 2;
+            w[i][j] = !in ? 0u : F32 ? *(const uint16_t *)codes : *(const unsigned *)codes;
+            s[i][j] = scale_value(in ? p.scales[((size_t)rt * p.kgroups + kg) * GROUP_BYTES + 4 * place + wave] : 0);
+        }
+    with_past(p.past, [&](auto PAST) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < RUNS; j++) {
+                const int t = ROWS * rt + 4 * i + r0, k = KT * kt + 64 * j + V * c;
+                if (t >= p.rows || k >= p.K) continue;
+                if constexpr (F32) {
+                    typedef __attribute__((ext_vector_type(2))) float f32x2;
+                    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j], s[i][j], 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j], s[i][j], 1);
+                    store_past(PAST, (f32x4 *)((float *)p.y + (size_t)t * p.row + k), f32x4{a[0], a[1], b[0], b[1]});
+                } else {
+                    u32x4 o;
+                    o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i][j], s[i][j], 0));
+                    o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i][j], s[i][j], 1));
+                    o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i][j], s[i][j], 2));
+                    o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i][j], s[i][j], 3));
+                    store_past(PAST, (u32x4 *)((uint16_t *)p.y + (size_t)t * p.row + k), o);
+                }
+            }
+    });
 }
 
 // Flat codes and scales into this layout (TO), or back: a thread a block. Blocks beyond K become 0.

@@ -8,10 +8,10 @@
 // products behind the waits.
 //
 // Bound by the matrix units and LDS together. A K tile of 256 x 256 is 1,024 clocks of a CU's products; its waves' operands are 96 KB
-// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 144 us, 4.2 PFLOP/s: the products
+// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 140 us, 4.3 PFLOP/s: the products
 // alone, on such data, ran at 6.3 in a loop without any loads, the chip at 1.8 of its 2.4 GHz for its power. Tiles of 256 x 128, two
-// workgroups a CU: 150 us; 128 x 128: 173; four waves of 128 x 128, which read a third less of LDS but have nothing that runs while
-// they wait: 149.
+// workgroups a CU, took 150 us where these took 144; 128 x 128: 173; four waves of 128 x 128, which read a third less of LDS but have
+// nothing that runs while they wait: 149.
 #pragma once
 #include <utility>
 
@@ -75,7 +75,9 @@ __device__ __forceinline__ void lds_wait(u32x4 (&r)[F], unsigned (&s)[2][F]) {
 }
 
 // A wave's outputs, rows t0 .. and columns c0 ..: lane l's accumulators of a 32 x 32 part are columns 8 (e / 4) + 4 (l / 32) + e % 4 of row
-// l % 32. 32 rows at a time go through `mine`, LDS of the wave's own, so that stores take whole lines.
+// l % 32. 32 rows at a time go through `mine`, LDS of the wave's own, so that stores take whole lines, past the caches where rows of Y
+// begin at them: 4,096 x 14,336 x 5,120 148 us with ordinary stores, 140 past the caches, which W and X then have to themselves; 2,000 x 6,389
+// x 160, where they do not, 12.3 and 16.6.
 constexpr int out_row(int NT) { return 32 * NT * 4 + 16; }
 template <int MT, int NT>
 __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&acc)[MT][NT], uint8_t *mine, int t_first, int c0) {
@@ -97,12 +99,14 @@ __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&a
             const uint8_t *from = mine + lane / LANES * OUT_ROW + 32 * (lane % LANES);
             uint16_t *to = (uint16_t *)p.y + (size_t)t * p.y_row + c;
             const int rows = c + 8 <= p.N ? p.T - t : 0;
+            with_past(p.past, [&](auto PAST) CLEF_INLINE {
 #pragma unroll
-            for (int r = 0; r < 32; r += ROWS_I) {
-                const f32x4 a = *(const f32x4 *)(from + r * OUT_ROW), b = *(const f32x4 *)(from + r * OUT_ROW + 16);
-                if (r < rows)
-                    *(u32x4_any *)(to + (size_t)r * p.y_row) = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
-            }
+                for (int r = 0; r < 32; r += ROWS_I) {
+                    const f32x4 a = *(const f32x4 *)(from + r * OUT_ROW), b = *(const f32x4 *)(from + r * OUT_ROW + 16);
+                    if (r < rows)
+                        store_past(PAST, (u32x4_any *)(to + (size_t)r * p.y_row), u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])});
+                }
+            });
             if (c0 + WN > p.N && p.N % 8) {
 #pragma unroll 1
                 for (int r = 0; r < 32; r += ROWS_I)
@@ -123,10 +127,12 @@ __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&a
             v[r] = z;
         }
 #pragma unroll
-        for (int r = 0; r < 32 / ROWS_I; r++) {
-            v[r] += *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
-            if (r * ROWS_I < rows) *(f32x4_any *)((float *)p.y + (size_t)(t + r * ROWS_I) * p.y_row + c) = v[r];
-        }
+        for (int r = 0; r < 32 / ROWS_I; r++) v[r] += *(const f32x4 *)(from + r * ROWS_I * OUT_ROW);
+        with_past(p.past, [&](auto PAST) CLEF_INLINE {
+#pragma unroll
+            for (int r = 0; r < 32 / ROWS_I; r++)
+                if (r * ROWS_I < rows) store_past(PAST, (f32x4_any *)((float *)p.y + (size_t)(t + r * ROWS_I) * p.y_row + c), v[r]);
+        });
         if (c0 + WN > p.N && p.N % 4) {
 #pragma unroll 1
             for (int r = 0; r < 32; r += ROWS_I)

@@ -54,8 +54,9 @@ bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size) {
     return T <= 1 || (g->x_row % v == 0 && g->out_row % v == 0);
 }
 
-rotary::Group group(const clef_hip_rotary_heads *g) {
-    return rotary::Group{g->x, g->out, g->norm, g->x_row, g->x_head, g->out_row, g->out_head, g->heads};
+rotary::Group group(const clef_hip_rotary_heads *g, int size) {
+    return rotary::Group{g->x, g->out, g->norm, g->x_row, g->x_head, g->out_row, g->out_head, g->heads,
+                         whole_lines(g->out, g->out_row * size) && whole_lines(g->out, g->out_head * size)};
 }
 
 template <int TYPE, int V, int L, int I, bool HALF>
@@ -137,7 +138,7 @@ bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, siz
     if (a->T == 0 || a->q.heads + a->k.heads == 0) return true;
     if (!a->pos || !a->freq || ((uintptr_t)a->pos & 3u) || ((uintptr_t)a->freq & 7u)) return fail(err, errlen, "rotary: pos and freq must be aligned device pointers");
     rotary::Params p;
-    p.q = group(&a->q); p.k = group(&a->k); p.pos = a->pos; p.freq = a->freq;
+    p.q = group(&a->q, size); p.k = group(&a->k, size); p.pos = a->pos; p.freq = a->freq;
     p.T = a->T; p.hd = a->hd; p.n_rot = a->n_rot; p.half = a->layout == CLEF_HIP_ROTARY_HALF; p.axes = a->axes;
     p.eps = a->eps; p.magnitude = a->magnitude;
     // the longest runs that heads divide into and that pointers and strides allow
