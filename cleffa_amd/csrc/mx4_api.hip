@@ -138,8 +138,8 @@ void launch4(const mx4::GemmParams &p, hipStream_t s) {
     if (launch_rows<1, 1, 8, 3>(p, s) || launch_rows<1, 2, 8, 3>(p, s) || launch_rows<2, 2, 8, 2>(p, s) || launch_rows<2, 4, 8, 2>(p, s) ||
         launch_rows<4, 4, 8, 2>(p, s))
         return;
-    // rounds of 40 K tiles, us: 256 rows x 14,336 small 16.7, middle 13.7, large 18.6, square 26; 512 rows 31.8, 24.7, 23.3; 4,096 rows 227, 173, 150, 144;
-    // 1,160 x 5,120 x 6,144 27.7, 26.6, 26.1, 32, with a residual 32.9, 29.8, 29.5; 2,048 rows 44, 39, 39, 37.5
+    // rounds of 40 K tiles, us: 256 rows x 14,336 small 17.2, middle 14.4, large 18.1, square 25.5; 512 rows 32, 26, 23.5, 28; 2,048 rows large 73, square 70;
+    // 4,096 rows 227, 163, 145 and 149, 149; 3,000 x 10,240 x 4,096 large 61.5, square 59.8; 1,160 x 5,120 x 6,144 27.7, 26.6, 25.8, 33; 2,048 rows 46, 41, 36 to 42, 38
     const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 22.f, 41.f);
     const float square = 36.f * (float)((tiles<Square>(p) + kCus - 1) / kCus);
     if (square < large && square < middle && square < small) launch_tile<Square>(p, s);
