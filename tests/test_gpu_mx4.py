@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from cleffa_amd import Mx4Matrix, mx4_gemm
+from cleffa_amd import Mx4Matrix, _lib, mx4_gemm
 from tests import mx4_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -170,7 +170,7 @@ SHAPES = [(1, 1, 32), (1, 16, 128), (1, 100, 5120), (1, 517, 96), (2, 640, 544),
           (33, 64, 640), (45, 1024, 1024), (64, 130, 416), (65, 200, 3200), (127, 255, 544), (128, 384, 256), (200, 96, 1120), (257, 513, 768),
           (300, 1000, 672), (520, 777, 2080), (1025, 515, 1536),
           # the larger tiles of both forms, K of one tile to three groups, and between
-          (520, 2105, 32), (257, 4099, 544), (1025, 2050, 288), (1025, 2047, 1120), (1025, 4100, 416), (700, 6150, 1056), (2000, 6390, 160), (130, 14300, 672), (2048, 6400, 512), (1900, 6301, 1696)]
+          (520, 2105, 32), (257, 4099, 544), (1025, 2050, 288), (1025, 2047, 1120), (1025, 4100, 416), (700, 6150, 1056), (2000, 6390, 160), (130, 14300, 672), (2048, 6400, 512), (1900, 6301, 1696), (1100, 5120, 288)]
 
 
 @pytest.mark.parametrize("T,N,K", SHAPES)
@@ -297,6 +297,67 @@ def test_quantise_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert np.array_equal(_np(v), ref.values(*ref.quantise(_np(y))))
+
+
+@pytest.mark.parametrize("bf", [False, True], ids=["x4", "xbf16"])
+def test_two_streams(bf):
+    """Calls that overlap on two streams give what they give alone."""
+    calls, alone, out = [], [], []
+    for T, N, K, seed in ((300, 2050, 1056, 1), (40, 5000, 2080, 2)):
+        X, W = _operands(T, N, K, seed, bf)[:2]
+        calls.append((X, W))
+        alone.append(mx4_gemm(X, W, out="f32"))
+        out.append([torch.zeros_like(alone[-1]) for _ in range(8)])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for (X, W), y, s in zip(calls, out, streams):
+            mx4_gemm(X, W, Y=y[i], stream=s)
+    torch.cuda.synchronize()
+    for want, ys in zip(alone, out):
+        assert all(torch.equal(y, want) for y in ys)
+
+
+def test_outputs_beyond_32_bits():
+    """Y of more than 2^32 bytes, with rows of X in both types: the rows at both ends and across 2^31 and 2^32 bytes as a call on them alone."""
+    T, N, K = _lib.MX4_MAX, 2080, 64
+    _say("large Y", T, N, K)
+    x = torch.randn(T, K, device="cuda", dtype=torch.bfloat16)
+    W, X = Mx4Matrix.quantised(torch.randn(N, K, device="cuda")), Mx4Matrix.quantised(x)
+    at = [0, (1 << 31) // (2 * N) // 16 * 16, (1 << 32) // (2 * N) // 16 * 16, T - 64]
+    for big in (X, x):
+        y = mx4_gemm(big, W)
+        for t in at:
+            part = x[t:t + 64].contiguous()
+            want = mx4_gemm(part if big is x else Mx4Matrix.quantised(part), W, out="f32").double()
+            got = y[t:t + 64].double()
+            # K of one tile: the forms' sums differ in their order at most, 128 terms, and both round
+            mag = part.double().abs() @ W.values().double().abs().T * 2      # 4-bit values of X are off by less than themselves
+            assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * mag).all()), t
+        del y
+
+
+def test_matrices_beyond_32_bits():
+    """A matrix of more than 2^32 bytes of codes: quantised, read back, and as the weight of few and of more rows."""
+    N, K = _lib.MX4_MAX, 8320
+    _say("large W", N, K)
+    x = torch.empty(N, K, device="cuda", dtype=torch.bfloat16)
+    x.normal_()
+    W = Mx4Matrix.quantised(x)
+    tail = Mx4Matrix.quantised(x[-100:].contiguous())
+    assert W.codes.numel() > 1 << 32
+    v = W.values(out=x)
+    want = tail.values()
+    assert torch.equal(v[-100:], want)
+    del v, x
+    for T in (3, 70):
+        xb = torch.randn(T, K, device="cuda", dtype=torch.bfloat16)
+        X = Mx4Matrix.quantised(xb)
+        for rows, values in ((X, X.values()), (xb, xb)):
+            y = mx4_gemm(rows, W, out="f32")[:, -100:]
+            exact = _np(values) @ _np(want).T
+            _check(y, exact, _off(_np(values), _np(want), rows is xb))
+            del y
 
 
 def test_empty():

@@ -181,6 +181,22 @@ def test_bad_values_stay_in_their_pair_or_head():
     assert normed[1, 2].all() and normed[2, 0, 63] and normed.any(-1).sum() == 2
 
 
+def test_rows_beyond_32_bits():
+    """2^20 rows of 4.5 GB, in place: the last ones and those across 2^32 bytes as a call on them alone."""
+    T, nh, nkv, hd = 1 << 20, 14, 3, 128
+    _say("large", T)
+    qkv = torch.randn(T, (nh + 2 * nkv) * hd, device="cuda", dtype=torch.bfloat16)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    r = Rotary(128, layout="interleaved", scaling={"kind": "linear", "factor": 8.0})
+    q, k = r.heads(qkv, nh, nkv, hd, gated=False)
+    at = [0, (1 << 32) // (2 * qkv.shape[1]) - 32, T - 64]
+    want = [r.apply(q[t:t + 64].contiguous(), k[t:t + 64].contiguous(), pos[t:t + 64].contiguous()) for t in at]
+    v = [qkv[t:t + 64, (nh + nkv) * hd:].clone() for t in at]
+    r.apply(q, k, pos, q_out=q, k_out=k)
+    for t, (wq, wk), wv in zip(at, want, v):
+        assert torch.equal(q[t:t + 64], wq) and torch.equal(k[t:t + 64], wk) and torch.equal(qkv[t:t + 64, (nh + nkv) * hd:], wv)
+
+
 def test_in_a_graph():
     q, k, qw, kw = _inputs(33, 24, 4, 256, torch.bfloat16, 4)
     pos = torch.arange(33, dtype=torch.int32, device="cuda")
