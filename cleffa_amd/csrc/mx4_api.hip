@@ -133,14 +133,14 @@ void launch_wide(const mx4::GemmParams &p, hipStream_t s) {
 void launch4(const mx4::GemmParams &p, hipStream_t s) {
     using Small = mx4::TileCfg<64, 128, 64, 32, 4, 2>;
     using Middle = mx4::TileCfg<128, 128, 64, 64, 4, 2>;
-    using Large = mx4::TileCfg<256, 128, 128, 64, 3, 2>;
+    using Large = mx4::TileCfg<256, 128, 64, 64, 3, 2>;      // eight waves; with four, where each CU has one: 425 x 10,240 x 4,096 17.0 us, with eight 16.0
     using Square = mx4::TileCfg<256, 256, 128, 64, 4, 1>;    // eight waves, one workgroup a CU
     if (launch_rows<1, 1, 8, 3>(p, s) || launch_rows<1, 2, 8, 3>(p, s) || launch_rows<2, 2, 8, 2>(p, s) || launch_rows<2, 4, 8, 2>(p, s) ||
         launch_rows<4, 4, 8, 2>(p, s))
         return;
-    // rounds of 40 K tiles, us: 256 rows x 14,336 small 17.2, middle 14.4, large 18.1, square 25.5; 512 rows 32, 26, 23.5, 28; 2,048 rows large 73, square 70;
-    // 4,096 rows 227, 163, 145 and 149, 149; 3,000 x 10,240 x 4,096 large 61.5, square 59.8; 1,160 x 5,120 x 6,144 27.7, 26.6, 25.8, 33; 2,048 rows 46, 41, 36 to 42, 38
-    const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 22.f, 41.f);
+    // rounds of 40 K tiles, us: 256 rows x 14,336 small 15.8, middle 12.8, large 17.2, square 25.0; 512 rows 32, 25, 23, 27; 2,048 rows large 73, square 70;
+    // 4,096 rows 222, 161, 144, 143; 3,000 x 10,240 x 4,096 95, 74, 67, 61; 1,160 x 5,120 x 6,144 27.6, 26.7, 24.0, 31; 2,048 rows 45, 40, 40, 38
+    const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 20.f, 41.f);
     const float square = 36.f * (float)((tiles<Square>(p) + kCus - 1) / kCus);
     if (square < large && square < middle && square < small) launch_tile<Square>(p, s);
     else if (small <= middle && small <= large) launch_tile<Small>(p, s);

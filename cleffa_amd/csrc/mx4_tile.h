@@ -8,10 +8,10 @@
 // products behind the waits.
 //
 // Bound by the matrix units and LDS together. A K tile of 256 x 256 is 1,024 clocks of a CU's products; its waves' operands are 96 KB
-// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 140 us, 4.3 PFLOP/s: the products
+// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 137 us, 4.4 PFLOP/s: the products
 // alone, on such data, ran at 6.3 in a loop without any loads, the chip at 1.8 of its 2.4 GHz for its power. Tiles of 256 x 128, two
-// workgroups a CU, read a ninth more and take 0 to 7% longer (1,900 x 6,301 x 1,696 20.9 us against 19.5); tiles of 128 x 128 163. Four
-// waves of 128 x 128 read a third less of LDS, but nothing runs while they wait: 149 us where eight took 144.
+// workgroups a CU, take 0 to 10% longer (3,000 x 10,240 x 4,096 66.7 us against 60.8), tiles of 128 x 128 161. Four waves of
+// 128 x 128 read a third less of LDS, but nothing runs while they wait: 149 us where eight took 144.
 #pragma once
 #include <utility>
 
