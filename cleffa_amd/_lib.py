@@ -150,7 +150,7 @@ class RotaryArgs(ctypes.Structure):
     _fields_ = [
         ("T", c_int), ("hd", c_int), ("n_rot", c_int), ("layout", c_int), ("axes", c_int), ("type", c_int),
         ("eps", c_float), ("magnitude", c_float), ("pos", c_void_p), ("freq", c_void_p),
-        *((f"{g}.{name}", t) for g in "qk" for name, t in _HEADS),
+        *((f"{g}.{name}", t) for g in "qk" for name, t in _HEADS), ("bf16_out", c_int),
     ]
 
 

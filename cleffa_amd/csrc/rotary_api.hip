@@ -27,11 +27,10 @@ bool fail(char *err, size_t errlen, const char *fmt, ...) {
     return false;
 }
 
-bool group_ok(const char *what, const clef_hip_rotary_heads *g, int T, int hd, int size, char *err, size_t errlen) {
+bool group_ok(const char *what, const clef_hip_rotary_heads *g, int T, int hd, int size, int out_size, char *err, size_t errlen) {
     if (g->heads < 0 || g->heads > 4096) return fail(err, errlen, "rotary: %d %s heads", g->heads, what);
     if (g->heads == 0 || T == 0) return true;
-    const uintptr_t a = (uintptr_t)(size - 1);
-    if (!g->x || !g->out || ((uintptr_t)g->x & a) || ((uintptr_t)g->out & a) || ((uintptr_t)g->norm & 3u))
+    if (!g->x || !g->out || (uintptr_t)g->x % size || (uintptr_t)g->out % out_size || ((uintptr_t)g->norm & 3u))
         return fail(err, errlen, "rotary: %s, its output and norm must be aligned device pointers", what);
     if ((T > 1 && (g->x_row < 0 || g->out_row < 0)) || (g->heads > 1 && (g->x_head < 0 || g->out_head < 0)))
         return fail(err, errlen, "rotary: negative %s strides", what);
@@ -40,60 +39,60 @@ bool group_ok(const char *what, const clef_hip_rotary_heads *g, int T, int hd, i
     const bool by_row = head >= hd && (T == 1 || row >= (g->heads - 1) * g->out_head + hd);
     const bool by_head = row >= hd && (g->heads == 1 || head >= (T - 1) * g->out_row + hd);
     if (!by_row && !by_head) return fail(err, errlen, "rotary: heads or rows of the %s output overlap", what);
+    if (g->x == g->out && size != out_size) return fail(err, errlen, "rotary: %s in place needs outputs of the same type", what);
     if (g->x == g->out && ((T > 1 && g->x_row != g->out_row) || (g->heads > 1 && g->x_head != g->out_head)))
         return fail(err, errlen, "rotary: %s in place needs the same strides", what);
     return true;
 }
 
-// whether all of a group's runs of v values of `size` bytes start at multiples of their size
-bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size) {
+// whether all of a group's runs of v values of `size` bytes, `out_size` of its outputs, start at multiples of their size
+bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size, int out_size) {
     if (g->heads == 0) return true;
-    const uintptr_t a = (uintptr_t)(v * size - 1);
-    if (((uintptr_t)g->x & a) || ((uintptr_t)g->out & a)) return false;
+    if ((uintptr_t)g->x % (v * size) || (uintptr_t)g->out % (v * out_size)) return false;
     if (g->heads > 1 && (g->x_head % v || g->out_head % v)) return false;
     return T <= 1 || (g->x_row % v == 0 && g->out_row % v == 0);
 }
 
-rotary::Group group(const clef_hip_rotary_heads *g, int size) {
+rotary::Group group(const clef_hip_rotary_heads *g, int out_size) {
     return rotary::Group{g->x, g->out, g->norm, g->x_row, g->x_head, g->out_row, g->out_head, g->heads,
-                         whole_lines(g->out, g->out_row * size) && whole_lines(g->out, g->out_head * size)};
+                         whole_lines(g->out, g->out_row * out_size) && whole_lines(g->out, g->out_head * out_size)};
 }
 
-template <int TYPE, int V, int L, int I, bool HALF>
+template <int TYPE, int OUT, int V, int L, int I, bool HALF>
 void launch_tokens(const rotary::Params &p, hipStream_t s) {
-    if (p.T <= 512) hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, 1, HALF>), dim3((unsigned)p.T), dim3(rotary::kThreads), 0, s, p);
-    else hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, V, L, I, 4, HALF>), dim3((unsigned)((p.T + 3) / 4)), dim3(rotary::kThreads), 0, s, p);
+    if (p.T <= 512) hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, OUT, V, L, I, 1, HALF>), dim3((unsigned)p.T), dim3(rotary::kThreads), 0, s, p);
+    else hipLaunchKernelGGL((rotary::rotary_kernel<TYPE, OUT, V, L, I, 4, HALF>), dim3((unsigned)((p.T + 3) / 4)), dim3(rotary::kThreads), 0, s, p);
 }
-template <int TYPE, int V, int L, int I>
+template <int TYPE, int OUT, int V, int L, int I>
 void launch(rotary::Params &p, hipStream_t s) {
     p.q_units = (p.q.heads + 64 / L - 1) / (64 / L);
     p.units = p.q_units + (p.k.heads + 64 / L - 1) / (64 / L);
-    if (p.half) launch_tokens<TYPE, V, L, I, true>(p, s);
-    else launch_tokens<TYPE, V, L, I, false>(p, s);
+    if (p.half) launch_tokens<TYPE, OUT, V, L, I, true>(p, s);
+    else launch_tokens<TYPE, OUT, V, L, I, false>(p, s);
 }
 // L: the least power of two of lanes that holds a head in pairs of runs of V
-template <int TYPE, int V>
+template <int TYPE, int OUT, int V>
 void launch_runs(rotary::Params &p, hipStream_t s) {
     const int pairs = (p.hd + 2 * V - 1) / (2 * V);
-    if (pairs <= 4) launch<TYPE, V, 4, 1>(p, s);
-    else if (pairs <= 8) launch<TYPE, V, 8, 1>(p, s);
-    else if (pairs <= 16) launch<TYPE, V, 16, 1>(p, s);
+    if (pairs <= 4) launch<TYPE, OUT, V, 4, 1>(p, s);
+    else if (pairs <= 8) launch<TYPE, OUT, V, 8, 1>(p, s);
+    else if (pairs <= 16) launch<TYPE, OUT, V, 16, 1>(p, s);
     else if constexpr (V <= 4) {
-        if (pairs <= 32) launch<TYPE, V, 32, 1>(p, s);
+        if (pairs <= 32) launch<TYPE, OUT, V, 32, 1>(p, s);
         else if constexpr (V <= 2) {
-            if (pairs <= 64) launch<TYPE, V, 64, 1>(p, s);
-            else launch<TYPE, V, 64, 2>(p, s);
+            if (pairs <= 64) launch<TYPE, OUT, V, 64, 1>(p, s);
+            else launch<TYPE, OUT, V, 64, 2>(p, s);
         }
     }
 }
-template <int TYPE>
+template <int TYPE, int OUT>
 void launch_type(rotary::Params &p, int v, hipStream_t s) {
     if constexpr (TYPE != CLEF_HIP_OUT_F32) {
-        if (v == 8) return launch_runs<TYPE, 8>(p, s);
+        if (v == 8) return launch_runs<TYPE, OUT, 8>(p, s);
     }
-    if (v == 4) launch_runs<TYPE, 4>(p, s);
-    else if (v == 2) launch_runs<TYPE, 2>(p, s);
-    else launch_runs<TYPE, 1>(p, s);
+    if (v == 4) launch_runs<TYPE, OUT, 4>(p, s);
+    else if (v == 2) launch_runs<TYPE, OUT, 2>(p, s);
+    else launch_runs<TYPE, OUT, 1>(p, s);
 }
 
 }  // namespace
@@ -133,21 +132,23 @@ bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, siz
     if (a->axes < 1 || a->axes > 4) return fail(err, errlen, "rotary: %d position axes, 1 to 4 are supported", a->axes);
     if (a->type < CLEF_HIP_OUT_BF16 || a->type > CLEF_HIP_OUT_F32) return fail(err, errlen, "rotary: bad type %d", a->type);
     if (!(a->eps >= 0.f) || !isfinite(a->magnitude)) return fail(err, errlen, "rotary: bad eps or magnitude");
-    const int size = a->type == CLEF_HIP_OUT_F32 ? 4 : 2;
-    if (!group_ok("q", &a->q, a->T, a->hd, size, err, errlen) || !group_ok("k", &a->k, a->T, a->hd, size, err, errlen)) return false;
+    if (a->bf16_out != 0 && (a->bf16_out != 1 || a->type != CLEF_HIP_OUT_F32)) return fail(err, errlen, "rotary: bf16_out %d goes with f32 heads", a->bf16_out);
+    const int size = a->type == CLEF_HIP_OUT_F32 ? 4 : 2, out_size = a->bf16_out ? 2 : size;
+    if (!group_ok("q", &a->q, a->T, a->hd, size, out_size, err, errlen) || !group_ok("k", &a->k, a->T, a->hd, size, out_size, err, errlen)) return false;
     if (a->T == 0 || a->q.heads + a->k.heads == 0) return true;
     if (!a->pos || !a->freq || ((uintptr_t)a->pos & 3u) || ((uintptr_t)a->freq & 7u)) return fail(err, errlen, "rotary: pos and freq must be aligned device pointers");
     rotary::Params p;
-    p.q = group(&a->q, size); p.k = group(&a->k, size); p.pos = a->pos; p.freq = a->freq;
+    p.q = group(&a->q, out_size); p.k = group(&a->k, out_size); p.pos = a->pos; p.freq = a->freq;
     p.T = a->T; p.hd = a->hd; p.n_rot = a->n_rot; p.half = a->layout == CLEF_HIP_ROTARY_HALF; p.axes = a->axes;
     p.eps = a->eps; p.magnitude = a->magnitude;
     // the longest runs that heads divide into and that pointers and strides allow
     int v = 16 / size;
-    while (v > 1 && (a->hd % v || (p.half && (a->n_rot / 2) % v) || !runs_ok(&a->q, a->T, v, size) || !runs_ok(&a->k, a->T, v, size))) v /= 2;
+    while (v > 1 && (a->hd % v || (p.half && (a->n_rot / 2) % v) || !runs_ok(&a->q, a->T, v, size, out_size) || !runs_ok(&a->k, a->T, v, size, out_size))) v /= 2;
     const hipStream_t s = (hipStream_t)stream;
-    if (a->type == CLEF_HIP_OUT_BF16) launch_type<CLEF_HIP_OUT_BF16>(p, v, s);
-    else if (a->type == CLEF_HIP_OUT_F16) launch_type<CLEF_HIP_OUT_F16>(p, v, s);
-    else launch_type<CLEF_HIP_OUT_F32>(p, v, s);
+    if (a->type == CLEF_HIP_OUT_BF16) launch_type<CLEF_HIP_OUT_BF16, CLEF_HIP_OUT_BF16>(p, v, s);
+    else if (a->type == CLEF_HIP_OUT_F16) launch_type<CLEF_HIP_OUT_F16, CLEF_HIP_OUT_F16>(p, v, s);
+    else if (a->bf16_out) launch_type<CLEF_HIP_OUT_F32, CLEF_HIP_OUT_BF16>(p, v, s);
+    else launch_type<CLEF_HIP_OUT_F32, CLEF_HIP_OUT_F32>(p, v, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(err, errlen, "rotary launch failed: %s", hipGetErrorString(e));
     return true;

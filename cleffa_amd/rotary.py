@@ -84,33 +84,37 @@ class Rotary:
             raise ValueError(f"the dims of a head of {name} must be contiguous")
         return t.data_ptr(), 0, 0
 
-    def _heads(self, x, out, norm, name, T, hd, dtype):
+    def _heads(self, x, out, norm, name, T, hd, dtype, out_dtype):
         if x is None:
             if out is not None or norm is not None:
                 raise ValueError(f"{name}: an output or norm without heads")
             return 0, None, None, 0, 0, 0, 0, None
         shape = (T, x.shape[1] if isinstance(x, torch.Tensor) and x.dim() == 3 else -1, hd)
         px, row, head = self._view(x, name, shape, dtype)
-        po, out_row, out_head = (px, row, head) if out is x else self._view(out, name + "_out", shape, dtype)
+        po, out_row, out_head = (px, row, head) if out is x and out_dtype is dtype else self._view(out, name + "_out", shape, out_dtype)
         return shape[1], px, po, row, head, out_row, out_head, None if norm is None else _arg(norm, name + "_norm", (hd,), torch.float32, self.device)
 
     def apply(self, q, k, pos, q_norm=None, k_norm=None, q_out=None, k_out=None, stream=None):
         """q [T][nh][hd] and k [T][nkv][hd] (or None), bf16, f16 or f32, turned by pos (int32 [T] or [T][axes]), each after its
         RMSNorm where a weight [hd] f32 is given. Rows and heads may lie apart (views of a projection's rows). q_out and
-        k_out: new tensors where they are None; q and k themselves for a rotation in place. Returns (q_out, k_out)."""
+        k_out: new tensors where they are None; q and k themselves for a rotation in place; of q's type, or bf16 where q is
+        f32, which rounds once where a projection's bf16 rows have been rounded before. Returns (q_out, k_out)."""
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPE_OUT:
             raise TypeError("q must be a bf16, f16 or f32 tensor [T][heads][hd]")
         T, _, hd = q.shape
         dtype = q.dtype
+        given = k_out if q_out is None else q_out
+        narrow = dtype is torch.float32 and isinstance(given, torch.Tensor) and given.dtype is torch.bfloat16
+        out_dtype = torch.bfloat16 if narrow else dtype
         if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            q_out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
         if k_out is None and k is not None:
-            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            k_out = torch.empty_like(k, dtype=out_dtype, memory_format=torch.contiguous_format)
         if not isinstance(pos, torch.Tensor) or pos.dtype is not torch.int32 or pos.device != self.device or not pos.is_contiguous():
             raise ValueError("pos must be contiguous int32 on the operator's device")
         if pos.shape != (T, self.axes) and (self.axes > 1 or pos.shape != (T,)):
             raise ValueError(f"pos has shape {tuple(pos.shape)}, expected {(T, self.axes)}")
         a = _lib.RotaryArgs(T, hd, self.n_rot, self._layout, self.axes, _DTYPE_OUT[dtype], self.eps, self.magnitude, pos.data_ptr(), self.freq.data_ptr(),
-                            *self._heads(q, q_out, q_norm, "q", T, hd, dtype), *self._heads(k, k_out, k_norm, "k", T, hd, dtype))
+                            *self._heads(q, q_out, q_norm, "q", T, hd, dtype, out_dtype), *self._heads(k, k_out, k_norm, "k", T, hd, dtype, out_dtype), int(narrow))
         _launch(_lib.load().clef_hip_rotary, a, self.device, stream)
         return q_out, k_out

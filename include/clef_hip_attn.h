@@ -553,8 +553,9 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
  *
  * Pair j < n_rot / 2 of a head, dims (j, j + n_rot / 2) in the half layout (the prologues') or (2j, 2j + 1) in the interleaved one,
  * turns by a = pos[t][j % axes] * f_j: (x, y) -> magnitude * (x cos a - y sin a, y cos a + x sin a). Dims from n_rot on are
- * normalised alone. Angles are reduced in f64, so that far positions keep theirs; norm and rotation run in f32, rounded once.
- * Negated positions turn back.
+ * normalised alone. Angles are reduced in f64, so that far positions keep theirs; norm and rotation run in f32, rounded once, at the
+ * store. Heads of bf16 rows of a product were rounded before, as in the prologues above: q and k are then off by the square root of two times
+ * one rounding. f32 rows with bf16_out are rounded here alone. Negated positions turn back.
  *
  * clef_hip_rotary_freqs (host only): freq[j] = f_j / 2 pi, turns a position, in f64. f_j = theta^(-2j / n_rot); scaled for texts
  * `factor` times as long: LINEAR f_j / factor; BASE theta * factor^(n_rot / (n_rot - 2)) for theta; PARTS keep f_j + (1 - keep) f_j /
@@ -583,6 +584,7 @@ typedef struct {
     const int32_t *pos;       /* [T][axes] */
     const double *freq;       /* [n_rot / 2], device */
     clef_hip_rotary_heads q, k;
+    int bf16_out;             /* 1: of f32 heads, outputs in bf16 (not in place); 0: outputs of the heads' type */
 } clef_hip_rotary_args;
 bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, size_t errlen);
 
