@@ -12,6 +12,7 @@ This mirrors what cleffa's Metal backend does around its attention kernels:
 torch provides device memory and the stream; every computation runs in libclef_hip_attn.so.
 Shapes and dtypes are checked here, on the host, before any launch.
 """
+import contextlib
 import ctypes
 import math
 
@@ -69,6 +70,24 @@ def _stream_handle(stream):
             return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
         stream = torch.cuda.current_stream()
     return ctypes.c_void_p(stream.cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(stream):
+    """Where a call makes its results, planes and tables: in the memory of the stream that it runs on. Memory of the current one torch
+    could have taken from, or give to, work there that the call does not wait for."""
+    return _HERE if stream is None else torch.cuda.stream(stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(stream):
+    """Where a call makes its results, planes and tables: in the memory of the stream that it runs on. Memory of the current one torch
+    could have taken from, or give to, work there that the call does not wait for."""
+    return _HERE if stream is None else torch.cuda.stream(stream)
 
 
 _ERR = ctypes.c_char * 512
@@ -348,15 +367,16 @@ class TextAttention:
         not given. A "core" call with a table reads what the last "prep" call wrote."""
         lib = _lib.load()
         out_type, odt = _OUT_TYPES[out_dtype]
-        if out is None:
-            out = torch.empty((plan.T, self.nh * self.hd), dtype=odt, device=self.device)
-        if k_plane is None:
-            kvT = plan.kvT
-            k_plane, vt_plane = self.planes(kvT, fp32=qkv.dtype == torch.float32)
-        elif kvT is None:
-            kvT = k_plane.shape[1]
-        if rope_cs is None and stage == "prefill" and self.n_rot:
-            rope_cs = self.rope_table(plan.T)
+        with _on(stream):
+            if out is None:
+                out = torch.empty((plan.T, self.nh * self.hd), dtype=odt, device=self.device)
+            if k_plane is None:
+                kvT = plan.kvT
+                k_plane, vt_plane = self.planes(kvT, fp32=qkv.dtype == torch.float32)
+            elif kvT is None:
+                kvT = k_plane.shape[1]
+            if rope_cs is None and stage == "prefill" and self.n_rot:
+                rope_cs = self.rope_table(plan.T)
         a = self.args(qkv, q_norm, k_norm, pos3, plan, out, k_plane, vt_plane, kvT,
                       out_type=out_type, gate=gate, ovf=ovf, f16_lim=f16_lim, rope_cs=rope_cs,
                       trace=trace, schedule=schedule)
@@ -388,12 +408,14 @@ class TextAttention:
             _check(X, "X", (T, H), torch.bfloat16, dev)
             _check(W, "W", (self.row, H), torch.bfloat16, dev)
         if qkv is None:
-            qkv = torch.empty((T, self.row), dtype=torch.bfloat16, device=dev)
+            with _on(stream):
+                qkv = torch.empty((T, self.row), dtype=torch.bfloat16, device=dev)
         _check(qkv, "qkv", (T, self.row), torch.bfloat16, dev)
         if prologue:
             if k_plane is None:
                 kvT = plan.kvT
-                k_plane, vt_plane = self.planes(kvT)
+                with _on(stream):
+                    k_plane, vt_plane = self.planes(kvT)
             elif kvT is None:
                 kvT = k_plane.shape[1]
             a = self.args(qkv, q_norm, k_norm, pos3, plan, None, k_plane, vt_plane, kvT, ovf=ovf, f16_lim=f16_lim,
@@ -445,7 +467,8 @@ class TextAttention:
             out = to = None
         else:
             if out is None:
-                out = torch.empty((T, self.nh * hd), dtype=odt, device=dev)
+                with _on(stream):
+                    out = torch.empty((T, self.nh * hd), dtype=odt, device=dev)
             to = _arg(out, "out", (T, self.nh * hd), odt, dev)
         a = _lib.Kv8Args(self.nh, self.nkv, hd, self.n_rot, self.eps, self.scale, T, row, cache.max_seqs, cache.max_pages, cache.n_pages,
                          plan.max_new, qkv, q_norm, k_norm, pos3, self.inv_freq.data_ptr(), *pools, plan.work.data_ptr(), int(gate), to,
@@ -486,7 +509,8 @@ class VisionAttention:
         _check(pos2, "pos2", (P, 2), torch.int32, dev)
         out_type, odt = _OUT_TYPES[out_dtype]
         if out is None:
-            out = torch.empty((P, self.E), dtype=odt, device=dev)
+            with _on(stream):
+                out = torch.empty((P, self.E), dtype=odt, device=dev)
         _check(out, "out", (P, self.E), odt, dev)
         if ovf is not None:
             _check(ovf, "ovf", (P,), torch.int32, dev)
@@ -495,7 +519,8 @@ class VisionAttention:
             q_plane = k_plane = vt_plane = None
         else:
             if scratch is None:
-                scratch = self.scratch(P, kvT)
+                with _on(stream):
+                    scratch = self.scratch(P, kvT)
             q_plane, k_plane, vt_plane = scratch
             _check(q_plane, "q_plane", (self.heads, P, self.hd), torch.bfloat16, dev)
             _check(k_plane, "k_plane", (self.heads, kvT, self.hd), torch.bfloat16, dev)

@@ -7,7 +7,7 @@ import torch
 
 from . import _lib
 from ._lib import c_void_p  # noqa: F401
-from .attention import _err, _stream_handle
+from .attention import _err, _on, _stream_handle
 
 Y_F32, Y_BF16 = 0, 1
 
@@ -25,7 +25,8 @@ def gemm(X, W, Y=None, out="bf16", acc=False, workspace=None, stream=None):
     if Y is None:
         if acc:
             raise ValueError("acc needs the Y to add into")
-        Y = torch.empty(T, N, dtype=dt, device=X.device)
+        with _on(stream):
+            Y = torch.empty(T, N, dtype=dt, device=X.device)
     if Y.shape != (T, N) or Y.dtype != dt or not Y.is_contiguous():
         raise ValueError(f"Y must be contiguous {dt} [{T}][{N}]")
     ws = 0 if workspace is None else workspace.numel() * workspace.element_size()

@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from ._lib import AttnConfig, GgufTensorInfo
-from .attention import _err, _stream_handle
+from .attention import _err, _on, _stream_handle
 
 _NP = {_lib.GGML_F32: np.float32, _lib.GGML_F16: np.float16, _lib.GGML_BF16: np.uint16}
 
@@ -77,10 +77,11 @@ class GgufFile:
         device (the QKV GEMM's and o_proj's W, the path's norm weights)."""
         c = self.attn_config()
         n_attn = 2 * c.nh * c.hd + 2 * c.nkv * c.hd
-        w_qkv = torch.empty(n_attn, c.H, dtype=torch.bfloat16, device=device)
-        w_o = torch.empty(c.H, c.nh * c.hd, dtype=torch.bfloat16, device=device)
-        qn = torch.empty(c.hd, dtype=torch.float32, device=device)
-        kn = torch.empty(c.hd, dtype=torch.float32, device=device)
+        with _on(stream):
+            w_qkv = torch.empty(n_attn, c.H, dtype=torch.bfloat16, device=device)
+            w_o = torch.empty(c.H, c.nh * c.hd, dtype=torch.bfloat16, device=device)
+            qn = torch.empty(c.hd, dtype=torch.float32, device=device)
+            kn = torch.empty(c.hd, dtype=torch.float32, device=device)
         err = _err()
         ok = _lib.load().clef_hip_gguf_attn_layer(self._h, ctypes.byref(c), layer, w_qkv.data_ptr(), w_o.data_ptr(),
                                                   qn.data_ptr(), kn.data_ptr(), _stream_handle(stream), err, len(err))
@@ -89,10 +90,11 @@ class GgufFile:
 
     def vis_layer(self, layer, heads=16, device="cuda", stream=None):
         E = 72 * heads
-        w_qkv = torch.empty(3 * E, E, dtype=torch.bfloat16, device=device)
-        b_qkv = torch.empty(3 * E, dtype=torch.float32, device=device)
-        w_o = torch.empty(E, E, dtype=torch.bfloat16, device=device)
-        b_o = torch.empty(E, dtype=torch.float32, device=device)
+        with _on(stream):
+            w_qkv = torch.empty(3 * E, E, dtype=torch.bfloat16, device=device)
+            b_qkv = torch.empty(3 * E, dtype=torch.float32, device=device)
+            w_o = torch.empty(E, E, dtype=torch.bfloat16, device=device)
+            b_o = torch.empty(E, dtype=torch.float32, device=device)
         err = _err()
         ok = _lib.load().clef_hip_gguf_vis_layer(self._h, layer, heads, w_qkv.data_ptr(), b_qkv.data_ptr(), w_o.data_ptr(),
                                                  b_o.data_ptr(), _stream_handle(stream), err, len(err))

@@ -6,13 +6,16 @@ attention with weights in 4 bits, for prompts with activations in 4 bits too.
     qkv = mx4_gemm(x.quantise(h), w)                # or mx4_gemm(h, w): activations stay in bf16
 
 Formats and layouts: include/clef_hip_attn.h. ``Mx4Matrix.from_codes`` takes codes and scales as files store them.
+
+Calls run on the current stream, or on ``stream``; what they make lies in that stream's memory, as if made with it current. What
+they are given has to stay until the call has run (``Tensor.record_stream`` where it is dropped before).
 """
 import ctypes
 
 import torch
 
 from . import _lib
-from .attention import _DTYPE_OUT, _arg, _device, _err, _launch, init_device
+from .attention import _DTYPE_OUT, _arg, _device, _err, _launch, _on, init_device
 from .gemm import Y_BF16, Y_F32
 
 _Y_TYPES = {torch.bfloat16: Y_BF16, torch.float32: Y_F32}
@@ -79,7 +82,9 @@ class Mx4Matrix:
         """x [rows][K] in 4 bits, in new buffers."""
         if x.dim() != 2:
             raise ValueError(f"a matrix is needed, not {tuple(x.shape)}")
-        return cls(x.shape[0], x.shape[1], x.device).quantise(x, stream=stream)
+        with _on(stream):
+            m = cls(x.shape[0], x.shape[1], x.device)
+        return m.quantise(x, stream=stream)
 
     @classmethod
     def from_codes(cls, codes, scales, stream=None):
@@ -87,13 +92,15 @@ class Mx4Matrix:
         [rows][K / 32], as files store them (on the device)."""
         if codes.dim() != 2 or scales.dim() != 2:
             raise ValueError(f"codes and scales must be matrices, not {tuple(codes.shape)} and {tuple(scales.shape)}")
-        m = cls(codes.shape[0], 2 * codes.shape[1], codes.device)
+        with _on(stream):
+            m = cls(codes.shape[0], 2 * codes.shape[1], codes.device)
         return m._pack(codes, scales, 0, stream)
 
     def to_codes(self, stream=None):
         """(codes [rows][K / 2], scales [rows][K / 32]), as from_codes takes them."""
-        codes = torch.empty(self.rows, self.K // 2, dtype=torch.uint8, device=self.device)
-        scales = torch.empty(self.rows, self.K // _lib.MX4_BLOCK, dtype=torch.uint8, device=self.device)
+        with _on(stream):
+            codes = torch.empty(self.rows, self.K // 2, dtype=torch.uint8, device=self.device)
+            scales = torch.empty(self.rows, self.K // _lib.MX4_BLOCK, dtype=torch.uint8, device=self.device)
         self._pack(codes, scales, 1, stream)
         return codes, scales
 
@@ -121,7 +128,8 @@ class Mx4Matrix:
         if out is None:
             if out_dtype not in ("bf16", "f32"):
                 raise ValueError(f"out_dtype {out_dtype!r}: bf16 or f32")
-            out = torch.empty(self.rows, self.K, dtype=torch.bfloat16 if out_dtype == "bf16" else torch.float32, device=self.device)
+            with _on(stream):
+                out = torch.empty(self.rows, self.K, dtype=torch.bfloat16 if out_dtype == "bf16" else torch.float32, device=self.device)
         if not isinstance(out, torch.Tensor) or out.dtype not in _Y_TYPES:
             raise TypeError("out must be a bf16 or f32 tensor")
         px, row = _rows_arg(out, "out", (self.rows, self.K), out.dtype, self.device, 8)
@@ -151,7 +159,8 @@ def mx4_gemm(X, W, Y=None, out="bf16", residual=None, stream=None):
     if Y is None:
         if out not in ("bf16", "f32"):
             raise ValueError(f"out {out!r}: bf16 or f32")
-        Y = torch.empty(T, N, dtype=torch.bfloat16 if out == "bf16" and residual is None else torch.float32, device=dev)
+        with _on(stream):
+            Y = torch.empty(T, N, dtype=torch.bfloat16 if out == "bf16" and residual is None else torch.float32, device=dev)
     if not isinstance(Y, torch.Tensor) or Y.dtype not in _Y_TYPES:
         raise TypeError("Y must be a bf16 or f32 tensor")
     py, y_row = _rows_arg(Y, "Y", (T, N), Y.dtype, dev)

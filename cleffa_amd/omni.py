@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from ._lib import OmniAttnArgs, OmniPrepArgs
-from .attention import _device, _err, _i32p, _ptr, _stream_handle
+from .attention import _device, _err, _i32p, _on, _ptr, _stream_handle
 
 HD = 128
 BLOCK_Q = 16
@@ -69,9 +69,10 @@ class OmniAttention:
         for w in (q_norm, k_norm):
             if w.shape != (HD,) or w.dtype != torch.float32:
                 raise ValueError("norm weights must be f32 [128]")
-        Q, K, V = self.planes(T) if planes is None else planes
-        if status is None:
-            status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        with _on(stream):
+            Q, K, V = self.planes(T) if planes is None else planes
+            if status is None:
+                status = torch.zeros(1, dtype=torch.int32, device=self.device)
         a = OmniPrepArgs()
         a.nh, a.nkv, a.T, a.kvT, a.eps, a.rope_exact = self.nh, self.nkv, T, K.shape[1], self.eps, int(self.rope_exact)
         a.qkv, a.q_norm, a.k_norm, a.pos3, a.freq = _ptr(qkv), _ptr(q_norm), _ptr(k_norm), _ptr(pos3), _ptr(self.freq)
@@ -83,7 +84,8 @@ class OmniAttention:
     def attention(self, Q, K, V, plan, out=None, stream=None):
         T = plan.T
         if out is None:
-            out = torch.empty(T, self.nh * HD, dtype=torch.float32, device=self.device)
+            with _on(stream):
+                out = torch.empty(T, self.nh * HD, dtype=torch.float32, device=self.device)
         if out.shape != (T, self.nh * HD) or out.dtype != torch.float32:
             raise ValueError("out must be f32 [T][nh*128]")
         if Q.shape[1] < T or K.shape[1] < T + SLACK or V.shape != K.shape:

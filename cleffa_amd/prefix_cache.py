@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _stream_handle
+from .attention import _on, _stream_handle
 
 
 class PrefixEntry:
@@ -33,8 +33,9 @@ class PrefixEntry:
             return False
         if keep > self.cap:
             raise ValueError(f"keep {keep} exceeds the entry's {self.cap} rows")
-        K = [torch.empty(self.nkv, cap, self.hd, dtype=torch.float16, device=self.device) for _ in range(self.n_layers)]
-        Vt = [torch.empty(self.nkv, self.hd, cap, dtype=torch.bfloat16, device=self.device) for _ in range(self.n_layers)]
+        with _on(stream):
+            K = [torch.empty(self.nkv, cap, self.hd, dtype=torch.float16, device=self.device) for _ in range(self.n_layers)]
+            Vt = [torch.empty(self.nkv, self.hd, cap, dtype=torch.bfloat16, device=self.device) for _ in range(self.n_layers)]
         err = ctypes.create_string_buffer(256)
         s = _stream_handle(stream)
         for l in range(self.n_layers):
@@ -43,5 +44,8 @@ class PrefixEntry:
             ok = lib.clef_hip_prefix_copy(ks, vs, self.cap, K[l].data_ptr(), Vt[l].data_ptr(), cap,
                                           self.nkv, self.hd, int(keep) if ks else 0, s, err, len(err))
             _lib.check(ok, err)
+        for t in (*self.K, *self.Vt):     # their memory is free behind the copies, whichever stream's it is
+            if t is not None:
+                t.record_stream(torch.cuda.current_stream(t.device) if stream is None else stream)
         self.K, self.Vt, self.cap = K, Vt, cap
         return True

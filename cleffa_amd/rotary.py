@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .attention import _DTYPE_OUT, _arg, _device, _launch, _err, init_device
+from .attention import _DTYPE_OUT, _arg, _device, _launch, _on, _err, init_device
 
 
 class Rotary:
@@ -107,9 +107,11 @@ class Rotary:
         narrow = dtype is torch.float32 and isinstance(given, torch.Tensor) and given.dtype is torch.bfloat16
         out_dtype = torch.bfloat16 if narrow else dtype
         if q_out is None:
-            q_out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+            with _on(stream):
+                q_out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
         if k_out is None and k is not None:
-            k_out = torch.empty_like(k, dtype=out_dtype, memory_format=torch.contiguous_format)
+            with _on(stream):
+                k_out = torch.empty_like(k, dtype=out_dtype, memory_format=torch.contiguous_format)
         if not isinstance(pos, torch.Tensor) or pos.dtype is not torch.int32 or pos.device != self.device or not pos.is_contiguous():
             raise ValueError("pos must be contiguous int32 on the operator's device")
         if pos.shape != (T, self.axes) and (self.axes > 1 or pos.shape != (T,)):
