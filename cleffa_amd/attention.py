@@ -394,7 +394,6 @@ class TextAttention:
         planes (and rope_cs) as the "prep" stage would, so forward(stage="core") may follow on
         the same planes and table. W may also be an mx4.Mx4Matrix, and X then one too: the product is
         mx4_gemm's, and the "prep" stage runs behind it. Returns qkv."""
-        from .mx4 import Mx4Matrix, mx4_gemm
         dev = self.device
         T = plan.T
         four_bit = isinstance(W, Mx4Matrix)
@@ -542,3 +541,6 @@ class VisionAttention:
         return (torch.empty((self.heads, max(P, 1), self.hd), dtype=torch.bfloat16, device=dev),
                 torch.empty((self.heads, kvT, self.hd), dtype=torch.bfloat16, device=dev),
                 torch.empty((self.heads, self.hd, kvT), dtype=torch.bfloat16, device=dev))
+
+
+from .mx4 import Mx4Matrix, mx4_gemm  # noqa: E402  (for project; at the end, since mx4 takes helpers from here)
