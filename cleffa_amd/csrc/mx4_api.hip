@@ -11,6 +11,7 @@
 #include "mx4_rows16.h"
 #include "mx4_tile.h"
 #include "mx4_wide.h"
+#include "ranges.h"
 
 using namespace clef_hip;
 
@@ -57,14 +58,17 @@ bool matrix_ok(const char *what, const uint8_t *codes, const uint8_t *scales, ch
     return true;
 }
 
-// Whether the residual is Y itself, or none of its values one of Y's: the other side of it, or other columns of rows of the same length.
+// Y and the residual by rows, each row from its first to its last value.
+Rows rows_of(const void *p, int n, long row, long values, long size) { return Rows{(uintptr_t)p, n, n > 1 ? row * size : 0, values * size}; }
+// Whether the residual is Y itself, or none of its values one of Y's.
 bool apart(const clef_hip_mx4_gemm_args *a) {
-    const uintptr_t y = (uintptr_t)a->y, r = (uintptr_t)a->residual;
-    if (y == r) return a->T == 1 || a->y_row == a->r_row;
-    const uintptr_t y_end = y + 4 * ((size_t)(a->T - 1) * a->y_row + a->N), r_end = r + 4 * ((size_t)(a->T - 1) * a->r_row + a->N);
-    if (r >= y_end || y >= r_end) return true;
-    const long d = ((long)(r - y) / 4 % a->y_row + a->y_row) % a->y_row;
-    return a->T > 1 && a->y_row == a->r_row && (r - y) % 4 == 0 && d >= a->N && d <= a->y_row - a->N;
+    return (a->y == a->residual && (a->T == 1 || a->y_row == a->r_row)) || !meet(rows_of(a->y, a->T, a->y_row, a->N, 4), rows_of(a->residual, a->T, a->r_row, a->N, 4));
+}
+// Whether Y has bytes of a matrix's buffers.
+bool meets_matrix(const Rows &y, const uint8_t *codes, const uint8_t *scales, int rows, int K) {
+    const size_t tiles = (size_t)mx4::ceil_div(rows, mx4::ROWS);
+    return meets(y, (uintptr_t)codes, (uintptr_t)codes + tiles * mx4::ceil_div(K, mx4::KT) * mx4::TILE_BYTES) ||
+           meets(y, (uintptr_t)scales, (uintptr_t)scales + tiles * mx4::ceil_div(K, mx4::KG) * mx4::GROUP_BYTES);
 }
 
 mx4::Matrix matrix(const uint8_t *codes, const uint8_t *scales, int rows, int K) {
@@ -224,6 +228,9 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     if (a->y_type != CLEF_HIP_GEMM_Y_F32 && a->y_type != CLEF_HIP_GEMM_Y_BF16) return fail(err, errlen, "4-bit product: bad y_type %d", a->y_type);
     if (a->residual && a->y_type != CLEF_HIP_GEMM_Y_F32) return fail(err, errlen, "4-bit product: a residual needs an f32 Y");
     if (a->y_row < a->N || (a->residual && a->r_row < a->N)) return fail(err, errlen, "4-bit product: rows of Y and the residual must hold %d values", a->N);
+    const int y_size = a->y_type == CLEF_HIP_GEMM_Y_BF16 ? 2 : 4;
+    if (!span_ok(a->T, a->y_row, y_size) || (a->residual && !span_ok(a->T, a->r_row, 4)) || (a->x_bf16 && !span_ok(a->T, a->x_row, 2)))
+        return fail(err, errlen, "4-bit product: rows too far apart");
     if (!a->x_codes != !a->x_scales) return fail(err, errlen, "4-bit product: x_codes and x_scales must both be set or both be NULL");
     if (!a->x_codes == !a->x_bf16) return fail(err, errlen, "4-bit product: X must be given in 4 bits or in bf16");
     if (a->T == 0) return true;
@@ -231,9 +238,13 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
     if (a->x_codes && !matrix_ok("4-bit product: X", a->x_codes, a->x_scales, err, errlen)) return false;
     if (a->x_bf16 && (!aligned16(a->x_bf16) || a->x_row < a->K || a->x_row % 8))
         return fail(err, errlen, "4-bit product: X must be 16-byte aligned, its row %ld >= %d and a multiple of 8", a->x_row, a->K);
-    if (!a->y || ((uintptr_t)a->y & (a->y_type == CLEF_HIP_GEMM_Y_BF16 ? 1u : 3u)) || ((uintptr_t)a->residual & 3u))
+    if (!a->y || (uintptr_t)a->y % y_size || ((uintptr_t)a->residual & 3u))
         return fail(err, errlen, "4-bit product: Y and the residual must be aligned device pointers");
     if (a->residual && !apart(a)) return fail(err, errlen, "4-bit product: the residual may be Y itself, but not overlap it otherwise");
+    const Rows y = rows_of(a->y, a->T, a->y_row, a->N, y_size);
+    if (meets_matrix(y, a->w_codes, a->w_scales, a->N, a->K)) return fail(err, errlen, "4-bit product: Y overlaps W");
+    if (a->x_codes ? meets_matrix(y, a->x_codes, a->x_scales, a->T, a->K) : meet(y, rows_of(a->x_bf16, a->T, a->x_row, a->K, 2)))
+        return fail(err, errlen, "4-bit product: Y overlaps X");
     mx4::GemmParams p;
     p.w = matrix(a->w_codes, a->w_scales, a->N, a->K);
     p.x = matrix(a->x_codes, a->x_scales, a->T, a->K);

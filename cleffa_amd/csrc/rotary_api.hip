@@ -7,6 +7,7 @@
 #include <stdio.h>
 
 #include "clef_hip_attn.h"
+#include "ranges.h"
 #include "rotary.h"
 
 using namespace clef_hip;
@@ -34,6 +35,8 @@ bool group_ok(const char *what, const clef_hip_rotary_heads *g, int T, int hd, i
         return fail(err, errlen, "rotary: %s, its output and norm must be aligned device pointers", what);
     if ((T > 1 && (g->x_row < 0 || g->out_row < 0)) || (g->heads > 1 && (g->x_head < 0 || g->out_head < 0)))
         return fail(err, errlen, "rotary: negative %s strides", what);
+    if (!span_ok(T, g->x_row, size) || !span_ok(T, g->out_row, size) || !span_ok(g->heads, g->x_head, size) || !span_ok(g->heads, g->out_head, size))
+        return fail(err, errlen, "rotary: %s too far apart", what);
     // rows of heads, or heads of rows
     const long row = T > 1 ? g->out_row : LONG_MAX, head = g->heads > 1 ? g->out_head : LONG_MAX;
     const bool by_row = head >= hd && (T == 1 || row >= (g->heads - 1) * g->out_head + hd);
@@ -51,6 +54,16 @@ bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size, int out_siz
     if ((uintptr_t)g->x % (v * size) || (uintptr_t)g->out % (v * out_size)) return false;
     if (g->heads > 1 && (g->x_head % v || g->out_head % v)) return false;
     return T <= 1 || (g->x_row % v == 0 && g->out_row % v == 0);
+}
+
+// Whether outputs have bytes of heads that are read, or of each other; heads turned in place are their own outputs.
+bool overlap(const clef_hip_rotary_args *a, int size, int out_size) {
+    const auto heads = [&](const void *p, const clef_hip_rotary_heads &g, long row, long head, long size) {
+        return Heads{(uintptr_t)p, a->T, a->T > 1 ? row * size : 0, g.heads, g.heads > 1 ? head * size : 0, a->hd * size};
+    };
+    const Heads q = heads(a->q.x, a->q, a->q.x_row, a->q.x_head, size), k = heads(a->k.x, a->k, a->k.x_row, a->k.x_head, size);
+    const Heads qo = heads(a->q.out, a->q, a->q.out_row, a->q.out_head, out_size), ko = heads(a->k.out, a->k, a->k.out_row, a->k.out_head, out_size);
+    return (a->q.x != a->q.out && meet(qo, q)) || (a->k.x != a->k.out && meet(ko, k)) || meet(qo, k) || meet(ko, q) || meet(qo, ko);
 }
 
 rotary::Group group(const clef_hip_rotary_heads *g, int out_size) {
@@ -137,6 +150,7 @@ bool clef_hip_rotary(const clef_hip_rotary_args *a, void *stream, char *err, siz
     if (!group_ok("q", &a->q, a->T, a->hd, size, out_size, err, errlen) || !group_ok("k", &a->k, a->T, a->hd, size, out_size, err, errlen)) return false;
     if (a->T == 0 || a->q.heads + a->k.heads == 0) return true;
     if (!a->pos || !a->freq || ((uintptr_t)a->pos & 3u) || ((uintptr_t)a->freq & 7u)) return fail(err, errlen, "rotary: pos and freq must be aligned device pointers");
+    if (overlap(a, size, out_size)) return fail(err, errlen, "rotary: an output overlaps the other one, or heads that are read");
     rotary::Params p;
     p.q = group(&a->q, out_size); p.k = group(&a->k, out_size); p.pos = a->pos; p.freq = a->freq;
     p.T = a->T; p.hd = a->hd; p.n_rot = a->n_rot; p.half = a->layout == CLEF_HIP_ROTARY_HALF; p.axes = a->axes;

@@ -517,7 +517,8 @@ bool clef_hip_mx4_sizes(int rows, int K, size_t *code_bytes, size_t *scale_bytes
 /* quantise: x [rows][row] into codes and scales. A block's scale is 2^e, e the least integer from -127 on with max|x| <
  * 7 * 2^e (so that the largest rounds to at most 6), at most 125; a value becomes the nearest code, ties to the one with an even fraction.
  * A block with an infinity or a NaN becomes NaN. values: the reverse, exact in bf16 and f32 (the same fields; x is
- * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity). */
+ * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity).
+ * Codes, scales and x may not overlap. */
 typedef struct {
     int rows, K, type;        /* type: CLEF_HIP_OUT_* of x */
     long row;                 /* row stride of x in elements, a multiple of 8 */
@@ -534,7 +535,7 @@ bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scale
 /* Y[T][N] = X[T][K] . W[N][K]^T (+ residual), W in 4 bits, X in 4 bits (x_codes, x_scales) or in bf16 (x_bf16, its rows x_row
  * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly, and summed
  * in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
- * be Y itself (the same rows), but not overlap it otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W. The sums' order
+ * be Y itself (the same rows), but not overlap it otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W (refused). The sums' order
  * depends on the sizes alone: results do not change from run to run. No workspace. */
 typedef struct {
     int T, N, K, y_type;
@@ -573,7 +574,8 @@ typedef struct {
     int heads;                /* 0: none */
     const void *x;            /* head h of row t starts at x + t * x_row + h * x_head elements */
     void *out;                /* may be x with the same strides; without a norm only the turned dims are then touched. Else no
-                                 output overlaps an input, or the other output */
+                                 output overlaps an input, or the other output (refused; rows
+                                 of different lengths are taken as whole) */
     long x_row, x_head, out_row, out_head;
     const float *norm;        /* [hd] f32, as given (already 1 + w), or NULL */
 } clef_hip_rotary_heads;
