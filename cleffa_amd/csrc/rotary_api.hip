@@ -124,6 +124,7 @@ bool clef_hip_rotary_freqs(int n_rot, double theta, int scaling, double factor, 
     if (!freq) return fail(err, errlen, "rotary: missing freq");
     const double tau = 6.283185307179586476925;
     const double base = scaling == CLEF_HIP_ROTARY_BASE ? theta * pow(factor, (double)n_rot / (n_rot - 2)) : theta;
+    if (!isfinite(base)) return fail(err, errlen, "rotary: theta %g scaled by %g is too large", theta, factor);
     for (int j = 0; j < n_rot / 2; j++) {
         double f = pow(base, -2. * j / n_rot);
         if (scaling == CLEF_HIP_ROTARY_LINEAR) f /= factor;

@@ -37,3 +37,11 @@ def test_output_types():
             r.apply(*args, **kw)
     with pytest.raises(RuntimeError, match="GPU"):
         r.apply(q, q, pos, q_out=half, k_out=half.clone())
+
+
+@pytest.mark.parametrize("n,theta,factor", [(4, 1e7, 1e151), (64, 1e300, 1e9), (4, 1e300, 1e9)])
+def test_a_base_beyond_f64_is_refused(n, theta, factor):
+    """It would make every frequency but the first zero."""
+    with pytest.raises(RuntimeError, match="too large"):
+        Rotary(n, theta=theta, scaling={"kind": "base", "factor": factor}, device="cpu")
+    assert (Rotary(n, theta=1e7, scaling={"kind": "base", "factor": 1e100}, device="cpu").freq > 0).all()
