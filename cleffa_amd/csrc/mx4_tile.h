@@ -74,6 +74,14 @@ __device__ __forceinline__ void lds_wait(u32x4 (&r)[F], unsigned (&s)[2][F]) {
                      "+v"(s[1][4]), "+v"(s[1][5])::"memory");
 }
 
+// Between what lanes write to LDS and what other lanes of the wave read or overwrite of it. The hardware takes a wave's LDS instructions in order,
+// so this costs none: it keeps the compiler from moving them across, which it may where it sees that a lane's own addresses differ.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A wave's outputs, rows t0 .. and columns c0 ..: lane l's accumulators of a 32 x 32 part are columns 8 (e / 4) + 4 (l / 32) + e % 4 of row
 // l % 32. 32 rows at a time go through `mine`, LDS of the wave's own, so that stores take whole lines, past the caches where rows of Y
 // begin at them: 4,096 x 14,336 x 5,120 148 us with ordinary stores, 140 past the caches, which W and X then have to themselves; 2,000 x 6,389
@@ -86,12 +94,14 @@ __device__ __forceinline__ void store_tile(const GemmParams &p, const f32x16 (&a
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         const int t0 = t_first + 32 * i;
+        wave_lds_order();        // the rows before have been read
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 *(f32x4 *)(mine + (lane & 31) * OUT_ROW + (32 * j + 8 * e + 4 * (lane >> 5)) * 4) =
                     f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+        wave_lds_order();
         // V columns a lane, 16 bytes of Y; the columns before N that are fewer come after, one by one
         if (p.y_bf16) {
             constexpr int LANES = WN / 8, ROWS_I = 64 / LANES;    // lanes of a row, rows of an instruction
