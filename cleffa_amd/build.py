@@ -16,7 +16,7 @@ DEPS = SOURCES + BENCH_SOURCES + [ROOT / "csrc" / "attn_kernels.h", ROOT / "csrc
                   ROOT / "csrc" / "attn_vis.h", ROOT / "csrc" / "omni_attn.h", ROOT / "csrc" / "attn_text_f32.h", ROOT / "csrc" / "bf16_ops.h", ROOT / "csrc" / "split32.h", ROOT / "csrc" / "ranges.h",
                   ROOT / "csrc" / "gemm_kernel.h", ROOT / "csrc" / "kv_rows.h", ROOT / "csrc" / "text_ops.h",
                   *(ROOT / "csrc" / f"kv8_{part}.h" for part in ("attn", "pages", "params", "plan")),
-                  *(ROOT / "csrc" / f"mx4_{part}.h" for part in ("gemm", "params", "quant", "rows16", "tile", "wide")), ROOT / "csrc" / "rotary.h", ROOT / "csrc" / "gguf_view.h",
+                  *(ROOT / "csrc" / f"mx4_{part}.h" for part in ("forms", "gemm", "params", "quant", "rows16", "tile", "wide")), ROOT / "csrc" / "rotary.h", ROOT / "csrc" / "gguf_view.h",
                   REPO / "include" / "clef_hip_attn.h"]
 
 

@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include "clef_hip_attn.h"
+#include "mx4_forms.h"
 #include "mx4_gemm.h"
 #include "mx4_params.h"
 #include "mx4_quant.h"
@@ -38,9 +39,6 @@ bool launch_ok(const char *what, char *err, size_t errlen) {
     if (e != hipSuccess) return fail(err, errlen, "%s launch failed: %s", what, hipGetErrorString(e));
     return true;
 }
-
-// The compute units of the chips this library is built for (gfx950): forms are chosen for them.
-constexpr int kCus = 256;
 
 // A launch holds fewer than 2^32 threads: of rows / 16 x K / 512 workgroups of 256, fewer than 2^24.
 bool shape_ok(const char *what, int rows, int K, char *err, size_t errlen) {
@@ -80,50 +78,19 @@ void launch_quantise(const mx4::QuantParams &p, hipStream_t s) {
     hipLaunchKernelGGL(mx4::mx4_quantise_kernel<TYPE>, dim3((unsigned)(mx4::ceil_div(p.rows, mx4::ROWS) * p.kgroups)), dim3(mx4::kQuantThreads), 0, s, p);
 }
 
-// The forms of the product. Where a form's workgroups make no more than one for each CU, its K loop is the time, and the smallest
-// tile wins; else the rounds of workgroups count. Measured in us (three weights in turn, K 6,144 at N 5,120, 5,120 at 14,336):
-//   4 bits, rows forms MT x NT row and column tiles of 16: N 5,120, 16 rows: 1x2 5.1, 2x2 6.0, 1x4 6.3; 32 rows: 2x2 6.2, 1x2 6.7; 64 rows: 2x4 7.0,
-//     1x2 9.0; 128 rows: 4x4 9.7, tiles 64 x 128 10.7; 256 rows: tiles 64 x 128 11.1, 4x4 17.9. N 14,336, 16 rows: 1x4 8.5, 1x1 9.1; 96 rows: tiles
-//     64 x 128 10.7, 4x4 17.9.
-//   bf16 rows: N 5,120, 16 rows: 1x2 7.1, 1x4 9.1; 48 rows: 1x4 9.5, 1x2 11.4; 64 rows: 2x4 12.3, 1x4 14.0; 128 rows: 2x4 of four waves (two workgroups a
-//     CU) 20, of eight 24; tiles of 64 x 256 33 up to 256 rows. N 14,336, 96 rows: 28 and 31, 128 rows 34 and 31.
 template <int MT, int NT>
-long rows_blocks(const mx4::GemmParams &p) {
-    return (long)mx4::ceil_div(mx4::ceil_div(p.N, 16), NT) * mx4::ceil_div(mx4::ceil_div(p.T, 16), MT);
+void launch_rows(const mx4::GemmParams &p, hipStream_t s) {
+    constexpr int W = 8, D = MT == 1 ? 3 : 2;
+    hipLaunchKernelGGL((mx4::mx4_rows_kernel<MT, NT, W, D>), dim3((unsigned)mx4::blocks_of(p.T, p.N, 16 * MT, 16 * NT)), dim3(64 * W), 0, s, p);
 }
-template <int MT, int NT, int W, int D>
-bool launch_rows(const mx4::GemmParams &p, hipStream_t s) {
-    const long blocks = rows_blocks<MT, NT>(p);
-    if (blocks > kCus) return false;
-    hipLaunchKernelGGL((mx4::mx4_rows_kernel<MT, NT, W, D>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
-    return true;
-}
-template <int MT, int NT, int W>
-bool launch_rows16(const mx4::GemmParams &p, hipStream_t s) {
-    const long blocks = rows_blocks<MT, NT>(p);
-    if (blocks > (W == 8 ? kCus : 2 * kCus)) return false;
-    if constexpr (MT == 1) {
-        if (p.T <= 4) {
-            hipLaunchKernelGGL((mx4::mx4_rows16_kernel<1, NT, W, 1>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
-            return true;
-        }
-    }
-    hipLaunchKernelGGL((mx4::mx4_rows16_kernel<MT, NT, W, 4 * MT>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
-    return true;
+template <int MT, int NT, int W, int XF>
+void launch_rows16(const mx4::GemmParams &p, hipStream_t s) {
+    hipLaunchKernelGGL((mx4::mx4_rows16_kernel<MT, NT, W, XF>), dim3((unsigned)mx4::blocks_of(p.T, p.N, 16 * MT, 16 * NT)), dim3(64 * W), 0, s, p);
 }
 
 template <typename C>
-long tiles(const mx4::GemmParams &p) {
-    return (long)mx4::ceil_div(p.N, C::BN) * mx4::ceil_div(p.T, C::BM);
-}
-template <typename C>
 dim3 tile_grid(const mx4::GemmParams &p) {
     return dim3((unsigned)(8 * mx4::ceil_div(mx4::ceil_div(p.N, C::BN), 8) * mx4::ceil_div(p.T, C::BM)));
-}
-// The time of n tiles, two a CU at a time, of which a round takes `full` and one of no more than a CU each `half`.
-float rounds(long n, float half, float full) {
-    const long r = n % (2 * kCus);
-    return (float)(n / (2 * kCus)) * full + (r == 0 ? 0.f : r <= kCus ? half : full);
 }
 template <typename C>
 void launch_tile(const mx4::GemmParams &p, hipStream_t s) {
@@ -135,33 +102,34 @@ void launch_wide(const mx4::GemmParams &p, hipStream_t s) {
 }
 
 void launch4(const mx4::GemmParams &p, hipStream_t s) {
-    using Small = mx4::TileCfg<64, 128, 64, 32, 4, 2>;
-    using Middle = mx4::TileCfg<128, 128, 64, 64, 4, 2>;
-    using Large = mx4::TileCfg<256, 128, 64, 64, 3, 2>;      // eight waves; with four, where each CU has one: 425 x 10,240 x 4,096 17.0 us, with eight 16.0
-    using Square = mx4::TileCfg<256, 256, 128, 64, 4, 1>;    // eight waves, one workgroup a CU
-    if (launch_rows<1, 1, 8, 3>(p, s) || launch_rows<1, 2, 8, 3>(p, s) || launch_rows<2, 2, 8, 2>(p, s) || launch_rows<2, 4, 8, 2>(p, s) ||
-        launch_rows<4, 4, 8, 2>(p, s))
-        return;
-    // rounds of 40 K tiles, us: 256 rows x 14,336 small 15.8, middle 12.8, large 17.2, square 25.0; 512 rows 32, 25, 23, 27; 2,048 rows large 73, square 70;
-    // 4,096 rows 222, 161, 144, 143; 3,000 x 10,240 x 4,096 95, 74, 67, 61; 1,160 x 5,120 x 6,144 27.6, 26.7, 24.0, 31; 2,048 rows 45, 40, 40, 38
-    const float small = rounds(tiles<Small>(p), 10.5f, 16.7f), middle = rounds(tiles<Middle>(p), 13.f, 24.5f), large = rounds(tiles<Large>(p), 20.f, 41.f);
-    const float square = 36.f * (float)((tiles<Square>(p) + kCus - 1) / kCus);
-    if (square < large && square < middle && square < small) launch_tile<Square>(p, s);
-    else if (small <= middle && small <= large) launch_tile<Small>(p, s);
-    else if (middle <= large) launch_tile<Middle>(p, s);
-    else launch_tile<Large>(p, s);
+    switch (mx4::form4(p.T, p.N)) {
+    case mx4::ROWS_1X1: return launch_rows<1, 1>(p, s);
+    case mx4::ROWS_1X2: return launch_rows<1, 2>(p, s);
+    case mx4::ROWS_2X2: return launch_rows<2, 2>(p, s);
+    case mx4::ROWS_2X4: return launch_rows<2, 4>(p, s);
+    case mx4::ROWS_4X4: return launch_rows<4, 4>(p, s);
+    case mx4::TILE_64X128: return launch_tile<mx4::TileCfg<64, 128, 64, 32, 4, 2>>(p, s);
+    case mx4::TILE_128X128: return launch_tile<mx4::TileCfg<128, 128, 64, 64, 4, 2>>(p, s);
+    // eight waves; with four, where each CU has one: 425 x 10,240 x 4,096 17.0 us, with eight 16.0
+    case mx4::TILE_256X128: return launch_tile<mx4::TileCfg<256, 128, 64, 64, 3, 2>>(p, s);
+    // eight waves, one workgroup a CU
+    default: return launch_tile<mx4::TileCfg<256, 256, 128, 64, 4, 1>>(p, s);
+    }
 }
 
 void launch16(const mx4::GemmParams &p, hipStream_t s) {
-    using Small = mx4::WideCfg<64, 256, 64, 64, 2, 2>;      // two workgroups a CU
-    using Large = mx4::WideCfg<128, 256, 64, 128, 2, 1>;    // one
-    if (launch_rows16<1, 1, 8>(p, s) || launch_rows16<1, 2, 8>(p, s) || launch_rows16<1, 4, 8>(p, s) || launch_rows16<2, 4, 8>(p, s) || launch_rows16<2, 4, 4>(p, s))
-        return;
-    // rounds of 40 K tiles, us: 256 rows x 14,336 small 33, large 48; 512 rows 61, 57; 4,096 rows 451, 432
-    const long n = tiles<Large>(p);
-    const float small = rounds(tiles<Small>(p), 31.f, 64.f), large = 58.f * (float)((n + kCus - 1) / kCus);
-    if (small <= large) launch_wide<Small>(p, s);
-    else launch_wide<Large>(p, s);
+    switch (mx4::form16(p.T, p.N)) {
+    case mx4::ROWS16_1X1_FEW: return launch_rows16<1, 1, 8, 1>(p, s);
+    case mx4::ROWS16_1X1: return launch_rows16<1, 1, 8, 4>(p, s);
+    case mx4::ROWS16_1X2_FEW: return launch_rows16<1, 2, 8, 1>(p, s);
+    case mx4::ROWS16_1X2: return launch_rows16<1, 2, 8, 4>(p, s);
+    case mx4::ROWS16_1X4_FEW: return launch_rows16<1, 4, 8, 1>(p, s);
+    case mx4::ROWS16_1X4: return launch_rows16<1, 4, 8, 4>(p, s);
+    case mx4::ROWS16_2X4: return launch_rows16<2, 4, 8, 8>(p, s);
+    case mx4::ROWS16_2X4_W4: return launch_rows16<2, 4, 4, 8>(p, s);
+    case mx4::WIDE_64X256: return launch_wide<mx4::WideCfg<64, 256, 64, 64, 2, 2>>(p, s);      // two workgroups a CU
+    default: return launch_wide<mx4::WideCfg<128, 256, 64, 128, 2, 1>>(p, s);                  // one
+    }
 }
 
 }  // namespace
