@@ -59,7 +59,7 @@ bool runs_ok(const clef_hip_rotary_heads *g, int T, int v, int size, int out_siz
 // Whether outputs have bytes of heads that are read, or of each other; heads turned in place are their own outputs.
 bool overlap(const clef_hip_rotary_args *a, int size, int out_size) {
     const auto heads = [&](const void *p, const clef_hip_rotary_heads &g, long row, long head, long size) {
-        return Heads{(uintptr_t)p, a->T, a->T > 1 ? row * size : 0, g.heads, g.heads > 1 ? head * size : 0, a->hd * size};
+        return Heads{(uintptr_t)p, a->T, g.heads && a->T > 1 ? row * size : 0, g.heads, g.heads > 1 ? head * size : 0, a->hd * size};
     };
     const Heads q = heads(a->q.x, a->q, a->q.x_row, a->q.x_head, size), k = heads(a->k.x, a->k, a->k.x_row, a->k.x_head, size);
     const Heads qo = heads(a->q.out, a->q, a->q.out_row, a->q.out_head, out_size), ko = heads(a->k.out, a->k, a->k.out_row, a->k.out_head, out_size);

@@ -118,3 +118,8 @@ def test_rotary_overlaps(args):
 @pytest.mark.parametrize("over", [dict(x_row=1 << 50), dict(out_row=1 << 50), dict(x_head=1 << 50), dict(out_head=1 << 50, out_row=1 << 50)])
 def test_rotary_too_far_apart(over):
     _refused(_lib.load().clef_hip_rotary, _rotary_args(**over), "too far apart")
+
+
+def test_strides_of_no_heads_do_not_count():
+    a = _pair(k__heads=0, k__x_row=(1 << 63) - 1, k__out_row=(1 << 63) - 1, q__out=P(BASE + 4))
+    _refused(_lib.load().clef_hip_rotary, a, "overlaps")
