@@ -41,8 +41,10 @@ __device__ __forceinline__ void join_waves(const GemmParams &p, const f32x4 (&ac
 }
 
 // Few 4-bit rows: MT x NT tiles of 16 rows and 16 columns a workgroup, whose W waves share the K tiles and add their sums in LDS in a
-// fixed order. Operands come straight from memory, D K tiles ahead. Bound by the latency of the loads in flight: 45 rows x 14,336 x 5,120
-// read 39 MB in 10 us, and 16 rows x 5,120 x 6,144 16.8 MB in 5.1. K split over workgroups too, with sums joined behind, was not faster.
+// fixed order. Operands come straight from memory into D buffers of a K tile each. Nothing holds the loads where they are written: the
+// compiler moves the last buffer's down to their products, so that D - 1 K tiles are in flight, and with D = 2 none behind the second of
+// two. 45 rows x 14,336 x 5,120 read 39 MB in 9.9 us, and 16 rows x 5,120 x 6,144 16.8 MB in 5.1: latency, of the five or six K tiles of a wave one after
+// the other. What deeper or pinned loads would give is not measured.
 template <int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(GemmParams p) {
     __shared__ f32x4 part[W][MT * NT][64];

@@ -66,7 +66,8 @@ __device__ __forceinline__ unsigned quad_max(unsigned m) {
 }
 
 // A workgroup makes 16 rows x 512 columns, each of its four waves a tile of 16 x 128: four loads of 4 rows x 256 bytes, a
-// block's 32 values in four neighbouring lanes. Codes go through LDS, so that a tile's 1 KB is stored in a row.
+// block's 32 values in four neighbouring lanes. Codes go through LDS, so that a tile's 1 KB is stored in a row (written there four
+// to a bank, 3.9e5 conflict clocks on 1.1e5 instructions, behind the memory).
 // Bound by memory: 4,096 x 6,144 f16 values 11.0 us one call behind the other, 5.8 TB/s of what it reads and writes; reading alone takes
 // 8.0. Two row tiles a workgroup, for more loads in flight, took 11.5.
 constexpr int kQuantThreads = 256;

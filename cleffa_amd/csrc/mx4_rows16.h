@@ -63,7 +63,9 @@ __global__ __launch_bounds__(64 * W) void mx4_rows16_kernel(GemmParams p) {
         for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const unsigned base = lds_address(mine) + l16 * 256;
     auto k_tile = [&](Ops &o, int kt, int stage) CLEF_INLINE {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(GROUP) : "memory");     // in flight: the next K tile's
+        // the next K tile's may stay in flight. On every other K tile they do not: the compiler waits for W by a count of its own, which it
+        // takes over the ways around the loop's skip and the loads of X, and that is none.
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(GROUP) : "memory");
         u32x4 x[4 * MT];
         for_each<4>([&](auto J) CLEF_INLINE {
             constexpr int j = decltype(J)::value;

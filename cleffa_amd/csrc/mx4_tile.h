@@ -2,16 +2,18 @@
 //
 // The matrix instruction 32x32x64 takes from lane l 32 codes of row l % 32, block l / 32. Tiles of codes (16 rows x 128) go to
 // LDS as they lie in memory, 1 KB an instruction; a lane's 16 bytes of rows 32 i .. + 31, half h of the K tile, are at
-// 2048 i + 512 h + 1024 (l / 16 % 2) + 256 (l / 32) + 16 (l % 16): 256 bytes in a row for each 16 lanes, so no bank conflicts.
+// 2048 i + 512 h + 1024 (l / 16 % 2) + 256 (l / 32) + 16 (l % 16): 256 bytes in a row for each 16 lanes, all banks once.
 // Scales of four K tiles go to LDS together and from there into a register for each operand, of which the instruction
-// takes a byte. So the loop takes four K tiles at a time, one straight line of code: over branches the compiler would move the
+// takes a byte; those reads, four bytes a lane, meet two ways, rows 16 and on 256 bytes behind the others (counted: 3.4e6 conflict
+// clocks on 6.4e6 LDS instructions of 4,096 x 14,336 x 5,120). So the loop takes four K tiles at a time, one straight line of code: over branches the compiler would move the
 // products behind the waits.
 //
 // Bound by the matrix units and LDS together. A K tile of 256 x 256 is 1,024 clocks of a CU's products; its waves' operands are 96 KB
-// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. 4,096 x 14,336 x 5,120 takes 137 us, 4.4 PFLOP/s: the products
-// alone, on such data, ran at 6.3 in a loop without any loads, the chip at 1.8 of its 2.4 GHz for its power. Tiles of 256 x 128, two
-// workgroups a CU, take 0 to 10% longer (3,000 x 10,240 x 4,096 66.7 us against 60.8), tiles of 128 x 128 161. Four waves of
-// 128 x 128 read a third less of LDS, but nothing runs while they wait: 149 us where eight took 144.
+// of LDS reads and 32 KB of fills, at 128 bytes a clock as many again. The products alone ran at 6.3 PFLOP/s, on such data, in a loop
+// without any loads, the chip at 1.8 of its 2.4 GHz for its power. 4,096 x 14,336 x 5,120 takes 139 to 144 us in tiles of 256 x 128, two
+// workgroups a CU (4.2 to 4.3 PFLOP/s; 149 on one chip), 142 to 149 in tiles of 256 x 256, 162 to 164 in 128 x 128; 3,000 x 10,240 x 4,096 66 to 68
+// in 256 x 128 and 61 to 67 in 256 x 256. Four waves of 128 x 128 read a third less of LDS, but nothing runs while they wait: 149 us where
+// eight took 144.
 #pragma once
 #include <utility>
 
@@ -84,7 +86,7 @@ __device__ __forceinline__ void wave_lds_order() {
 
 // A wave's outputs, rows t0 .. and columns c0 ..: lane l's accumulators of a 32 x 32 part are columns 8 (e / 4) + 4 (l / 32) + e % 4 of row
 // l % 32. 32 rows at a time go through `mine`, LDS of the wave's own, so that stores take whole lines, past the caches where rows of Y
-// begin at them: 4,096 x 14,336 x 5,120 148 us with ordinary stores, 140 past the caches, which W and X then have to themselves; 2,000 x 6,389
+// begin at them: 4,096 x 14,336 x 5,120 148 us with ordinary stores, 140 past the caches (on one chip), which W and X then have to themselves; 2,000 x 6,389
 // x 160, where they do not, 12.3 and 16.6.
 constexpr int out_row(int NT) { return 32 * NT * 4 + 16; }
 template <int MT, int NT>

@@ -7,8 +7,8 @@
 // A code takes a quarter of a value's bytes, so a wave's part of the tile is wide in columns: 64 rows x 128 columns read 16 KB of X
 // and 8 KB of W a K tile.
 //
-// Bound by the matrix units: 4,096 x 14,336 x 5,120 takes 432 us, 1.39 PFLOP/s, where the products alone ran at 1.65 in a loop without
-// any loads and a large library product of 16-bit operands at 1.21. Widening
+// Bound by the matrix units: 4,096 x 14,336 x 5,120 takes 432 to 455 us on different chips, 1.32 to 1.39 PFLOP/s, where the products
+// alone ran at 1.65 in a loop without any loads and library products of 16-bit operands at 1.21 (8,192 cubed) and 1.27 (this one). Widening
 // issues between the products, while the matrix unit works.
 #pragma once
 #include "mx4_tile.h"
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES / 4 * C::PER_CU) void mx4_wide
     auto after = [&](unsigned st) CLEF_INLINE { return st == (STAGES - 1) * C::STAGE_BYTES ? 0u : st + C::STAGE_BYTES; };
     // K tile kt at POS of its group. X of a step is read two steps before, so that after the sixth step nothing more is read of this K
     // tile, and its buffer takes kt + STAGES with the last two steps. Reads stand behind a step's first product and the barrier behind
-    // some of its step's: with reads and barrier ahead of the products 4,096 x 14,336 x 5,120 took 452 us, against 432.
+    // some of its step's: with reads and barrier ahead of the products 4,096 x 14,336 x 5,120 took 452 us, against 432 on the same chip.
     auto k_tile = [&](int kt, auto POS) CLEF_INLINE {
         constexpr int pos = decltype(POS)::value, next = (pos + 1) & 3;
         const unsigned here = stage;

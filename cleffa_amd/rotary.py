@@ -25,7 +25,10 @@ class Rotary:
     a dict of "kind" ("linear", "base" or "parts"), "factor" and for "parts" "original" (the length that the model was
     trained for), "low" and "high" (1 and 32: pairs that turn less over it are stretched, that turn more are kept). magnitude
     multiplies all turned dims (None: 0.1 ln factor + 1 for "parts", else 1). freqs: radians a position of each pair,
-    float64 [n_rot / 2], in place of the formula."""
+    float64 [n_rot / 2], in place of the formula.
+
+    "parts" is linear in the turns of a pair. Checkpoints whose programs make it linear in the pair's index, between rounded
+    borders, need freqs; ones scaled with low 1 and high 4 usually have no magnitude: magnitude=1."""
 
     def __init__(self, n_rot, theta=1e7, layout="half", axes=1, scaling=None, magnitude=None, freqs=None, eps=1e-6, device="cuda"):
         if layout not in _lib.ROTARY_LAYOUTS:

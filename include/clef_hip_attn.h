@@ -516,6 +516,8 @@ bool clef_hip_mx4_sizes(int rows, int K, size_t *code_bytes, size_t *scale_bytes
 
 /* quantise: x [rows][row] into codes and scales. A block's scale is 2^e, e the least integer from -127 on with max|x| <
  * 7 * 2^e (so that the largest rounds to at most 6), at most 125; a value becomes the nearest code, ties to the one with an even fraction.
+ * The format leaves the choice of scales open; its specification's own conversion takes floor(log2 max|x|) - 2 and cuts 6 off from 7 on, so codes that
+ * other programs make differ in the blocks whose largest value has a mantissa from 1.75 on, about a fifth. clef_hip_mx4_pack takes those as they are.
  * A block with an infinity or a NaN becomes NaN. values: the reverse, exact in bf16 and f32 (the same fields; x is
  * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity).
  * Codes, scales and x may not overlap. */
@@ -533,8 +535,8 @@ bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scale
                        void *stream, char *err, size_t errlen);
 
 /* Y[T][N] = X[T][K] . W[N][K]^T (+ residual), W in 4 bits, X in 4 bits (x_codes, x_scales) or in bf16 (x_bf16, its rows x_row
- * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly, and summed
- * in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
+ * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly (but for
+ * what an s above 252, from elsewhere, takes beyond bf16, an infinity there), and summed in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
  * be Y itself (the same rows), but not overlap it otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W (refused). The sums' order
  * depends on the sizes alone: results do not change from run to run. No workspace. */
 typedef struct {
@@ -560,7 +562,8 @@ bool clef_hip_mx4_gemm(const clef_hip_mx4_gemm_args *a, void *stream, char *err,
  *
  * clef_hip_rotary_freqs (host only): freq[j] = f_j / 2 pi, turns a position, in f64. f_j = theta^(-2j / n_rot); scaled for texts
  * `factor` times as long: LINEAR f_j / factor; BASE theta * factor^(n_rot / (n_rot - 2)) for theta; PARTS keep f_j + (1 - keep) f_j /
- * factor, keep = (r - low) / (high - low) within 0 and 1, r = original * f_j / 2 pi the turns over the original length. */
+ * factor, keep = (r - low) / (high - low) within 0 and 1, r = original * f_j / 2 pi the turns over the original length. (A ramp that is linear in the
+ * pair's index between rounded borders, as some checkpoints' programs have it, is another: freq is then the caller's own.) */
 #define CLEF_HIP_ROTARY_NONE 0
 #define CLEF_HIP_ROTARY_LINEAR 1
 #define CLEF_HIP_ROTARY_BASE 2
