@@ -62,11 +62,19 @@ Rows rows_of(const void *p, int n, long row, long values, long size) { return Ro
 bool apart(const clef_hip_mx4_gemm_args *a) {
     return (a->y == a->residual && (a->T == 1 || a->y_row == a->r_row)) || !meet(rows_of(a->y, a->T, a->y_row, a->N, 4), rows_of(a->residual, a->T, a->r_row, a->N, 4));
 }
-// Whether Y has bytes of a matrix's buffers.
+// Whether rows have bytes of a matrix's buffers.
 bool meets_matrix(const Rows &y, const uint8_t *codes, const uint8_t *scales, int rows, int K) {
     const size_t tiles = (size_t)mx4::ceil_div(rows, mx4::ROWS);
     return meets(y, (uintptr_t)codes, (uintptr_t)codes + tiles * mx4::ceil_div(K, mx4::KT) * mx4::TILE_BYTES) ||
            meets(y, (uintptr_t)scales, (uintptr_t)scales + tiles * mx4::ceil_div(K, mx4::KG) * mx4::GROUP_BYTES);
+}
+
+// x of a quantisation or of values: rows not too far apart, and outside of the matrix.
+bool rows_ok(const char *what, const clef_hip_mx4_rows_args *a, char *err, size_t errlen) {
+    const int size = a->type == CLEF_HIP_OUT_F32 ? 4 : 2;
+    if (!span_ok(a->rows, a->row, size)) return fail(err, errlen, "%s: rows too far apart", what);
+    if (meets_matrix(rows_of(a->x, a->rows, a->row, a->K, size), a->codes, a->scales, a->rows, a->K)) return fail(err, errlen, "%s: x overlaps codes or scales", what);
+    return true;
 }
 
 mx4::Matrix matrix(const uint8_t *codes, const uint8_t *scales, int rows, int K) {
@@ -152,6 +160,7 @@ bool clef_hip_mx4_quantise(const clef_hip_mx4_rows_args *a, void *stream, char *
     if (a->rows == 0) return true;
     if (!matrix_ok("quantise:", a->codes, a->scales, err, errlen)) return false;
     if (!a->x || !aligned16(a->x)) return fail(err, errlen, "quantise: x must be a 16-byte aligned device pointer");
+    if (!rows_ok("quantise", a, err, errlen)) return false;
     mx4::QuantParams p{a->x, nullptr, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row, false};
     if (a->type == CLEF_HIP_OUT_BF16) launch_quantise<mx4::X_BF16>(p, (hipStream_t)stream);
     else if (a->type == CLEF_HIP_OUT_F16) launch_quantise<mx4::X_F16>(p, (hipStream_t)stream);
@@ -167,6 +176,7 @@ bool clef_hip_mx4_values(const clef_hip_mx4_rows_args *a, void *stream, char *er
     if (a->rows == 0) return true;
     if (!matrix_ok("values:", a->codes, a->scales, err, errlen)) return false;
     if (!a->x || !aligned16(a->x)) return fail(err, errlen, "values: x must be a 16-byte aligned device pointer");
+    if (!rows_ok("values", a, err, errlen)) return false;
     mx4::QuantParams p{nullptr, a->x, a->codes, a->scales, a->rows, a->K, mx4::ceil_div(a->K, mx4::KT), mx4::ceil_div(a->K, mx4::KG), a->row,
                        whole_lines(a->x, a->row * (a->type == CLEF_HIP_OUT_F32 ? 4 : 2))};
     const dim3 grid((unsigned)((long)mx4::ceil_div(a->rows, mx4::ROWS) * p.kgroups)), block(mx4::kQuantThreads);
@@ -181,6 +191,9 @@ bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scale
     if (rows == 0) return true;
     if (!matrix_ok("pack:", codes, scales, err, errlen)) return false;
     if (!flat_codes || !flat_scales || !aligned16(flat_codes)) return fail(err, errlen, "pack: flat codes must be a 16-byte aligned device pointer, flat scales a device pointer");
+    if (meets_matrix(rows_of(flat_codes, 1, 0, (long)rows * (K / 2), 1), codes, scales, rows, K) ||
+        meets_matrix(rows_of(flat_scales, 1, 0, (long)rows * (K / mx4::BLOCK), 1), codes, scales, rows, K))
+        return fail(err, errlen, "pack: flat codes or scales overlap the matrix");
     mx4::PackParams p{flat_codes, flat_scales, codes, scales, rows, K, mx4::ceil_div(K, mx4::KT), mx4::ceil_div(K, mx4::KG)};
     const size_t blocks = (size_t)rows * (to_flat ? K / mx4::BLOCK : 16 * p.kgroups);
     const dim3 grid((unsigned)((blocks + 255) / 256));

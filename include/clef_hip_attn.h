@@ -520,7 +520,7 @@ bool clef_hip_mx4_sizes(int rows, int K, size_t *code_bytes, size_t *scale_bytes
  * other programs make differ in the blocks whose largest value has a mantissa from 1.75 on, about a fifth. clef_hip_mx4_pack takes those as they are.
  * A block with an infinity or a NaN becomes NaN. values: the reverse, exact in bf16 and f32 (the same fields; x is
  * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity).
- * Codes, scales and x may not overlap. */
+ * x may not overlap codes or scales (refused). */
 typedef struct {
     int rows, K, type;        /* type: CLEF_HIP_OUT_* of x */
     long row;                 /* row stride of x in elements, a multiple of 8 */

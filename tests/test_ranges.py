@@ -123,3 +123,27 @@ def test_rotary_too_far_apart(over):
 def test_strides_of_no_heads_do_not_count():
     a = _pair(k__heads=0, k__x_row=(1 << 63) - 1, k__out_row=(1 << 63) - 1, q__out=P(BASE + 4))
     _refused(_lib.load().clef_hip_rotary, a, "overlaps")
+
+
+# 20 rows of 160 values, 240 apart, at BASE; codes 2 x 2 KB, scales 2 x 256 bytes
+@pytest.mark.parametrize("fn", ["quantise", "values"])
+@pytest.mark.parametrize("type_,codes,scales", [
+    (0, BASE, 1 << 24), (0, 1 << 24, BASE), (0, BASE - 4096 + 16, 1 << 24), (0, 1 << 24, BASE + 2 * (19 * 240 + 160) - 16), (2, BASE + 4 * (19 * 240 + 160) - 16, 1 << 24),
+    (2, 1 << 24, BASE + 4 * 160), (0, BASE + 320, 1 << 24)])
+def test_rows_over_their_matrix(fn, type_, codes, scales):
+    a = _lib.Mx4RowsArgs(20, 160, type_, 240, P(BASE), P(codes), P(scales))
+    _refused(getattr(_lib.load(), "clef_hip_mx4_" + fn), a, "overlaps")
+
+
+@pytest.mark.parametrize("fn", ["quantise", "values"])
+def test_rows_too_far_apart(fn):
+    _refused(getattr(_lib.load(), "clef_hip_mx4_" + fn), _lib.Mx4RowsArgs(20, 160, 0, 1 << 50, P(BASE), P(1 << 24), P(1 << 25)), "too far apart")
+
+
+@pytest.mark.parametrize("flat_codes,flat_scales", [(BASE, 1 << 24), (1 << 24, BASE), (BASE - 20 * 80 + 16, 1 << 24), (BASE + 4080, 1 << 24), (1 << 24, BASE + 4095), (BASE + 8192, 1 << 24),
+                                                    (1 << 24, BASE + 8192 + 511)])
+@pytest.mark.parametrize("to_flat", [0, 1])
+def test_pack_over_its_matrix(flat_codes, flat_scales, to_flat):
+    err = ctypes.create_string_buffer(256)
+    assert not _lib.load().clef_hip_mx4_pack(20, 160, flat_codes, flat_scales, BASE, BASE + 8192, to_flat, None, err, 256)
+    assert "overlap" in err.value.decode()
