@@ -81,15 +81,6 @@ def _on(stream):
     return _HERE if stream is None else torch.cuda.stream(stream)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(stream):
-    """Where a call makes its results, planes and tables: in the memory of the stream that it runs on. Memory of the current one torch
-    could have taken from, or give to, work there that the call does not wait for."""
-    return _HERE if stream is None else torch.cuda.stream(stream)
-
-
 _ERR = ctypes.c_char * 512
 
 

@@ -516,8 +516,9 @@ bool clef_hip_mx4_sizes(int rows, int K, size_t *code_bytes, size_t *scale_bytes
 
 /* quantise: x [rows][row] into codes and scales. A block's scale is 2^e, e the least integer from -127 on with max|x| <
  * 7 * 2^e (so that the largest rounds to at most 6), at most 125; a value becomes the nearest code, ties to the one with an even fraction.
- * The format leaves the choice of scales open; its specification's own conversion takes floor(log2 max|x|) - 2 and cuts 6 off from 7 on, so codes that
- * other programs make differ in the blocks whose largest value has a mantissa from 1.75 on, about a fifth. clef_hip_mx4_pack takes those as they are.
+ * The format leaves the choice of scales open; its specification's own conversion takes e = floor(log2 max|x|) - 2 and makes 6 of what lies
+ * above, so codes that other programs make differ in the blocks whose largest value has a mantissa from 1.75 on, about a fifth.
+ * clef_hip_mx4_pack takes those as they are.
  * A block with an infinity or a NaN becomes NaN. values: the reverse, exact in bf16 and f32 (the same fields; x is
  * written, type CLEF_HIP_OUT_BF16 or _F32; what an s above 252, from elsewhere, takes beyond bf16 becomes an infinity).
  * x may not overlap codes or scales (refused). */
@@ -536,8 +537,9 @@ bool clef_hip_mx4_pack(int rows, int K, uint8_t *flat_codes, uint8_t *flat_scale
 
 /* Y[T][N] = X[T][K] . W[N][K]^T (+ residual), W in 4 bits, X in 4 bits (x_codes, x_scales) or in bf16 (x_bf16, its rows x_row
  * elements apart). Products of 4-bit values are exact and summed in f32; with X in bf16 W is widened to bf16, exactly (but for
- * what an s above 252, from elsewhere, takes beyond bf16, an infinity there), and summed in f32. y_type CLEF_HIP_GEMM_Y_BF16 or _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may
- * be Y itself (the same rows), but not overlap it otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W (refused). The sums' order
+ * what an s above 252, from elsewhere, takes beyond bf16, an infinity there), and summed in f32. y_type CLEF_HIP_GEMM_Y_BF16 or
+ * _F32; residual [T][r_row] f32 (or NULL; f32 Y only) is added before the store and may be Y itself (the same rows), but not overlap it
+ * otherwise. Rows of W with a NaN block give NaN columns, rows of X NaN rows. Y may not overlap X or W (refused). The sums' order
  * depends on the sizes alone: results do not change from run to run. No workspace. */
 typedef struct {
     int T, N, K, y_type;
